@@ -31,6 +31,17 @@ extern "C" {
 #define MXQ_RD 2 /* "rd": truncate the 15-bit mantissa */
 #define MXQ_RZ 3 /* "rz": truncate the 23-bit mantissa */
 
+/* activation functions of an epilogue */
+#define MXQ_ACT_NONE 0
+#define MXQ_ACT_RELU 1
+#define MXQ_ACT_GELU 2      /* 0.5 z (1 + erf(z / sqrt 2)) */
+#define MXQ_ACT_GELU_TANH 3 /* 0.5 z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) */
+#define MXQ_ACT_SILU 4      /* z / (1 + exp(-z)) */
+/* what an epilogue does with its second operand */
+#define MXQ_EXTRA_NONE 0
+#define MXQ_EXTRA_MULTIPLY 1
+#define MXQ_EXTRA_ADD 2
+
 #define MXQ_OK 0
 #define MXQ_EINVAL -1   /* bad argument (null pointer, bad dtype, bad format, n % block_size != 0) */
 #define MXQ_ELAUNCH -2  /* the CUDA launch failed; see mxq_last_cuda_error() */
@@ -337,6 +348,43 @@ int64_t mxq_mx_linear_static_capacity(void);
 int mxq_mx_linear_static(const void* x, int x_dtype, int64_t M, int64_t K, int x_exp_bits, int x_frac_bits,
                          const uint8_t* w_codes, const uint8_t* w_sf, int w_hw_format, int w_tile_rows,
                          int64_t N, void* out, int out_dtype, const void* bias, int* status, void* stream);
+
+/*
+ * ---- Products with an epilogue, one weight or one per group of rows (no counterpart in the reference) ----
+ *
+ *   out[i, :] = act(Q(x[src(i), :]) * dequant(W[g])^T + bias[g]) (* | +) extra[i, :]      for offsets[g] <= i < offsets[g + 1]
+ *
+ * Q quantises to MXFP (32-element blocks along K, is_finite elements of x_exp_bits / x_frac_bits, any rounding mode);
+ * products, bias, activation and the second operand in fp32, one rounding to the output's type.
+ * mxq_mx_pack_experts re-encodes the weights once: scales / elements of a [groups, N, K] tensor blocked along K, as
+ * mxq_mxfp_extract writes them, into hw_codes (groups * N * K bytes; half of that with `nibbles`, 32-byte aligned) and
+ * hw_sf (groups * mxq_mx_sf_bytes(N, K, MXQ_OPERAND_A, 0) bytes).  `nibbles`: keep E2M1 codes two per byte for an E2M1
+ * activation (K % 256 == 0), which then runs on the 4-bit x 4-bit tensor-core kind.
+ */
+int mxq_mx_pack_experts(const uint8_t* scales, const uint8_t* elements, int64_t groups, int64_t N, int64_t K,
+                        int exp_bits, int frac_bits, int nibbles, uint8_t* hw_codes, uint8_t* hw_sf,
+                        int* hw_format, void* stream);
+/* Largest number of groups (1024). */
+int mxq_mx_max_groups(void);
+/*
+ * x [rows_in, K], out and extra [rows, N], bias [groups, N], all of x_dtype; bias and extra may be NULL.
+ *   row_index : rows source rows (int32, or int64 with index64), src(i) = row_index[i]; an index outside x stands for a row
+ *               of zeros.  NULL: src(i) = i, rows == rows_in.
+ *   offsets   : groups + 1 row numbers (int32, or int64 with offsets64).  They are read on the device; values are
+ *               clamped to [0, rows] and one that lies below an earlier one counts as that one, so that no content
+ *               of the array reaches outside the buffers.  NULL: one group of all rows (groups == 1).
+ *   zero_rest : rows of out outside every group are set to zero; otherwise they are left as they are.
+ *   scratch   : 256-byte aligned, at least mxq_mx_grouped_scratch_bytes(rows_in, rows, K) bytes, of this call alone.
+ * `extra` may be the same buffer as `out`.  K % 32 == 0, w_hw_format / w_codes / w_sf from mxq_mx_pack_experts.
+ * `status` as for mxq_mx_gemm.
+ */
+int64_t mxq_mx_grouped_scratch_bytes(int64_t rows_in, int64_t rows, int64_t K);
+int mxq_mx_grouped_linear(const void* x, int x_dtype, int64_t rows_in, int64_t rows, int64_t K, int x_exp_bits,
+                          int x_frac_bits, int x_round_mode, const void* row_index, int index64,
+                          const uint8_t* w_codes, const uint8_t* w_sf, int w_hw_format, int64_t groups, int64_t N,
+                          const void* offsets, int offsets64, void* out, const void* bias, int activation,
+                          const void* extra, int extra_mode, int zero_rest, void* scratch, int64_t scratch_bytes,
+                          int* status, void* stream);
 
 #ifdef __cplusplus
 }

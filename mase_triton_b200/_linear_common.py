@@ -2,8 +2,12 @@
 
 from __future__ import annotations
 
+import math
 import re
 from typing import NamedTuple
+
+import torch
+from torch import Tensor
 
 _LAYER_RE = re.compile(r"X(q?)W(q?)")
 
@@ -29,3 +33,18 @@ def parse_layer_type(layer_type: str) -> LinearKind:
 def check_backend(backend: str) -> None:
     if backend not in ("separate", "fused"):
         raise NotImplementedError(f"backend {backend!r} not implemented")
+
+
+def activate(z: Tensor, activation: str | None) -> Tensor:
+    """The activation of a linear's epilogue, on fp32 values."""
+    if activation is None:
+        return z
+    if activation == "relu":
+        return torch.relu(z)
+    if activation == "gelu":
+        return 0.5 * z * (1 + torch.erf(z * math.sqrt(0.5)))
+    if activation == "gelu_tanh":
+        return 0.5 * z * (1 + torch.tanh(math.sqrt(2 / math.pi) * (z + 0.044715 * z * z * z)))
+    if activation == "silu":
+        return z * torch.sigmoid(z)
+    raise ValueError(f"activation {activation!r} is not known")

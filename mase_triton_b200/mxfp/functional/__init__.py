@@ -6,5 +6,6 @@ from .cast import (  # noqa: F401
     permute_for_dequantize,
     quantize_dequantize,
 )
+from .grouped import mxfp_grouped_linear  # noqa: F401
 from .linear import mxfp_linear, parse_mxfp_linear_type  # noqa: F401
 from .matmul import mxfp_matmul  # noqa: F401

@@ -15,9 +15,10 @@ import torch
 from torch import Tensor
 
 from ... import _lib, tc_linear
-from ..._linear_common import check_backend, parse_layer_type
+from ..._linear_common import activate, check_backend, parse_layer_type
 from ..meta import MXFPMeta, MXFPTensorMeta
 from .. import gemm as _gemm
+from .. import grouped as _grouped
 from .cast import compose_mxfp_tensor, quantize_dequantize
 
 LayerType = Literal["XWB", "XWBq", "XWqB", "XWqBq", "XqWB", "XqWBq", "XqWqB", "XqWqBq"]
@@ -38,6 +39,14 @@ def block_scaled_ok(x: Tensor, x_meta: MXFPMeta | None, w_tensor_meta: MXFPTenso
     shape = tuple(w_tensor_meta.shape)
     return (len(shape) == 2 and w_tensor_meta.block_dim in (1, -1) and _gemm.supported(w_tensor_meta.meta) and _gemm.supported(x_meta)
             and x.is_cuda and x.dtype in _lib.DTYPE_ID and x.shape[-1] == shape[1] and shape[1] % 32 == 0 and x.numel() > 0)
+
+
+def require_epilogue(x: Tensor, x_meta: MXFPMeta | None, w_tensor_meta: MXFPTensorMeta | None, both_quantised: bool) -> None:
+    """Raise for a fused linear whose product cannot take an epilogue (an empty ``x`` can)."""
+    probe = x if x.numel() > 0 or x.ndim == 0 else x.new_empty(1, x.shape[-1])
+    if not both_quantised or not block_scaled_ok(probe, x_meta, w_tensor_meta):
+        raise NotImplementedError("backend='fused' takes an activation, multiplier or residual where activation and weight are quantised with "
+                                  "32-element blocks along in_features and is_finite elements, on CUDA; use backend='separate'")
 
 
 def _fused_linear(x: Tensor, x_meta: MXFPMeta | None, w: Tensor | None, w_scales: Tensor | None, w_elements: Tensor | None,
@@ -82,6 +91,34 @@ def _fused_linear(x: Tensor, x_meta: MXFPMeta | None, w: Tensor | None, w_scales
     return tc_linear.dense_linear(x, compose_mxfp_tensor(w_scales, w_elements, w_tensor_meta).contiguous(), bias)
 
 
+def linear_with_epilogue(x: Tensor, x_meta: MXFPMeta, w: "_grouped.PackedExperts", bias: Tensor | None, activation: str | None,
+                         multiplier: Tensor | None, residual: Tensor | None) -> Tensor:
+    """``act(Q(x) @ W^T + bias) (* multiplier | + residual)`` in one product, both operands quantised up to the tensor cores."""
+    lead = x.shape[:-1]
+
+    def flat(t: Tensor | None, name: str) -> Tensor | None:
+        if t is not None and tuple(t.shape) != (*lead, w.N):
+            raise ValueError(f"{name} has to have the result's shape {(*lead, w.N)}: got {tuple(t.shape)}")
+        return None if t is None else t.reshape(-1, w.N)
+
+    y = _grouped.grouped_linear(x.reshape(-1, w.K), x_meta, w, None, None if bias is None else bias.to(x.dtype).reshape(1, -1), activation,
+                                flat(multiplier, "multiplier"), flat(residual, "residual"))
+    return y.reshape(*lead, w.N)
+
+
+def _separate_epilogue(y: Tensor, activation: str | None, multiplier: Tensor | None, residual: Tensor | None) -> Tensor:
+    extra, mode = _grouped.epilogue_operand(multiplier, residual)
+    if extra is not None and (extra.shape != y.shape or extra.dtype != y.dtype):
+        raise ValueError(f"{'multiplier' if mode == _grouped.EXTRA_MULTIPLY else 'residual'} has to be {y.dtype} {tuple(y.shape)}: "
+                         f"got {extra.dtype} {tuple(extra.shape)}")
+    z = activate(y.float(), activation)
+    if mode == _grouped.EXTRA_MULTIPLY:
+        z = z * extra.float()
+    elif mode == _grouped.EXTRA_ADD:
+        z = z + extra.float()
+    return z.to(y.dtype)
+
+
 def mxfp_linear(
     x: Tensor,
     x_meta: MXFPMeta | None,
@@ -95,9 +132,25 @@ def mxfp_linear(
     b_tensor_meta: MXFPTensorMeta | None,
     layer_type: LayerType,
     backend: Literal["separate", "fused"],
+    activation: str | None = None,
+    multiplier: Tensor | None = None,
+    residual: Tensor | None = None,
 ) -> Tensor:
+    """The reference's ``mxfp_linear``, with an epilogue that it lacks: ``act(y) * multiplier`` or ``act(y) + residual`` for the
+    linear's result ``y``.  ``activation``: ``"relu"``, ``"gelu"``, ``"gelu_tanh"``, ``"silu"`` or ``None``; ``multiplier`` / ``residual`` have
+    the result's shape and ``x``'s dtype.  ``backend="fused"`` takes the epilogue where activation and weight stay quantised
+    (``XqWq*``): products, bias and epilogue in fp32, rounded once, the weight packed in every call (``MXFPLinearPTQ``
+    keeps it packed).  ``backend="separate"`` rounds the linear's result first, as it does without an epilogue."""
     kind = parse_layer_type(layer_type)
     check_backend(backend)
+    _grouped.check_activation(activation)
+    epilogue = activation is not None or multiplier is not None or residual is not None
+    if backend == "fused" and epilogue:
+        bias = b if not kind.b_quantised else (compose_mxfp_tensor(b_scales, b_elements, b_tensor_meta) if b is not None else None)
+        require_epilogue(x, x_meta, w_tensor_meta, kind.x_quantised and kind.w_quantised)
+        n, k = tuple(w_tensor_meta.shape)
+        return linear_with_epilogue(x, x_meta, _grouped.pack_experts(w_scales, w_elements, 1, n, k, w_tensor_meta.meta, x_meta), bias,
+                                    activation, multiplier, residual)
     if backend == "fused":
         # the reference only uses bias codes when a plain bias is passed as well (then the codes win); the fused route
         # hands them on as codes so that the block-scaled GEMM can decode them in its epilogue
@@ -111,4 +164,5 @@ def mxfp_linear(
     if kind.x_quantised:
         x = quantize_dequantize(x, block_dim=-1, mxfp_meta=x_meta)       # same bits as extract + compose
     weight = compose_mxfp_tensor(w_scales, w_elements, w_tensor_meta) if kind.w_quantised else w
-    return torch.nn.functional.linear(x, weight, bias)
+    y = torch.nn.functional.linear(x, weight, bias)
+    return _separate_epilogue(y, activation, multiplier, residual) if epilogue else y

@@ -68,6 +68,10 @@ class MXFPLinearPTQ(PTQLinearBase):
         self.register_buffer("_tc_codes", None, persistent=False)
         self.register_buffer("_tc_sf", None, persistent=False)
         self._tc_info = None          # (versions of the code tensors it was built from, hw_format, tile_rows)
+        # the same weight for the product with an epilogue, where it is the left operand
+        self.register_buffer("_row_codes", None, persistent=False)
+        self.register_buffer("_row_sf", None, persistent=False)
+        self._row_info = None         # (versions, hw_format)
 
         if "Wq" in layer_type:
             if w_scales is None:
@@ -109,6 +113,19 @@ class MXFPLinearPTQ(PTQLinearBase):
         n, k = self.w_tensor_meta.shape
         return _gemm.PackedOperand(self._tc_codes, self._tc_sf, self._tc_info[1], n, k, _gemm.OPERAND_B, self._tc_info[2])
 
+    def row_weight(self):
+        """The quantised weight as the product with an epilogue reads it (``mxfp.grouped``), kept on the module and rebuilt
+        like :meth:`tensor_core_weight`."""
+        from . import grouped as _grouped
+
+        versions = (self.w_elements._version, self.w_scales._version)
+        n, k = self.w_tensor_meta.shape
+        if self._row_codes is None or self._row_info is None or self._row_info[0] != versions or self._row_codes.device != self.w_elements.device:
+            p = _grouped.pack_experts(self.w_scales.data, self.w_elements.data, 1, n, k, self.w_tensor_meta.meta, self.x_mxfp_meta)
+            self._row_codes, self._row_sf = p.codes, p.sf
+            self._row_info = (versions, p.hw_format)
+        return _grouped.PackedExperts(self._row_codes, self._row_sf, self._row_info[1], 1, n, k)
+
     def export_packed(self) -> dict:
         """A ``torch.save``-able dict holding this layer with its element codes bit-packed to their true width
         (4 / 6 / 8 bits) and its tensor metas; see ``mase_triton_b200.mxfp.storage``."""
@@ -124,7 +141,10 @@ class MXFPLinearPTQ(PTQLinearBase):
         return import_packed(record, device, backend)
 
     @torch.no_grad()
-    def forward(self, input: Tensor) -> Tensor:
+    def forward(self, input: Tensor, activation: str | None = None, multiplier: Tensor | None = None, residual: Tensor | None = None) -> Tensor:
+        """``act(linear(input)) * multiplier`` or ``act(linear(input)) + residual``; see ``mxfp_linear``."""
+        if activation is not None or multiplier is not None or residual is not None:
+            return self._forward_with_epilogue(input, activation, multiplier, residual)
         if (self.backend == "fused" and "Xq" in self.layer_type and "Wq" in self.layer_type
                 and MXFP_F.linear.block_scaled_ok(input, self.x_mxfp_meta, self.w_tensor_meta)):
             # both operands stay quantised: the module's own tensor-core form of the weight, no per-call packing.
@@ -137,6 +157,17 @@ class MXFPLinearPTQ(PTQLinearBase):
             w=self.weight, w_scales=self.w_scales, w_elements=self.w_elements, w_tensor_meta=self.w_tensor_meta,
             b=self.bias, b_scales=self.b_scales, b_elements=self.b_elements, b_tensor_meta=self.b_tensor_meta,
             layer_type=self.layer_type, backend=self.backend,
+        )
+
+    def _forward_with_epilogue(self, input: Tensor, activation: str | None, multiplier: Tensor | None, residual: Tensor | None) -> Tensor:
+        if self.backend == "fused":
+            MXFP_F.linear.require_epilogue(input, self.x_mxfp_meta, self.w_tensor_meta, "Xq" in self.layer_type and "Wq" in self.layer_type)
+            return MXFP_F.linear.linear_with_epilogue(input, self.x_mxfp_meta, self.row_weight(), self.bias, activation, multiplier, residual)
+        return MXFP_F.mxfp_linear(
+            x=input, x_meta=self.x_mxfp_meta,
+            w=self.weight, w_scales=self.w_scales, w_elements=self.w_elements, w_tensor_meta=self.w_tensor_meta,
+            b=self.bias, b_scales=self.b_scales, b_elements=self.b_elements, b_tensor_meta=self.b_tensor_meta,
+            layer_type=self.layer_type, backend=self.backend, activation=activation, multiplier=multiplier, residual=residual,
         )
 
     def pack_input(self, input: Tensor):
@@ -190,3 +221,80 @@ class MXFPLinearPTQ(PTQLinearBase):
                    dtype=getattr(torch, w_tensor_meta.dtype), device=torch.device(w_tensor_meta.device),
                    w_scales=w_scales, w_elements=w_elements, w_tensor_meta=w_tensor_meta,
                    b_scales=b_scales, b_elements=b_elements, b_tensor_meta=b_tensor_meta)
+
+
+class MXFPGroupedLinearPTQ(PTQLinearBase):
+    """One quantised linear per group of rows (the experts of a layer); the reference has no counterpart.
+
+    ``w_scales`` ``[groups*out*in/32, 1]`` and ``w_elements`` ``[groups*out*in/32, 32]`` are uint8 Parameters holding a
+    ``[groups, out_features, in_features]`` weight (blocks along ``in_features``), ``bias`` is ``[groups, out_features]``.
+    The activation is quantised in every call, both operands stay quantised up to the tensor cores.
+    """
+
+    _code_tensors = ("w_scales", "w_elements")
+    _meta_follows = {"w_tensor_meta": "w_scales"}
+
+    def __init__(self, w_scales: Tensor, w_elements: Tensor, w_tensor_meta: MXFPTensorMeta, bias: Tensor | None, x_mxfp_meta: MXFPMeta):
+        super().__init__()
+        from . import grouped as _grouped
+
+        self.groups, self.out_features, self.in_features = MXFP_F.grouped.expert_shape(w_tensor_meta)
+        _grouped.check_formats(x_mxfp_meta, w_tensor_meta.meta, self.in_features)
+        if bias is not None and tuple(bias.shape) != (self.groups, self.out_features):
+            raise ValueError(f"bias has to have the shape {(self.groups, self.out_features)}: got {tuple(bias.shape)}")
+        self.x_mxfp_meta = x_mxfp_meta
+        self.w_scales, self.w_elements = self._frozen(w_scales), self._frozen(w_elements)
+        self.w_tensor_meta = w_tensor_meta
+        self.bias = None if bias is None else self._frozen(bias)
+        # the weights as the kernel reads them, built on first use; they follow .to() and stay out of state_dict()
+        self.register_buffer("_row_codes", None, persistent=False)
+        self.register_buffer("_row_sf", None, persistent=False)
+        self._row_info = None         # (versions of the code tensors it was built from, hw_format)
+
+    @classmethod
+    def from_weight(cls, weight: Tensor, bias: Tensor | None, x_mxfp_meta: MXFPMeta, w_mxfp_meta: MXFPMeta):
+        """Quantise ``weight [groups, out_features, in_features]``."""
+        if weight.ndim != 3:
+            raise ValueError(f"the weight has to be [groups, out_features, in_features]: got {tuple(weight.shape)}")
+        with torch.no_grad():
+            w_scales, w_elements, w_tensor_meta = MXFP_F.extract_mxfp_components(weight, block_dim=-1, mxfp_meta=w_mxfp_meta)
+            return cls(w_scales, w_elements, w_tensor_meta, None if bias is None else bias.detach().clone(), x_mxfp_meta)
+
+    @classmethod
+    def from_linears(cls, layers: list[nn.Linear], x_mxfp_meta: MXFPMeta, w_mxfp_meta: MXFPMeta):
+        """Quantise the linears of a layer's experts (same sizes, all with a bias or none)."""
+        biases = [layer.bias for layer in layers]
+        if any(b is None for b in biases) and not all(b is None for b in biases):
+            raise ValueError("either all linears have a bias or none")
+        with torch.no_grad():
+            return cls.from_weight(torch.stack([layer.weight for layer in layers]), None if biases[0] is None else torch.stack(biases), x_mxfp_meta, w_mxfp_meta)
+
+    @classmethod
+    def from_quantized(cls, w_scales: Tensor, w_elements: Tensor, w_tensor_meta: MXFPTensorMeta, bias: Tensor | None, x_mxfp_meta: MXFPMeta):
+        """Rebuild a layer from stored codes (tensor metas are not part of ``state_dict``)."""
+        return cls(w_scales, w_elements, w_tensor_meta, bias, x_mxfp_meta)
+
+    def row_weight(self):
+        """The weights as the kernel reads them, rebuilt when the code tensors were written, moved by ``.to()``."""
+        from . import grouped as _grouped
+
+        versions = (self.w_elements._version, self.w_scales._version)
+        if self._row_codes is None or self._row_info is None or self._row_info[0] != versions or self._row_codes.device != self.w_elements.device:
+            p = _grouped.pack_experts(self.w_scales.data, self.w_elements.data, self.groups, self.out_features, self.in_features,
+                                      self.w_tensor_meta.meta, self.x_mxfp_meta)
+            self._row_codes, self._row_sf = p.codes, p.sf
+            self._row_info = (versions, p.hw_format)
+        return _grouped.PackedExperts(self._row_codes, self._row_sf, self._row_info[1], self.groups, self.out_features, self.in_features)
+
+    @torch.no_grad()
+    def forward(self, input: Tensor, offsets: Tensor, activation: str | None = None, multiplier: Tensor | None = None,
+                residual: Tensor | None = None, row_index: Tensor | None = None, out: Tensor | None = None) -> Tensor:
+        """``mxfp_grouped_linear`` with this layer's weights."""
+        from . import grouped as _grouped
+
+        bias = None if self.bias is None else self.bias.to(input.dtype)
+        return _grouped.grouped_linear(input, self.x_mxfp_meta, self.row_weight(), offsets, bias, activation, multiplier, residual, row_index, out)
+
+    def extra_repr(self) -> str:
+        return (f"groups={self.groups}, in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}, "
+                f"w_mxfp_meta={self.w_tensor_meta.meta}, x_mxfp_meta={self.x_mxfp_meta}")
