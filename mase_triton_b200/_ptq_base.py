@@ -9,6 +9,7 @@ because ``compose_*`` dispatches on the meta's device string
 
 from __future__ import annotations
 
+import torch
 from torch import nn
 
 from .utils.qlayer import ChangeDtypeError
@@ -22,9 +23,17 @@ class PTQLinearBase(nn.Module):
     in_features: int
     out_features: int
 
+    # the quantised weight as the products with an epilogue read it (mxfp.grouped), and the versions of the codes it was
+    # built from; built on first use
+    _row_weight = None
+
+    def __getstate__(self):
+        return self.__dict__ | {"_row_weight": None}          # a copy counts its tensors' versions anew
+
     def _apply(self, fn, recurse=True):
         before = {name: getattr(self, name).dtype for name in self._code_tensors if getattr(self, name) is not None}
         result = super()._apply(fn, recurse)
+        self._row_weight = None
         for name, dtype in before.items():
             now = getattr(self, name).dtype
             if now != dtype:
@@ -37,4 +46,8 @@ class PTQLinearBase(nn.Module):
 
     @staticmethod
     def _frozen(t):
+        if t.is_inference():
+            # what a layer lays out once is rebuilt when a tensor's version changes, which inference tensors do not count
+            with torch.inference_mode(False):
+                t = t.clone()
         return nn.Parameter(t, requires_grad=False)

@@ -9,9 +9,8 @@
 // The right operand's width is free in steps of 16, so a ragged group is cut into tiles of equal width and at most 15
 // rows of padding, and one row costs a tile of 16 and not one of 128.  What that asks for:
 //   * the rows' codes are loaded by TMA in boxes of 64 and 16 rows from the row the group begins at, whatever it is;
-//   * the rows' scales lie in memory as one 32-bit word (four blocks) per row and 128 elements of K, the words of
-//     consecutive rows side by side; a warp gathers those of a tile into the 512-byte chunks that tcgen05.cp expects,
-//     so that no layout depends on where the groups begin;
+//   * the rows' scales are written by the quantiser in the 512-byte chunks that tcgen05.cp expects, chunks per row tile:
+//     the quantiser finds its row's group and tile by itself;
 //   * an accumulator holds a feature per lane and a row per column: bias is one value per lane, and the 32 lanes of a
 //     warp read the second operand and write the result 32 consecutive features at a time.
 // Which rows belong to which group is read on the device: no size but the upper bounds is known to the host.
@@ -19,10 +18,9 @@
 // Operand layout in HBM:
 //   weights: codes [groups * N, K] (bytes, or nibbles for E2M1 x E2M1), scales per group as for a left operand of mxq_gemm.cu
 //            ([ceil(N / 256)][ceil(K / 128)][2][512] bytes);
-//   rows:    codes [rows, K], scales [ceil(K / 128)][pitch] words, pitch = rows rounded up to 4.
-#include <cmath>
-
-#include "mxq_codec.h"
+//   rows:    codes [rows, K], scales [tile slot][ceil(K / 128)][chunks][512] bytes.  With tiles of at most `width` rows, tile t of a
+//            group that begins at row f has slot f / width + group + t: no two tiles share one, and no sum over the groups before is needed.
+#include "mxq_device.cuh"
 #include "mxq_tc.cuh"
 
 namespace mxq {
@@ -32,7 +30,7 @@ using namespace tc;
 
 constexpr int MAX_GROUPS = MX_MAX_GROUPS;
 constexpr int EPI_WARPS = 8;                     // two per TMEM lane quadrant
-constexpr int FIRST_EPI_WARP = 4;                // warps 0..2: TMA producer, MMA issuer, scale gatherer
+constexpr int FIRST_EPI_WARP = 4;                // warps 0, 1, 3: weight copies, MMA issuer, row copies
 constexpr int THREADS = (FIRST_EPI_WARP + EPI_WARPS) * 32;
 
 enum : int { X_NONE = MXQ_EXTRA_NONE, X_MUL = MXQ_EXTRA_MULTIPLY, X_ADD = MXQ_EXTRA_ADD };
@@ -56,32 +54,15 @@ template <int MH_, int BT_, int STAGES_, bool MXF4_> struct Cfg {
     static_assert(ACC_STRIDE == BT || SFW_COL + SF_STEPS * 8 <= ACC_STRIDE, "tensor memory");
     static_assert(SFX_COL + SF_STEPS * 8 <= 512, "tensor memory");
     static_assert(STAGE_BYTES % 1024 == 0, "the 128-byte swizzle repeats every 1024 bytes");
-    static constexpr int TABLE_BYTES = 2 * (MAX_GROUPS + 1) * 4;
-    static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + 256 + TABLE_BYTES;
+    // behind the ring: barriers, the group table, the epilogue's 2 KiB per warp
+    static constexpr int TABLE_END = (256 + 2 * (MAX_GROUPS + 1) * 4 + 15) / 16 * 16;
+    static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + TABLE_END + EPI_WARPS * 2048;
     static_assert(SMEM_BYTES <= 232448, "more shared memory than a CTA can have");
 };
 using Wide = Cfg<2, 240, 3, false>;
 using WideFp4 = Cfg<2, 240, 3, true>;
 using Narrow = Cfg<1, 128, 6, false>;
-using NarrowFp4 = Cfg<1, 128, 6, true>;
-
-struct Params {
-    const uint8_t* w_sf;         // weight scales, w_sf_group bytes per group
-    int64_t w_sf_group;
-    const uint32_t* x_sf;        // row scales
-    int64_t x_sf_pitch;          // words per 128-element step of K
-    void* out;
-    const void* bias;            // [groups, N] or null
-    const void* extra;           // [rows, N] or null
-    const void* offsets;         // [groups + 1], or null: one group of all rows
-    int offsets64;
-    int rows, groups, N, K;
-    int width;                   // rows per tile at most (a multiple of 16, <= BT)
-    int act, extra_mode;
-    int zero_rest;               // write zeros into the rows that belong to no group
-    uint32_t idesc;              // instruction descriptor without the width
-    int* status;
-};
+using NarrowFp4 = Cfg<1, 128, 5, true>;
 
 template <int DT> struct Elem;
 template <> struct Elem<MXQ_F32> { typedef float T; };
@@ -93,6 +74,26 @@ __device__ __forceinline__ float widen(__half v) { return __half2float(v); }
 __device__ __forceinline__ void narrow(float v, float& o) { o = v; }
 __device__ __forceinline__ void narrow(float v, __nv_bfloat16& o) { o = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void narrow(float v, __half& o) { o = __float2half_rn(v); }
+
+// Four consecutive features of a row as one 8-byte (fp32: 16-byte) access; `left` of the row's features begin here, `vector`: rows and
+// base are aligned to four.  Held as words: a struct of four 16-bit values is copied member by member, i.e. in 2-byte accesses.
+template <class T> struct Words { typedef uint2 V; };
+template <> struct Words<float> { typedef uint4 V; };
+template <class T> union Four {
+    typename Words<T>::V w;
+    T v[4];
+    __device__ __forceinline__ Four() {}
+};
+template <class T> __device__ __forceinline__ void load_four(const T* at, int left, int vector, Four<T>& o) {
+    if (vector) { if (left > 0) o.w = *reinterpret_cast<const typename Words<T>::V*>(at); return; }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) if (k < left) o.v[k] = at[k];
+}
+template <class T> __device__ __forceinline__ void store_four(T* at, int left, int vector, const Four<T>& o) {
+    if (vector) { if (left > 0) *reinterpret_cast<typename Words<T>::V*>(at) = o.w; return; }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) if (k < left) at[k] = o.v[k];
+}
 
 // z * sigmoid(2u) is 0.5 z (1 + tanh u); exp overflows to Inf for very negative arguments and the quotient is then 0
 __device__ __forceinline__ float sigmoid_times(float z, float a) { return __fdividef(z, 1.0f + __expf(-a)); }
@@ -108,9 +109,12 @@ __device__ __forceinline__ float activate(float z, int act) {
 
 // where a unit of work lies: features [f0, f0 + FEATURES) of group g for rows [row, row + rows)
 struct Unit {
-    int g, f0, ftile, row, rows;
+    int g, f0, ftile, row, rows, slot;
     __device__ __forceinline__ uint32_t padded() const { return (uint32_t)(rows + 15) & ~15u; }
 };
+
+// Rows per tile of a group of n rows cut into tt = ceil(n / width) tiles: equal, a multiple of 16, at most `width`; the last tile is never empty.
+__device__ __forceinline__ int tile_rows(int n, int tt) { return ((n + tt - 1) / tt + 15) & ~15; }
 
 // The group table (tile counts summed over the groups, first rows) and the walk over the units of one CTA.
 struct Walk {
@@ -123,39 +127,97 @@ struct Walk {
         const int tt = tiles[g + 1] - tiles[g], begin = first[g], n = first[g + 1] - begin;
         int ti, fi;
         tile_coords(u - tiles[g] * ftiles, tt, ftiles, ti, fi);
-        // tiles of equal width: ceil(n / tt) rounded up to 16 is at most `width`, and the last tile is never empty
-        const int w = ((n + tt - 1) / tt + 15) & ~15;
-        return Unit{g, fi * features, fi, begin + ti * w, min(w, n - ti * w)};
+        const int w = tile_rows(n, tt);
+        return Unit{g, fi * features, fi, begin + ti * w, min(w, n - ti * w), begin / width + g + ti};
     }
 };
 
-__device__ __forceinline__ int offset_at(const Params& p, int i) {
-    if (p.offsets == nullptr) return i == 0 ? 0 : p.rows;
-    const int64_t v = p.offsets64 ? reinterpret_cast<const long long*>(p.offsets)[i] : (int64_t)reinterpret_cast<const int*>(p.offsets)[i];
-    return (int)min(max(v, (int64_t)0), (int64_t)p.rows);
-}
+// The rows of a call and how they are grouped.
+struct Groups {
+    const void* offsets;         // [groups + 1], or null: one group of all rows
+    int offsets64, rows, groups;
+    int width;                   // rows per tile at most (a multiple of 16)
+    __device__ __forceinline__ int offset(int i) const {
+        if (offsets == nullptr) return i == 0 ? 0 : rows;
+        const int64_t v = offsets64 ? reinterpret_cast<const long long*>(offsets)[i] : (int64_t)reinterpret_cast<const int*>(offsets)[i];
+        return (int)min(max(v, (int64_t)0), (int64_t)rows);
+    }
+};
 
 // One warp: first[i] = the largest of offsets[0 .. i] (offsets that fall back leave an empty group and never an overlap),
 // tiles[i] = row tiles of the groups before i.
-__device__ __forceinline__ void build_table(const Params& p, int* tiles, int* first, int lane) {
+__device__ __forceinline__ void build_table(const Groups& g, int* tiles, int* first, int lane) {
     int high = 0, sum = 0;
-    for (int base = 0; base <= p.groups; base += 32) {
+    for (int base = 0; base <= g.groups; base += 32) {
         const int i = base + lane;
-        int v = i <= p.groups ? offset_at(p, i) : 0;
+        int v = i <= g.groups ? g.offset(i) : 0;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) { const int up = __shfl_up_sync(~0u, v, o); if (lane >= o) v = max(v, up); }
         v = max(v, high);
         const int before = __shfl_up_sync(~0u, v, 1);
         // rows of group i - 1, which the running sum at i counts
-        int t = (i == 0 || i > p.groups) ? 0 : ((v - (lane == 0 ? high : before)) + p.width - 1) / p.width;
+        int t = (i == 0 || i > g.groups) ? 0 : ((v - (lane == 0 ? high : before)) + g.width - 1) / g.width;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) { const int up = __shfl_up_sync(~0u, t, o); if (lane >= o) t += up; }
         t += sum;
-        if (i <= p.groups) { first[i] = v; tiles[i] = t; }
+        if (i <= g.groups) { first[i] = v; tiles[i] = t; }
         high = __shfl_sync(~0u, v, 31);
         sum = __shfl_sync(~0u, t, 31);
     }
 }
+
+// Where the scales of one row lie: its tile's slot and its row in the tile.
+struct Place {
+    int slot, r;
+    __device__ __forceinline__ Place() : slot(-1), r(0) {}
+    __device__ __forceinline__ Place(const Groups& g, int group, int begin, int end, int row) {
+        const int n = end - begin, w = tile_rows(n, (n + g.width - 1) / g.width), t = (row - begin) / w;
+        slot = begin / g.width + group + t;
+        r = row - begin - t * w;
+    }
+    // byte of K block kb: chunk r / 128 of its 128-element step, (r % 32) * 16 + (r % 128 / 32) * 4 + kb % 4 within
+    __device__ __forceinline__ int64_t at(int kb, int KT128, int chunks) const {
+        return (((int64_t)slot * KT128 + (kb >> 2)) * chunks + (r >> 7)) * 512 + (r & 31) * 16 + ((r & 127) >> 5) * 4 + (kb & 3);
+    }
+};
+
+// The whole CTA: place of one row, slot -1 for a row of no group.  The group is the first whose end lies behind the row (in the
+// running maximum of the offsets, that is the first offset behind it), its begin the largest offset up to there.
+__device__ __forceinline__ Place find_row(const Groups& g, int row, int* s_two) {
+    if (g.offsets == nullptr) return Place(g, 0, 0, g.rows, row);
+    if (threadIdx.x == 0) { s_two[0] = g.groups; s_two[1] = 0; }
+    __syncthreads();
+    int group = g.groups;
+    for (int e = threadIdx.x; e < g.groups && group == g.groups; e += blockDim.x) if (g.offset(e + 1) > row) group = e;
+    group = __reduce_min_sync(~0u, group);
+    if ((threadIdx.x & 31) == 0) atomicMin(&s_two[0], group);
+    __syncthreads();
+    group = s_two[0];
+    if (group == g.groups) return Place();
+    int begin = 0;
+    for (int e = threadIdx.x; e <= group; e += blockDim.x) begin = max(begin, g.offset(e));
+    begin = __reduce_max_sync(~0u, begin);
+    if ((threadIdx.x & 31) == 0) atomicMax(&s_two[1], begin);
+    __syncthreads();
+    begin = s_two[1];
+    return begin > row ? Place() : Place(g, group, begin, g.offset(group + 1), row);
+}
+
+struct Params {
+    const uint8_t* w_sf;         // weight scales, w_sf_group bytes per group
+    int64_t w_sf_group;
+    const uint8_t* x_sf;         // row scales
+    void* out;
+    const void* bias;            // [groups, N] or null
+    const void* extra;           // [rows, N] or null
+    Groups rows;
+    int N, K;
+    int act, extra_mode;
+    int zero_rest;               // write zeros into the rows that belong to no group
+    int vector;                  // out, extra and their rows are aligned to four elements
+    uint32_t idesc;              // instruction descriptor without the width
+    int* status;
+};
 
 template <class C, int DT>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -178,7 +240,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) { mbar_init(full_bar(s), 2); mbar_init(empty_bar(s), 1); }      // full: the copies and the gathered scales
+        for (int s = 0; s < STAGES; ++s) { mbar_init(full_bar(s), 2); mbar_init(empty_bar(s), 1); }      // full: weight copies, row copies
         for (int a = 0; a < 2; ++a) { mbar_init(accum_full(a), 1); mbar_init(accum_empty(a), EPI_WARPS); }
         mbar_init(drain_bar, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -188,7 +250,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    if (warp == 3) build_table(p, tiles, first, lane);
+    if (warp == 3) build_table(p.rows, tiles, first, lane);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -196,11 +258,17 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 
     const int KT = (p.K + C::K_STEP - 1) / C::K_STEP, KT128 = (p.K + 127) / 128;
     const int ftiles = (p.N + C::FEATURES - 1) / C::FEATURES;
-    Walk walk(tiles, first, p.groups, ftiles, p.width);
+    Walk walk(tiles, first, p.rows.groups, ftiles, p.rows.width);
     auto halves_of = [&](const Unit& t) { return MH == 2 && p.N - t.f0 > 128 ? 2 : 1; };
 
-    if (warp == 0) {
-        // ---------------- TMA producer ----------------
+    // The kernel before this one quantises the rows.  It lets this one start when everything before it has completed, so that
+    // all but its own output may be read at once: the weights are on their way while the rows are quantised.
+    // (The kernel behind this one may come up too; it waits for this one's end before it touches memory.)
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (warp != 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    if (warp == 0 || warp == 3) {
+        // ---------------- copies: weights and their scales (warp 0), rows (warp 3) ----------------
         bool ok = true;
         uint32_t it = 0;
         for (int u = blockIdx.x; u < walk.total && ok; u += gridDim.x) {
@@ -210,21 +278,30 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             const uint8_t* sf = p.w_sf + (size_t)t.g * p.w_sf_group +
                                 (MH == 2 ? (size_t)t.ftile * KT128 * 1024 : (size_t)(t.ftile >> 1) * KT128 * 1024 + (t.ftile & 1) * 512);
             const int w_row = t.g * p.N + t.f0;
-            const uint32_t tx = (uint32_t)halves * (16384u + C::SF_STEPS * 512u) + n * 128u;
+            const uint8_t* x_sf = p.x_sf + (size_t)t.slot * KT128 * (C::X_CHUNKS * 512);
+            const uint32_t x_chunks = n > 128 ? 2 : 1;
             for (int kt = 0; kt < KT && ok; ++kt, ++it) {
                 const int s = it % STAGES;
                 if (it >= STAGES) ok = mbar_wait(empty_bar(s), ((it / STAGES) & 1) ^ 1, p.status, ST_PRODUCER_TIMEOUT);
                 if (!ok) break;
                 if (lane == 0) {
                     const uint32_t st = ring + s * C::STAGE_BYTES;
-                    mbar_expect_tx(full_bar(s), tx);
-                    for (int h = 0; h < halves; ++h) tma_load_2d(st + h * 16384, &map_w, kt * C::K_STEP, w_row + h * 128, full_bar(s));
-                    uint32_t r = 0;
-                    for (; r + 64 <= n; r += 64) tma_load_2d(st + C::W_BYTES + r * 128, &map_x64, kt * C::K_STEP, t.row + r, full_bar(s));
-                    for (; r < n; r += 16) tma_load_2d(st + C::W_BYTES + r * 128, &map_x16, kt * C::K_STEP, t.row + r, full_bar(s));
+                    if (warp == 0) {
+                        mbar_expect_tx(full_bar(s), (uint32_t)halves * (16384u + C::SF_STEPS * 512u));
+                        for (int h = 0; h < halves; ++h) tma_load_2d(st + h * 16384, &map_w, kt * C::K_STEP, w_row + h * 128, full_bar(s));
 #pragma unroll
-                    for (int c = 0; c < C::SF_STEPS; ++c)
-                        bulk_load(st + C::W_BYTES + C::X_BYTES + c * C::SF_STEP_BYTES, sf + (size_t)(kt * C::SF_STEPS + c) * 1024, halves * 512, full_bar(s));
+                        for (int c = 0; c < C::SF_STEPS; ++c)
+                            bulk_load(st + C::W_BYTES + C::X_BYTES + c * C::SF_STEP_BYTES, sf + (size_t)(kt * C::SF_STEPS + c) * 1024, halves * 512, full_bar(s));
+                    } else {
+                        mbar_expect_tx(full_bar(s), n * 128u + C::SF_STEPS * x_chunks * 512u);
+                        uint32_t r = 0;
+                        for (; r + 64 <= n; r += 64) tma_load_2d(st + C::W_BYTES + r * 128, &map_x64, kt * C::K_STEP, t.row + r, full_bar(s));
+                        for (; r < n; r += 16) tma_load_2d(st + C::W_BYTES + r * 128, &map_x16, kt * C::K_STEP, t.row + r, full_bar(s));
+#pragma unroll
+                        for (int c = 0; c < C::SF_STEPS; ++c)
+                            bulk_load(st + C::W_BYTES + C::X_BYTES + c * C::SF_STEP_BYTES + MH * 512, x_sf + (size_t)(kt * C::SF_STEPS + c) * (C::X_CHUNKS * 512),
+                                      x_chunks * 512u, full_bar(s));
+                    }
                 }
                 __syncwarp();
             }
@@ -295,46 +372,16 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             __syncwarp();
             mbar_wait(drain_bar, 0, nullptr, 0);
         }
-    } else if (warp == 2) {
-        // ---------------- scales of the rows: words of consecutive rows -> chunks ----------------
-        // chunk c of a tile: rows 128c .. 128c + 127, the word of row r at (r % 32) * 16 + (r / 32) * 4: lane l owns rows l, l + 32, ...
-        bool ok = true;
-        uint32_t it = 0;
-        for (int u = blockIdx.x; u < walk.total && ok; u += gridDim.x) {
-            const Unit t = walk.at(u, C::FEATURES);
-            const int chunks = C::X_CHUNKS == 2 && t.rows > 128 ? 2 : 1;
-            for (int kt = 0; kt < KT && ok; ++kt, ++it) {
-                const int s = it % STAGES;
-                uint32_t w[C::SF_STEPS * C::X_CHUNKS][4];
-#pragma unroll
-                for (int c = 0; c < C::SF_STEPS; ++c) {
-                    const uint32_t* src = p.x_sf + (size_t)(kt * C::SF_STEPS + c) * p.x_sf_pitch;
-#pragma unroll
-                    for (int ch = 0; ch < C::X_CHUNKS; ++ch)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int r = ch * 128 + j * 32 + lane;
-                            w[c * C::X_CHUNKS + ch][j] = r < t.rows ? __ldcg(src + t.row + r) : 0x7F7F7F7Fu;
-                        }
-                }
-                if (it >= STAGES) ok = mbar_wait(empty_bar(s), ((it / STAGES) & 1) ^ 1, p.status, ST_PRODUCER_TIMEOUT);
-                if (!ok) break;
-                uint8_t* dst = ring_ptr + s * C::STAGE_BYTES + C::W_BYTES + C::X_BYTES + MH * 512;
-#pragma unroll
-                for (int c = 0; c < C::SF_STEPS; ++c)
-                    for (int ch = 0; ch < chunks; ++ch) {
-                        const uint32_t* v = w[c * C::X_CHUNKS + ch];
-                        *reinterpret_cast<uint4*>(dst + c * C::SF_STEP_BYTES + ch * 512 + lane * 16) = make_uint4(v[0], v[1], v[2], v[3]);
-                    }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(full_bar(s));
-            }
-        }
     } else if (warp >= FIRST_EPI_WARP) {
         // ---------------- epilogue ----------------
+        // A warp takes 16 rows x 32 features at a time: tensor memory (a feature per lane) -> its own 2 KiB of shared memory
+        // -> four consecutive features per lane, 8 lanes a row: loads of the second operand and stores are whole 64-byte
+        // (fp32: 128-byte) segments.  The second operand of the next 16 rows is requested before the current ones are worked on, that of a
+        // tile's first ones before the accumulator is complete.
         typedef typename Elem<DT>::T T;
         const int q = warp & 3, side = (warp - FIRST_EPI_WARP) >> 2;      // lane quadrant; the two warps of one take 16-row chunks in turn
+        const int er = lane >> 3, ef = q * 32 + (lane & 7) * 4;           // this lane's row (of every four) and first feature
+        float* slot = reinterpret_cast<float*>(ring_ptr + STAGES * C::STAGE_BYTES + C::TABLE_END) + (warp - FIRST_EPI_WARP) * 512;
         T* out = reinterpret_cast<T*>(p.out);
         const T* extra = reinterpret_cast<const T*>(p.extra);
         bool ok = true;
@@ -343,47 +390,77 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             const Unit t = walk.at(u, C::FEATURES);
             const int halves = halves_of(t);
             const int buf = MH == 1 ? (int)(count & 1u) : 0;
+            const int chunks = (t.rows + 15) >> 4;
+            Four<T> e[4];
+            auto request = [&](int h, int c) {
+                if (p.extra_mode == X_NONE) return;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = c * 16 + i * 4 + er, f = t.f0 + h * 128 + ef;
+                    if (r < t.rows) load_four(extra + (size_t)(t.row + r) * p.N + f, p.N - f, p.vector, e[i]);
+                }
+            };
+            if (side < chunks) request(0, side);
             ok = mbar_wait(accum_full(buf), MH == 1 ? (count >> 1) & 1 : count & 1, p.status, ST_EPILOGUE_TIMEOUT);
             tc_fence_after();
             if (!ok) break;
-            const int chunks = (t.rows + 15) >> 4;
             for (int h = 0; h < MH; ++h) {
                 const int a = MH == 1 ? buf : h;
-                const int f = t.f0 + h * 128 + q * 32 + lane;
-                const bool live = h < halves && f < p.N;
-                const float b = (p.bias != nullptr && live) ? widen(reinterpret_cast<const T*>(p.bias)[(size_t)t.g * p.N + f]) : 0.0f;
-                if (h < halves) {
+                const int f = t.f0 + h * 128 + ef;
+                const bool reads = h < halves && side < chunks;
+                float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (reads && p.bias != nullptr) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) if (f + i < p.N) bias[i] = widen(reinterpret_cast<const T*>(p.bias)[(size_t)t.g * p.N + f + i]);
+                }
+                if (reads) {
                     for (int c = side; c < chunks; c += 2) {
                         uint32_t r[32];
                         tmem_ld_32x32b_x16(tmem + ((uint32_t)(q * 32) << 16) + a * C::ACC_STRIDE + c * 16, r);
                         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                        const int n = min(16, t.rows - c * 16);
-                        const size_t at = (size_t)(t.row + c * 16) * p.N + f;
-                        T e[16];
-#pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            if (p.extra_mode != X_NONE && live && j < n) e[j] = extra[at + (size_t)j * p.N];
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            if (!live || j >= n) continue;
-                            float y = activate(__uint_as_float(r[j]) + b, p.act);
-                            if (p.extra_mode == X_MUL) y *= widen(e[j]);
-                            else if (p.extra_mode == X_ADD) y += widen(e[j]);
-                            T o;
-                            narrow(y, o);
-                            out[at + (size_t)j * p.N] = o;
+                        if (c + 2 >= chunks) {                               // the last read of this accumulator: hand it back
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(accum_empty(a));
                         }
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) slot[j * 32 + lane] = __uint_as_float(r[j]);
+                        __syncwarp();
+                        Four<T> now[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) now[i].w = e[i].w;
+                        if (c + 2 < chunks) request(h, c + 2);
+                        else if (h + 1 < halves) request(h + 1, side);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float4 v = reinterpret_cast<const float4*>(slot)[i * 32 + lane];
+                            const int row = c * 16 + i * 4 + er;
+                            if (row < t.rows) {
+                                float y[4] = {v.x, v.y, v.z, v.w};
+                                Four<T> o;
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) {
+                                    y[k] = activate(y[k] + bias[k], p.act);
+                                    if (p.extra_mode == X_MUL) y[k] *= widen(now[i].v[k]);
+                                    else if (p.extra_mode == X_ADD) y[k] += widen(now[i].v[k]);
+                                    narrow(y[k], o.v[k]);
+                                }
+                                store_four(out + (size_t)(t.row + row) * p.N + f, p.N - f, p.vector, o);
+                            }
+                        }
+                        __syncwarp();
                     }
+                } else {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(accum_empty(a));
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(accum_empty(a));
             }
         }
         if (p.zero_rest) {
             // rows before the first group and behind the last one
-            const int lo = first[0], hi = first[p.groups];
-            const int64_t rest = (int64_t)(lo + p.rows - hi) * p.N;
+            const int lo = first[0], hi = first[p.rows.groups];
+            const int64_t rest = (int64_t)(lo + p.rows.rows - hi) * p.N;
             for (int64_t i = (int64_t)blockIdx.x * (EPI_WARPS * 32) + (threadIdx.x - FIRST_EPI_WARP * 32); i < rest; i += (int64_t)gridDim.x * (EPI_WARPS * 32)) {
                 const int64_t before = (int64_t)lo * p.N;
                 narrow(0.0f, out[i < before ? i : i - before + (int64_t)hi * p.N]);
@@ -407,22 +484,32 @@ struct CodeTables {
     uint32_t bad[8];        // bit c: reference code c is one that the hardware reads as Inf / NaN
 };
 
+// Operand of the product: codes, scale chunks, chunks per 128-element step.
+struct RowOperand {
+    uint8_t *codes, *sf;
+    int K, chunks, nibbles;
+};
+
 // One thread per row and 32-element block, padding blocks of the last 128 elements included (scale 2^0; the copies fill their
 // codes with zeros).  A row index outside x gives a row of zeros.
 __global__ void __launch_bounds__(256) pack_rows_kernel(const uint8_t* __restrict__ scales, const uint8_t* __restrict__ elements,
-                                                        const void* __restrict__ row_index, int index64, int64_t rows_in, int64_t rows,
-                                                        int K, int nibbles, uint8_t* __restrict__ codes, uint8_t* __restrict__ sf, int64_t sf_pitch,
-                                                        const __grid_constant__ CodeTables t) {
+                                                        const void* __restrict__ row_index, int index64, int64_t rows_in, const Groups g,
+                                                        const RowOperand o_, const __grid_constant__ CodeTables t) {
     __shared__ uint8_t s_plain[256], s_halved[256];
+    __shared__ int s_tiles[MAX_GROUPS + 1], s_first[MAX_GROUPS + 1];
     s_plain[threadIdx.x] = t.plain[threadIdx.x];
     s_halved[threadIdx.x] = t.halved[threadIdx.x];
+    if (threadIdx.x < 32) build_table(g, s_tiles, s_first, threadIdx.x);
     __syncthreads();
-    const int blocks = (K + 127) / 128 * 4;
+    const int K = o_.K, blocks = (K + 127) / 128 * 4;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= rows * blocks) return;
-    const int64_t row = i / blocks;
-    const int kb = (int)(i - row * blocks);
-    uint8_t* sf_at = sf + ((int64_t)(kb >> 2) * sf_pitch + row) * 4 + (kb & 3);
+    if (i >= (int64_t)g.rows * blocks) return;
+    const int row = (int)(i / blocks), kb = (int)(i - (int64_t)row * blocks);
+    if (row < s_first[0] || row >= s_first[g.groups]) return;
+    int lo = 0, hi = g.groups;                           // the last group that begins at or before the row
+    while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (s_first[mid] <= row) lo = mid; else hi = mid; }
+    uint8_t* codes = o_.codes;
+    uint8_t* sf_at = o_.sf + Place(g, lo, s_first[lo], s_first[lo + 1], row).at(kb, (K + 127) / 128, o_.chunks);
     if (kb * 32 >= K) { *sf_at = 127; return; }
     int64_t src = row;
     if (row_index != nullptr)
@@ -436,11 +523,11 @@ __global__ void __launch_bounds__(256) pack_rows_kernel(const uint8_t* __restric
         scale = scales[src * (K / 32) + kb];
     }
     const uint8_t* cb = reinterpret_cast<const uint8_t*>(c);
-    if (nibbles) {
+    if (o_.nibbles) {
         uint32_t o[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
         for (int j = 0; j < 32; ++j) o[j >> 3] |= (uint32_t)(cb[j] & 0xFu) << (4 * (j & 7));
-        *reinterpret_cast<uint4*>(codes + row * (K / 2) + kb * 16) = make_uint4(o[0], o[1], o[2], o[3]);
+        *reinterpret_cast<uint4*>(codes + (int64_t)row * (K / 2) + kb * 16) = make_uint4(o[0], o[1], o[2], o[3]);
         *sf_at = (uint8_t)scale;
         return;
     }
@@ -452,10 +539,153 @@ __global__ void __launch_bounds__(256) pack_rows_kernel(const uint8_t* __restric
     uint8_t* ob = reinterpret_cast<uint8_t*>(o);
 #pragma unroll
     for (int j = 0; j < 32; ++j) ob[j] = lut[cb[j]];
-    uint4* to = reinterpret_cast<uint4*>(codes + row * K + kb * 32);
+    uint4* to = reinterpret_cast<uint4*>(codes + (int64_t)row * K + kb * 32);
     to[0] = o[0];
     to[1] = o[1];
     *sf_at = (uint8_t)((any_bad && scale < 255u) ? scale + 1u : scale);
+}
+
+// One pass from x to the operand (built-in round-to-nearest formats, 16-byte aligned rows): 8 elements per lane, the 4 lanes of a
+// block agree on its maximum by shuffles, every lane derives the scale, quantises (the dequantised quotient in fp32, as the
+// fused quantise-dequantise kernel forms it) and converts to the hardware's codes, which is exact.  A block with a value that
+// the hardware's format lacks is stored as (scale + 1, elements / 2).  One CTA per row segment: the row is looked up once.
+// OUT: the operand's format, 0 = E4M3 bytes, 1 = E5M2 bytes, 5 = E2M1 nibbles.
+// Bound by memory (x read once, gathered rows mostly from L2) and integer issue about equally.
+constexpr int QUANT_ACCESSES = 2;                // accesses of 8 elements per lane
+template <class KIn, class F, int OUT>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restrict__ x, const void* __restrict__ row_index, int index64, int64_t rows_in,
+                                                            const Groups g, const RowOperand o_, int segments, int early) {
+    __shared__ int s_two[2];
+    // everything before this kernel has completed; then the product may start: until it waits for this kernel it only reads what is older
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (early) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const F f{};
+    constexpr int BYTES = 8 * KIn::size;
+    const int K = o_.K;
+    const int row = (int)(blockIdx.x / (unsigned)segments);
+    const int first = ((int)(blockIdx.x % (unsigned)segments) * QUANT_ACCESSES * (int)blockDim.x + (int)threadIdx.x) * 8;
+    int64_t src = row;
+    if (row_index != nullptr)
+        src = index64 ? reinterpret_cast<const long long*>(row_index)[row] : (int64_t)reinterpret_cast<const int*>(row_index)[row];
+    const bool there = src >= 0 && src < rows_in;                            // a row index outside x gives a row of zeros
+    const char* from = reinterpret_cast<const char*>(x) + src * K * KIn::size;
+    uint32_t raw[QUANT_ACCESSES][BYTES / 4];
+#pragma unroll
+    for (int a = 0; a < QUANT_ACCESSES; ++a) {
+        const int k = first + a * (int)blockDim.x * 8;
+#pragma unroll
+        for (int i = 0; i < BYTES / 16; ++i) {
+            const uint4 v = there && k < K ? __ldg(reinterpret_cast<const uint4*>(from + (int64_t)k * KIn::size) + i) : make_uint4(0, 0, 0, 0);
+            raw[a][4 * i] = v.x; raw[a][4 * i + 1] = v.y; raw[a][4 * i + 2] = v.z; raw[a][4 * i + 3] = v.w;
+        }
+    }
+    const Place place = find_row(g, row, s_two);
+    if (place.slot < 0) return;
+#pragma unroll
+    for (int a = 0; a < QUANT_ACCESSES; ++a) {
+        const int k = first + a * (int)blockDim.x * 8;
+        uint32_t b[8], amax = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (KIn::size == 4) b[i] = raw[a][i];
+            else b[i] = KIn::to_bits(i & 1 ? raw[a][i >> 1] >> 16 : raw[a][i >> 1] & 0xFFFFu);
+            amax = max(amax, b[i] & 0x7FFFFFFFu);
+        }
+        amax = max(amax, __shfl_xor_sync(~0u, amax, 1));
+        amax = max(amax, __shfl_xor_sync(~0u, amax, 2));
+        uint32_t sbyte = 0;
+        const uint32_t header = block_header(amax, f);                       // 2^-se, the scale byte, and whether the block holds Inf / NaN
+        sbyte = (header >> 8) & 0xFFu;
+        const float inv = __uint_as_float(header & 0x7F800000u);
+        const bool special = header & 1u;
+        float v[8];
+        bool bad = false;
+        constexpr float hw_max = OUT == 0 ? 448.0f : OUT == 1 ? 57344.0f : 6.0f;
+        constexpr float fmt_max = F{}.eb() == 4 ? 480.0f : F{}.eb() == 5 ? 114688.0f : 0.0f;     // the formats whose largest value the hardware lacks
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t qb = mx_quotient_bits(b[i], inv);
+            const uint32_t y = special ? 0u : qdq_mag_bits(qb, f);
+            if constexpr (fmt_max > hw_max) bad |= __uint_as_float(y) > hw_max;
+            v[i] = __uint_as_float(y | (qb & 0x80000000u));
+        }
+        if constexpr (fmt_max > hw_max) {
+            uint32_t any = bad ? 1u : 0u;
+            any |= __shfl_xor_sync(~0u, any, 1);
+            any |= __shfl_xor_sync(~0u, any, 2);
+            if (any) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] *= 0.5f;
+                sbyte += sbyte < 255u ? 1u : 0u;
+            }
+        }
+        if (special) sbyte = 255u;                                           // NaN to the tensor cores, whatever the codes
+        uint32_t o[2] = {0u, 0u};
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            uint16_t two;
+            if constexpr (OUT == 0) asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(v[i + 1]), "f"(v[i]));
+            else if constexpr (OUT == 1) asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(two) : "f"(v[i + 1]), "f"(v[i]));
+            else asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %1, %2;\n\tcvt.u16.u8 %0, t;\n\t}" : "=h"(two) : "f"(v[i + 1]), "f"(v[i]));
+            if constexpr (OUT == 5) o[0] |= (uint32_t)two << (4 * i);
+            else o[i >> 2] |= (uint32_t)two << (8 * (i & 2));
+        }
+        if (k < K) {
+            if constexpr (OUT == 5) *reinterpret_cast<uint32_t*>(o_.codes + ((int64_t)row * K + k) / 2) = o[0];
+            else *reinterpret_cast<uint2*>(o_.codes + (int64_t)row * K + k) = make_uint2(o[0], o[1]);
+            if ((threadIdx.x & 3) == 0) {
+                const int kb = k >> 5;
+                uint8_t* at = o_.sf + place.at(kb, (K + 127) / 128, o_.chunks);
+                *at = (uint8_t)sbyte;
+                if (k + 32 == K) for (int i = 1; i < 4 - (kb & 3); ++i) at[i] = 127;     // K blocks that only fill up the last 128 elements
+            }
+        }
+    }
+    if (!early) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+template <class... KArgs, class... Args>
+static int launch_after(void (*kernel)(KArgs...), unsigned grid, unsigned block, unsigned smem, cudaStream_t st, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+    if (e != cudaSuccess) { set_last_cuda_error(e); return MXQ_ELAUNCH; }
+    return check_launch();
+}
+
+// MXQ_ESIZE: not covered (a rounding mode other than to nearest, unaligned rows), take extract + pack_rows_kernel
+static int quantize_rows(const void* x, int x_dtype, const void* row_index, int index64, int64_t rows_in, const Groups& g, int eb, int fb, int rm,
+                         const RowOperand& o, cudaStream_t st) {
+    const int64_t K = o.K, rows = g.rows;
+    const int64_t lanes = (K / 8 + QUANT_ACCESSES - 1) / QUANT_ACCESSES;
+    const int block = lanes >= 256 ? 256 : (int)((lanes + 31) / 32 * 32);
+    const int64_t segments = (K / 8 + (int64_t)block * QUANT_ACCESSES - 1) / ((int64_t)block * QUANT_ACCESSES);
+    if (rm != MXQ_RN || reinterpret_cast<uintptr_t>(x) % 16 != 0 || rows * segments > (1ll << 31) - 1) return MXQ_ESIZE;
+    // a grid of one wave lets the product's CTAs come up beside it; a longer one keeps the SMs' registers to itself until its end
+    const int early = rows * segments <= 2 * sm_count();
+    int rc = MXQ_ESIZE;
+    with_kind(x_dtype, [&](auto kin) {
+        using KIn = decltype(kin);
+        with_preset(eb, fb, 1, rm, [&](auto fmt) {
+            using F = decltype(fmt);
+            auto go = [&](auto out) {
+                rc = launch_after(quantize_rows_kernel<KIn, F, decltype(out)::value>, (unsigned)(rows * segments), (unsigned)block, 0, st, x, row_index, index64,
+                                  rows_in, g, o, (int)segments, early);
+            };
+            if constexpr (F{}.eb() == 5) go(std::integral_constant<int, 1>{});
+            else if constexpr (F{}.eb() == 2 && F{}.fb() == 1) { if (o.nibbles) go(std::integral_constant<int, 5>{}); else go(std::integral_constant<int, 0>{}); }
+            else go(std::integral_constant<int, 0>{});
+        });
+    });
+    return rc;
 }
 
 // box of `box_rows` rows x 128 bytes of a [rows, K] operand
@@ -476,26 +706,40 @@ static int launch(const Params& p, const uint8_t* w_codes, const uint8_t* x_code
     const cudaError_t e = raise_smem_limit(grouped_kernel<C, DT>, C::SMEM_BYTES, attr_done);
     if (e != cudaSuccess) { set_last_cuda_error(e); return MXQ_ELAUNCH; }
     CUtensorMap mw, mx64, mx16;
-    if (!make_map(&mw, w_codes, (int64_t)p.groups * p.N, p.K, 128, C::MXF4) || !make_map(&mx64, x_codes, p.rows, p.K, 64, C::MXF4) ||
-        !make_map(&mx16, x_codes, p.rows, p.K, 16, C::MXF4)) return MXQ_ELAUNCH;
+    const Groups& g = p.rows;
+    if (!make_map(&mw, w_codes, (int64_t)g.groups * p.N, p.K, 128, C::MXF4) || !make_map(&mx64, x_codes, g.rows, p.K, 64, C::MXF4) ||
+        !make_map(&mx16, x_codes, g.rows, p.K, 16, C::MXF4)) return MXQ_ELAUNCH;
     // units at most: every group may end in a partial tile; what the groups leave is known on the device only
     const int64_t ftiles = (p.N + C::FEATURES - 1) / C::FEATURES;
-    const int64_t most = (int64_t)(p.rows / p.width + (p.groups < p.rows ? p.groups : p.rows)) * ftiles;
+    const int64_t most = (int64_t)(g.rows / g.width + (g.groups < g.rows ? g.groups : g.rows)) * ftiles;
     const int grid = (int)(most < sm_count() ? most : sm_count());
-    grouped_kernel<C, DT><<<grid, THREADS, C::SMEM_BYTES, st>>>(mw, mx64, mx16, p);
-    return check_launch();
+    return launch_after(grouped_kernel<C, DT>, (unsigned)grid, THREADS, C::SMEM_BYTES, st, mw, mx64, mx16, p);
 }
 
 template <class C>
 static int launch_dt(Params& p, int dt, const uint8_t* w_codes, const uint8_t* x_codes, cudaStream_t st) {
-    if (p.width == 0 || p.width > C::BT) p.width = C::BT;
     if (dt == MXQ_F32) return launch<C, MXQ_F32>(p, w_codes, x_codes, st);
     if (dt == MXQ_BF16) return launch<C, MXQ_BF16>(p, w_codes, x_codes, st);
     return launch<C, MXQ_F16>(p, w_codes, x_codes, st);
 }
 
+// element formats of the tensor-core path
+static bool valid_mx_preset(int eb, int fb) {
+    return (eb == 4 && fb == 3) || (eb == 5 && fb == 2) || (eb == 2 && (fb == 3 || fb == 1)) || (eb == 3 && fb == 2);
+}
 static int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
-static int64_t sf_pitch(int64_t rows) { return (rows + 3) / 4 * 4; }
+
+// Tile shape of a call, from the sizes that the host knows.
+struct Plan {
+    bool narrow;                 // 128 features, up to 128 rows (else 256 and 240)
+    int width;
+    int chunks() const { return narrow ? 1 : 2; }
+    int64_t sf_bytes(int64_t rows, int64_t groups, int64_t K) const { return (rows / width + groups + 1) * ((K + 127) / 128) * chunks() * 512; }
+};
+static Plan make_plan(int64_t rows, int64_t groups) {
+    const bool narrow = rows / groups <= 128;
+    return Plan{narrow, narrow ? Narrow::BT : Wide::BT};
+}
 
 }  // namespace grouped
 }  // namespace mxq
@@ -504,9 +748,9 @@ using namespace mxq;
 
 extern "C" int mxq_mx_max_groups(void) { return grouped::MAX_GROUPS; }
 
-extern "C" int64_t mxq_mx_grouped_scratch_bytes(int64_t rows_in, int64_t rows, int64_t K) {
-    if (rows_in < 0 || rows < 0 || K <= 0 || K % 32 != 0) return MXQ_EINVAL;
-    return grouped::align256(rows * K) + grouped::align256((K + 127) / 128 * grouped::sf_pitch(rows) * 4) + grouped::align256(rows_in * K) +
+extern "C" int64_t mxq_mx_grouped_scratch_bytes(int64_t rows_in, int64_t rows, int64_t K, int64_t groups) {
+    if (rows_in < 0 || rows < 0 || groups <= 0 || K <= 0 || K % 32 != 0) return MXQ_EINVAL;
+    return grouped::align256(rows * K) + grouped::align256(grouped::make_plan(rows, groups).sf_bytes(rows, groups, K)) + grouped::align256(rows_in * K) +
            grouped::align256(rows_in * K / 32);
 }
 
@@ -525,42 +769,49 @@ extern "C" int mxq_mx_grouped_linear(const void* x, int x_dtype, int64_t rows_in
     if (rows == 0) return MXQ_OK;
     if ((!x && rows_in > 0) || !w_codes || !w_sf || !out || !scratch || (extra_mode != MXQ_EXTRA_NONE && !extra)) return MXQ_EINVAL;
     if ((reinterpret_cast<uintptr_t>(w_codes) | reinterpret_cast<uintptr_t>(w_sf)) % 16 != 0 || reinterpret_cast<uintptr_t>(scratch) % 256 != 0) return MXQ_EINVAL;
-    if (scratch_bytes < mxq_mx_grouped_scratch_bytes(rows_in, rows, K)) return MXQ_ESIZE;
+    if (scratch_bytes < mxq_mx_grouped_scratch_bytes(rows_in, rows, K, groups)) return MXQ_ESIZE;
     // both operands E2M1 and the weight kept as nibbles: the 4-bit kind
     const bool x_e2m1 = x_exp_bits == 2 && x_frac_bits == 1;
     const bool fp4 = w_hw_format == 5;
     if (fp4 && (!x_e2m1 || K % 256 != 0 || reinterpret_cast<uintptr_t>(w_codes) % 32 != 0)) return MXQ_EINVAL;
     if (!fp4 && w_hw_format != 0 && w_hw_format != 1) return MXQ_EINVAL;
-    grouped::CodeTables tables;
-    int x_fmt = 0;
-    if (!hw_code_tables(x_exp_bits, x_frac_bits, tables.plain, tables.halved, tables.bad, &x_fmt)) return MXQ_EINVAL;
+    if (!grouped::valid_mx_preset(x_exp_bits, x_frac_bits) || x_round_mode < MXQ_RN || x_round_mode > MXQ_RZ) return MXQ_EINVAL;
+    const int x_fmt = x_exp_bits == 5 ? 1 : 0;
 
+    const grouped::Plan plan = grouped::make_plan(rows, groups);
+    const grouped::Groups g{offsets, offsets64, (int)rows, (int)groups, plan.width};
     uint8_t* codes = static_cast<uint8_t*>(scratch);
     uint8_t* sf = codes + grouped::align256(rows * K);
-    uint8_t* ref_codes = sf + grouped::align256((K + 127) / 128 * grouped::sf_pitch(rows) * 4);
+    uint8_t* ref_codes = sf + grouped::align256(plan.sf_bytes(rows, groups, K));
     uint8_t* ref_scales = ref_codes + grouped::align256(rows_in * K);
+    const grouped::RowOperand operand{codes, sf, (int)K, plan.chunks(), fp4};
     cudaStream_t st = (cudaStream_t)stream;
-    if (rows_in > 0) {
-        const int rc = mxq_mxfp_extract(x, x_dtype, ref_scales, ref_codes, rows_in * K, 32, x_exp_bits, x_frac_bits, 1, x_round_mode, stream);
-        if (rc != MXQ_OK) return rc;
+    int rc = grouped::quantize_rows(x, x_dtype, row_index, index64, rows_in, g, x_exp_bits, x_frac_bits, x_round_mode, operand, st);
+    if (rc == MXQ_ESIZE) {
+        if (rows_in > 0) {
+            rc = mxq_mxfp_extract(x, x_dtype, ref_scales, ref_codes, rows_in * K, 32, x_exp_bits, x_frac_bits, 1, x_round_mode, stream);
+            if (rc != MXQ_OK) return rc;
+        }
+        grouped::CodeTables tables;
+        int fmt;
+        if (!hw_code_tables(x_exp_bits, x_frac_bits, tables.plain, tables.halved, tables.bad, &fmt)) return MXQ_EINVAL;
+        const int64_t threads = rows * ((K + 127) / 128 * 4);
+        grouped::pack_rows_kernel<<<(unsigned)((threads + 255) / 256), 256, 0, st>>>(ref_scales, ref_codes, row_index, index64, rows_in, g, operand, tables);
+        rc = check_launch();
     }
-    const int64_t threads = rows * ((K + 127) / 128 * 4);
-    grouped::pack_rows_kernel<<<(unsigned)((threads + 255) / 256), 256, 0, st>>>(ref_scales, ref_codes, row_index, index64, rows_in, rows, (int)K, fp4, codes, sf,
-                                                                                grouped::sf_pitch(rows), tables);
-    const int rc = check_launch();
     if (rc != MXQ_OK) return rc;
 
     grouped::Params p{};
     p.w_sf = w_sf;
     p.w_sf_group = mxq_mx_sf_bytes(N, K, MXQ_OPERAND_A, 0);
-    p.x_sf = reinterpret_cast<const uint32_t*>(sf);
-    p.x_sf_pitch = grouped::sf_pitch(rows);
-    p.out = out; p.bias = bias; p.extra = extra; p.offsets = offsets; p.offsets64 = offsets64;
-    p.rows = (int)rows; p.groups = (int)groups; p.N = (int)N; p.K = (int)K;
+    p.x_sf = sf;
+    p.out = out; p.bias = bias; p.extra = extra; p.rows = g;
+    p.N = (int)N; p.K = (int)K;
+    const uintptr_t four = x_dtype == MXQ_F32 ? 16 : 8;
+    p.vector = N % 4 == 0 && reinterpret_cast<uintptr_t>(out) % four == 0 && reinterpret_cast<uintptr_t>(extra) % four == 0;
     p.act = activation; p.extra_mode = extra_mode; p.zero_rest = zero_rest; p.status = status;
     // formats of left (weight) and right (rows) operand, K-major both, E8M0 scales, M >> 4; E2M1 is 1 in the 4-bit kind's encoding
     p.idesc = (fp4 ? (1u << 7) | (1u << 10) : ((uint32_t)w_hw_format << 7) | ((uint32_t)x_fmt << 10)) | (1u << 23) | ((uint32_t)(128 >> 4) << 24);
-    const bool narrow = rows / groups <= 128;
-    if (fp4) return narrow ? grouped::launch_dt<grouped::NarrowFp4>(p, x_dtype, w_codes, codes, st) : grouped::launch_dt<grouped::WideFp4>(p, x_dtype, w_codes, codes, st);
-    return narrow ? grouped::launch_dt<grouped::Narrow>(p, x_dtype, w_codes, codes, st) : grouped::launch_dt<grouped::Wide>(p, x_dtype, w_codes, codes, st);
+    if (fp4) return plan.narrow ? grouped::launch_dt<grouped::NarrowFp4>(p, x_dtype, w_codes, codes, st) : grouped::launch_dt<grouped::WideFp4>(p, x_dtype, w_codes, codes, st);
+    return plan.narrow ? grouped::launch_dt<grouped::Narrow>(p, x_dtype, w_codes, codes, st) : grouped::launch_dt<grouped::Wide>(p, x_dtype, w_codes, codes, st);
 }

@@ -41,12 +41,16 @@ def block_scaled_ok(x: Tensor, x_meta: MXFPMeta | None, w_tensor_meta: MXFPTenso
             and x.is_cuda and x.dtype in _lib.DTYPE_ID and x.shape[-1] == shape[1] and shape[1] % 32 == 0 and x.numel() > 0)
 
 
-def require_epilogue(x: Tensor, x_meta: MXFPMeta | None, w_tensor_meta: MXFPTensorMeta | None, both_quantised: bool) -> None:
-    """Raise for a fused linear whose product cannot take an epilogue (an empty ``x`` can)."""
-    probe = x if x.numel() > 0 or x.ndim == 0 else x.new_empty(1, x.shape[-1])
-    if not both_quantised or not block_scaled_ok(probe, x_meta, w_tensor_meta):
+def require_epilogue(x_meta: MXFPMeta | None, w_tensor_meta: MXFPTensorMeta | None, kind) -> None:
+    """Raise for a kind of fused linear whose product takes no epilogue."""
+    ok = kind.x_quantised and kind.w_quantised and x_meta is not None and w_tensor_meta is not None
+    if ok:
+        shape = tuple(w_tensor_meta.shape)
+        ok = (len(shape) == 2 and w_tensor_meta.block_dim in (1, -1) and _gemm.supported(w_tensor_meta.meta) and _gemm.supported(x_meta)
+              and shape[1] % 32 == 0)
+    if not ok:
         raise NotImplementedError("backend='fused' takes an activation, multiplier or residual where activation and weight are quantised with "
-                                  "32-element blocks along in_features and is_finite elements, on CUDA; use backend='separate'")
+                                  "32-element blocks along in_features and is_finite elements; use backend='separate'")
 
 
 def _fused_linear(x: Tensor, x_meta: MXFPMeta | None, w: Tensor | None, w_scales: Tensor | None, w_elements: Tensor | None,
@@ -94,16 +98,16 @@ def _fused_linear(x: Tensor, x_meta: MXFPMeta | None, w: Tensor | None, w_scales
 def linear_with_epilogue(x: Tensor, x_meta: MXFPMeta, w: "_grouped.PackedExperts", bias: Tensor | None, activation: str | None,
                          multiplier: Tensor | None, residual: Tensor | None) -> Tensor:
     """``act(Q(x) @ W^T + bias) (* multiplier | + residual)`` in one product, both operands quantised up to the tensor cores."""
-    lead = x.shape[:-1]
-
-    def flat(t: Tensor | None, name: str) -> Tensor | None:
-        if t is not None and tuple(t.shape) != (*lead, w.N):
-            raise ValueError(f"{name} has to have the result's shape {(*lead, w.N)}: got {tuple(t.shape)}")
-        return None if t is None else t.reshape(-1, w.N)
-
-    y = _grouped.grouped_linear(x.reshape(-1, w.K), x_meta, w, None, None if bias is None else bias.to(x.dtype).reshape(1, -1), activation,
-                                flat(multiplier, "multiplier"), flat(residual, "residual"))
-    return y.reshape(*lead, w.N)
+    if x.ndim != 2:
+        lead = x.shape[:-1]
+        for t, name in ((multiplier, "multiplier"), (residual, "residual")):
+            if t is not None and t.shape != (*lead, w.N):
+                raise ValueError(f"{name} has to have the result's shape {(*lead, w.N)}: got {tuple(t.shape)}")
+        flat = [None if t is None else t.reshape(-1, w.N) for t in (multiplier, residual)]
+        return linear_with_epilogue(x.reshape(-1, x.shape[-1]), x_meta, w, bias, activation, *flat).reshape(*lead, w.N)
+    if bias is not None:
+        bias = (bias if bias.dtype == x.dtype else bias.to(x.dtype)).view(1, -1)
+    return _grouped.grouped_linear(x, x_meta, w, None, bias, activation, multiplier, residual)
 
 
 def _separate_epilogue(y: Tensor, activation: str | None, multiplier: Tensor | None, residual: Tensor | None) -> Tensor:
@@ -147,7 +151,7 @@ def mxfp_linear(
     epilogue = activation is not None or multiplier is not None or residual is not None
     if backend == "fused" and epilogue:
         bias = b if not kind.b_quantised else (compose_mxfp_tensor(b_scales, b_elements, b_tensor_meta) if b is not None else None)
-        require_epilogue(x, x_meta, w_tensor_meta, kind.x_quantised and kind.w_quantised)
+        require_epilogue(x_meta, w_tensor_meta, kind)
         n, k = tuple(w_tensor_meta.shape)
         return linear_with_epilogue(x, x_meta, _grouped.pack_experts(w_scales, w_elements, 1, n, k, w_tensor_meta.meta, x_meta), bias,
                                     activation, multiplier, residual)

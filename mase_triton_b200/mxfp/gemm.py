@@ -20,6 +20,7 @@ from . import kernels
 from .meta import MXFPMeta
 
 _STATUS: dict[torch.device, Tensor] = {}
+_STATUS_VIEW: dict[int, tuple[ctypes.c_int, int]] = {}
 _STATUS_TEXT = {1: "TMA producer wait ran out", 2: "MMA issuer wait ran out", 3: "epilogue wait ran out",
                 4: "copy-out (gather) wait ran out", 5: "operand dequantiser wait ran out"}
 
@@ -57,6 +58,17 @@ def status_word(device: torch.device) -> Tensor:
     if device not in _STATUS:
         _STATUS[device] = torch.zeros(1, dtype=torch.int32).pin_memory()
     return _STATUS[device]
+
+
+def status_address(index: int) -> int:
+    """Address of the status word of device ``index``, after the same look at it as :func:`_raise_if_failed`."""
+    view = _STATUS_VIEW.get(index)
+    if view is None:
+        address = status_word(torch.device("cuda", index)).data_ptr()
+        view = _STATUS_VIEW[index] = (ctypes.c_int.from_address(address), address)
+    if view[0].value != 0:
+        _raise_if_failed(torch.device("cuda", index))
+    return view[1]
 
 
 def _raise_if_failed(device: torch.device) -> None:

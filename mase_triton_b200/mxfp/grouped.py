@@ -11,7 +11,7 @@ import torch
 from torch import Tensor
 
 from .. import _lib
-from .gemm import _raise_if_failed, fp4_pair, is_e2m1, status_word, supported
+from .gemm import fp4_pair, is_e2m1, status_address, supported
 from .meta import MXFPMeta
 
 EXTRA_NONE, EXTRA_MULTIPLY, EXTRA_ADD = 0, 1, 2
@@ -83,64 +83,94 @@ def check_activation(activation: str | None) -> int:
         raise ValueError(f"activation {activation!r}: one of {[a for a in _lib.ACTIVATION_ID if a]} or None") from None
 
 
-def _index(t: Tensor, name: str, n: int | None, dev: torch.device) -> Tensor:
-    if t.dtype not in _INDEX_DTYPES or t.ndim != 1 or (n is not None and t.numel() != n):
-        raise ValueError(f"{name} has to be a 1-D int32 or int64 tensor{'' if n is None else f' of {n} entries'}: got {t.dtype} {tuple(t.shape)}")
-    if t.device != dev:
-        raise ValueError(f"{name} is on {t.device}, the input on {dev}")
-    return t.contiguous()
+def _bad_index(t: Tensor, name: str, n: int | None, dev: int) -> bool:
+    return t.dtype not in _INDEX_DTYPES or t.ndim != 1 or (n is not None and t.shape[0] != n) or t.get_device() != dev
+
+
+def _index_error(t: Tensor, name: str, n: int | None, x: Tensor) -> ValueError:
+    return ValueError(f"{name} has to be a 1-D int32 or int64 tensor{'' if n is None else f' of {n} entries'} on {x.device}: "
+                      f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _operand_error(t: Tensor, name: str, shape: tuple, x: Tensor) -> ValueError:
+    return ValueError(f"{name} has to be {x.dtype} {shape} on {x.device}: got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
 def grouped_linear(x: Tensor, x_meta: MXFPMeta, w: PackedExperts, offsets: Tensor | None, bias: Tensor | None = None,
                    activation: str | None = None, multiplier: Tensor | None = None, residual: Tensor | None = None,
                    row_index: Tensor | None = None, out: Tensor | None = None) -> Tensor:
     """``act(Q(x[row_index]) @ W_g^T + bias_g) (* multiplier | + residual)`` for ``x [tokens, K]``; the rows of group ``g`` are
-    ``offsets[g] .. offsets[g + 1]`` (``offsets=None``: one group of all rows).  Returns ``[rows, N]`` of ``x``'s dtype."""
-    _lib.require_cuda(x, "grouped_linear")
+    ``offsets[g] .. offsets[g + 1]`` (``offsets=None``: one group of all rows).  Returns ``[rows, N]`` of ``x``'s dtype.
+
+    A decoding step makes hundreds of these calls of a few microseconds each on the GPU, so the checks here are kept
+    to a few attribute reads each."""
+    if not x.is_cuda:
+        _lib.require_cuda(x, "grouped_linear")
     act = check_activation(activation)
     extra, extra_mode = epilogue_operand(multiplier, residual)
-    if x.dtype not in _lib.DTYPE_ID:
-        raise ValueError(f"input dtype {x.dtype}: one of {[str(d) for d in _lib.DTYPE_ID]}")
-    if x.ndim != 2 or x.shape[1] != w.K:
-        raise ValueError(f"input of shape {tuple(x.shape)}: expected [tokens, {w.K}]")
+    dtype, dev, N, K, groups = x.dtype, x.get_device(), w.N, w.K, w.groups
+    dtype_id = _lib.DTYPE_ID.get(dtype)
+    if dtype_id is None:
+        raise ValueError(f"input dtype {dtype}: one of {[str(d) for d in _lib.DTYPE_ID]}")
+    if x.ndim != 2 or x.shape[1] != K:
+        raise ValueError(f"input of shape {tuple(x.shape)}: expected [tokens, {K}]")
     if not supported(x_meta) or (w.hw_format == 5 and not is_e2m1(x_meta)):
         raise ValueError(f"the weight was packed for another activation format than {x_meta}")
-    dev, tokens, N = x.device, x.shape[0], w.N
-    if w.codes.device != dev:
-        raise ValueError(f"the weight is on {w.codes.device}, the input on {dev}")
+    if w.codes.get_device() != dev:
+        raise ValueError(f"the weight is on {w.codes.device}, the input on {x.device}")
     x = x.contiguous()
+    tokens = rows = x.shape[0]
+    offsets_ptr = index_ptr = bias_ptr = extra_ptr = None
+    offsets64 = index64 = 0
     if offsets is not None:
-        offsets = _index(offsets, "offsets", w.groups + 1, dev)
-    elif w.groups != 1:
+        if _bad_index(offsets, "offsets", groups + 1, dev):
+            raise _index_error(offsets, "offsets", groups + 1, x)
+        offsets = offsets.contiguous()
+        offsets_ptr, offsets64 = offsets.data_ptr(), int(offsets.dtype == torch.int64)
+    elif groups != 1:
         raise ValueError("offsets are missing")
-    rows = tokens
     if row_index is not None:
-        row_index = _index(row_index, "row_index", None, dev)
-        rows = row_index.numel()
-    for name, t, shape in (("bias", bias, (w.groups, N)), ("multiplier" if multiplier is not None else "residual", extra, (rows, N)), ("out", out, (rows, N))):
-        if t is not None and (t.device != dev or t.dtype != x.dtype or tuple(t.shape) != shape):
-            raise ValueError(f"{name} has to be {x.dtype} {shape} on {dev}: got {t.dtype} {tuple(t.shape)} on {t.device}")
-    if out is not None and not out.is_contiguous():
-        raise ValueError("out has to be contiguous")
-    bias = None if bias is None else bias.contiguous()
-    extra = None if extra is None else extra.contiguous()
-    zero_rest = out is None and offsets is not None
+        if _bad_index(row_index, "row_index", None, dev):
+            raise _index_error(row_index, "row_index", None, x)
+        row_index = row_index.contiguous()
+        rows = row_index.shape[0]
+        index_ptr, index64 = row_index.data_ptr(), int(row_index.dtype == torch.int64)
+    if bias is not None:
+        if bias.dtype != dtype or bias.shape != (groups, N) or bias.get_device() != dev:
+            raise _operand_error(bias, "bias", (groups, N), x)
+        bias = bias.contiguous()
+        bias_ptr = bias.data_ptr()
+    if extra is not None:
+        if extra.dtype != dtype or extra.shape != (rows, N) or extra.get_device() != dev:
+            raise _operand_error(extra, "residual" if multiplier is None else "multiplier", (rows, N), x)
+        extra = extra.contiguous()
+        extra_ptr = extra.data_ptr()
+    zero_rest = 0
     if out is None:
-        out = torch.empty((rows, N), dtype=x.dtype, device=dev)
+        zero_rest = int(offsets is not None)
+        out = torch.empty((rows, N), dtype=dtype, device=x.device)
+    else:
+        if out.dtype != dtype or out.shape != (rows, N) or out.get_device() != dev:
+            raise _operand_error(out, "out", (rows, N), x)
+        if not out.is_contiguous():
+            raise ValueError("out has to be contiguous")
+        if not out.is_inference():
+            torch.autograd.graph.increment_version(out)
     if rows == 0:
         return out
-    _raise_if_failed(dev)
+    status = status_address(dev)
     L = _lib.load()
-    nbytes = L.mxq_mx_grouped_scratch_bytes(tokens, rows, w.K)
+    nbytes = L.mxq_mx_grouped_scratch_bytes(tokens, rows, K, groups)
     # of this call alone: two captured graphs, or two streams, never share it
-    scratch = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        rc = L.mxq_mx_grouped_linear(
-            x.data_ptr(), _lib.DTYPE_ID[x.dtype], tokens, rows, w.K, x_meta.element_exp_bits, x_meta.element_frac_bits, _lib.ROUND_ID[x_meta.round_mode],
-            None if row_index is None else row_index.data_ptr(), int(row_index is not None and row_index.dtype == torch.int64),
-            w.codes.data_ptr(), w.sf.data_ptr(), w.hw_format, w.groups, N,
-            None if offsets is None else offsets.data_ptr(), int(offsets is not None and offsets.dtype == torch.int64),
-            out.data_ptr(), None if bias is None else bias.data_ptr(), act, None if extra is None else extra.data_ptr(), extra_mode, int(zero_rest),
-            scratch.data_ptr(), nbytes, status_word(dev).data_ptr(), _lib.stream_ptr(dev))
-    _lib.check(rc, "mxq_mx_grouped_linear")
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    args = (x.data_ptr(), dtype_id, tokens, rows, K, x_meta.element_exp_bits, x_meta.element_frac_bits, _lib.ROUND_ID[x_meta.round_mode], index_ptr, index64,
+            w.codes.data_ptr(), w.sf.data_ptr(), w.hw_format, groups, N, offsets_ptr, offsets64, out.data_ptr(), bias_ptr, act, extra_ptr, extra_mode, zero_rest,
+            scratch.data_ptr(), nbytes, status, torch.cuda.current_stream(dev).cuda_stream)
+    if torch.cuda.current_device() == dev:
+        rc = L.mxq_mx_grouped_linear(*args)
+    else:
+        with torch.cuda.device(dev):
+            rc = L.mxq_mx_grouped_linear(*args)
+    if rc != 0:
+        _lib.check(rc, "mxq_mx_grouped_linear")
     return out

@@ -13,6 +13,7 @@ from typing import Literal
 import torch
 from torch import Tensor, nn
 
+from .._linear_common import parse_layer_type
 from .._ptq_base import PTQLinearBase
 from . import functional as MXFP_F
 from .meta import MXFPMeta, MXFPTensorMeta
@@ -68,10 +69,6 @@ class MXFPLinearPTQ(PTQLinearBase):
         self.register_buffer("_tc_codes", None, persistent=False)
         self.register_buffer("_tc_sf", None, persistent=False)
         self._tc_info = None          # (versions of the code tensors it was built from, hw_format, tile_rows)
-        # the same weight for the product with an epilogue, where it is the left operand
-        self.register_buffer("_row_codes", None, persistent=False)
-        self.register_buffer("_row_sf", None, persistent=False)
-        self._row_info = None         # (versions, hw_format)
 
         if "Wq" in layer_type:
             if w_scales is None:
@@ -114,17 +111,16 @@ class MXFPLinearPTQ(PTQLinearBase):
         return _gemm.PackedOperand(self._tc_codes, self._tc_sf, self._tc_info[1], n, k, _gemm.OPERAND_B, self._tc_info[2])
 
     def row_weight(self):
-        """The quantised weight as the product with an epilogue reads it (``mxfp.grouped``), kept on the module and rebuilt
-        like :meth:`tensor_core_weight`."""
-        from . import grouped as _grouped
+        """The quantised weight as the product with an epilogue reads it (``mxfp.grouped``), kept with the module and rebuilt when
+        the code tensors were written or moved."""
+        w_scales, w_elements = self.w_scales, self.w_elements
+        if self._row_weight is None or self._row_weight[:2] != (w_elements._version, w_scales._version):
+            from . import grouped as _grouped
 
-        versions = (self.w_elements._version, self.w_scales._version)
-        n, k = self.w_tensor_meta.shape
-        if self._row_codes is None or self._row_info is None or self._row_info[0] != versions or self._row_codes.device != self.w_elements.device:
-            p = _grouped.pack_experts(self.w_scales.data, self.w_elements.data, 1, n, k, self.w_tensor_meta.meta, self.x_mxfp_meta)
-            self._row_codes, self._row_sf = p.codes, p.sf
-            self._row_info = (versions, p.hw_format)
-        return _grouped.PackedExperts(self._row_codes, self._row_sf, self._row_info[1], 1, n, k)
+            n, k = self.w_tensor_meta.shape
+            self._row_weight = (w_elements._version, w_scales._version,
+                                _grouped.pack_experts(w_scales.data, w_elements.data, 1, n, k, self.w_tensor_meta.meta, self.x_mxfp_meta))
+        return self._row_weight[2]
 
     def export_packed(self) -> dict:
         """A ``torch.save``-able dict holding this layer with its element codes bit-packed to their true width
@@ -161,7 +157,8 @@ class MXFPLinearPTQ(PTQLinearBase):
 
     def _forward_with_epilogue(self, input: Tensor, activation: str | None, multiplier: Tensor | None, residual: Tensor | None) -> Tensor:
         if self.backend == "fused":
-            MXFP_F.linear.require_epilogue(input, self.x_mxfp_meta, self.w_tensor_meta, "Xq" in self.layer_type and "Wq" in self.layer_type)
+            if self._row_weight is None:
+                MXFP_F.linear.require_epilogue(self.x_mxfp_meta, self.w_tensor_meta, parse_layer_type(self.layer_type))
             return MXFP_F.linear.linear_with_epilogue(input, self.x_mxfp_meta, self.row_weight(), self.bias, activation, multiplier, residual)
         return MXFP_F.mxfp_linear(
             x=input, x_meta=self.x_mxfp_meta,
@@ -246,10 +243,6 @@ class MXFPGroupedLinearPTQ(PTQLinearBase):
         self.w_scales, self.w_elements = self._frozen(w_scales), self._frozen(w_elements)
         self.w_tensor_meta = w_tensor_meta
         self.bias = None if bias is None else self._frozen(bias)
-        # the weights as the kernel reads them, built on first use; they follow .to() and stay out of state_dict()
-        self.register_buffer("_row_codes", None, persistent=False)
-        self.register_buffer("_row_sf", None, persistent=False)
-        self._row_info = None         # (versions of the code tensors it was built from, hw_format)
 
     @classmethod
     def from_weight(cls, weight: Tensor, bias: Tensor | None, x_mxfp_meta: MXFPMeta, w_mxfp_meta: MXFPMeta):
@@ -275,16 +268,15 @@ class MXFPGroupedLinearPTQ(PTQLinearBase):
         return cls(w_scales, w_elements, w_tensor_meta, bias, x_mxfp_meta)
 
     def row_weight(self):
-        """The weights as the kernel reads them, rebuilt when the code tensors were written, moved by ``.to()``."""
-        from . import grouped as _grouped
+        """The weights as the kernel reads them, kept with the module and rebuilt when the code tensors were written or moved."""
+        w_scales, w_elements = self.w_scales, self.w_elements
+        if self._row_weight is None or self._row_weight[:2] != (w_elements._version, w_scales._version):
+            from . import grouped as _grouped
 
-        versions = (self.w_elements._version, self.w_scales._version)
-        if self._row_codes is None or self._row_info is None or self._row_info[0] != versions or self._row_codes.device != self.w_elements.device:
-            p = _grouped.pack_experts(self.w_scales.data, self.w_elements.data, self.groups, self.out_features, self.in_features,
-                                      self.w_tensor_meta.meta, self.x_mxfp_meta)
-            self._row_codes, self._row_sf = p.codes, p.sf
-            self._row_info = (versions, p.hw_format)
-        return _grouped.PackedExperts(self._row_codes, self._row_sf, self._row_info[1], self.groups, self.out_features, self.in_features)
+            self._row_weight = (w_elements._version, w_scales._version,
+                                _grouped.pack_experts(w_scales.data, w_elements.data, self.groups, self.out_features, self.in_features,
+                                                      self.w_tensor_meta.meta, self.x_mxfp_meta))
+        return self._row_weight[2]
 
     @torch.no_grad()
     def forward(self, input: Tensor, offsets: Tensor, activation: str | None = None, multiplier: Tensor | None = None,
@@ -292,7 +284,9 @@ class MXFPGroupedLinearPTQ(PTQLinearBase):
         """``mxfp_grouped_linear`` with this layer's weights."""
         from . import grouped as _grouped
 
-        bias = None if self.bias is None else self.bias.to(input.dtype)
+        bias = self.bias
+        if bias is not None and bias.dtype != input.dtype:
+            bias = bias.to(input.dtype)
         return _grouped.grouped_linear(input, self.x_mxfp_meta, self.row_weight(), offsets, bias, activation, multiplier, residual, row_index, out)
 
     def extra_repr(self) -> str:

@@ -302,6 +302,50 @@ def test_strides_alignment_and_output_in_place(lib):
     assert torch.equal(layer(x, offsets_of(counts), residual=acc, out=acc), want)
 
 
+@pytest.mark.parametrize("meta", ALL, ids=lambda m: m.tag)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("K", [96, 256, 4160])
+def test_one_pass_quantiser_equals_extract_and_pack(lib, meta, dtype, K):
+    """Rows that lie on 16 bytes are quantised in one pass, others by the extract kernel (bit-exact to the oracle) and a
+    table: the same operand, so the same bits, whatever the values."""
+    layer, _, _ = linear_layer(128, K, meta, MXFP8_E4M3_fn if meta.element_exp_bits > 2 else meta, dtype)
+    g = torch.Generator(device=DEV).manual_seed(5)
+    x = torch.randn(40, K, generator=g, device=DEV) * torch.exp2(torch.randint(-30, 12, (40, K), generator=g, device=DEV).float())
+    x[0], x[1], x[2, ::2], x[3] = 0.0, -0.0, 0.0, 1.0
+    x[4, :64] = torch.tensor([479.0, 480.0, 448.0, 465.0, 0.9, -3.0, 2.0**-20, -(2.0**-24)] * 8, device=DEV)
+    x[5, :32] = torch.tensor([57344.0, 65000.0, 61440.0, -1e-7] * 8, device=DEV)
+    x[6] = torch.nextafter(torch.full((K,), 2.0**9, device=DEV), torch.zeros((), device=DEV))
+    if dtype == torch.float32:
+        x[7], x[8, :8] = 1e-40, 2.0**-126
+        x[9, 3], x[10, 40] = float("inf"), float("nan")
+    x = x.to(dtype)
+    aside = torch.empty(40 * K + 1, dtype=dtype, device=DEV)[1:].view(40, K)
+    aside.copy_(x)
+    a, b = layer(x, activation="relu"), layer(aside, activation="relu")
+    assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(), b.nan_to_num())
+    idx = torch.randint(-1, 41, (90,), generator=g, device=DEV)
+    one = MX.grouped._grouped.grouped_linear(x, meta, layer.row_weight(), None, row_index=idx)
+    two = MX.grouped._grouped.grouped_linear(aside, meta, layer.row_weight(), None, row_index=idx)
+    assert torch.equal(one.isnan(), two.isnan()) and torch.equal(one.nan_to_num(), two.nan_to_num())
+
+
+def test_inference_mode_and_copies(lib):
+    import copy
+
+    with torch.inference_mode():
+        layer, _, _, x = grouped_case([5, 6], 64, 64, MXFP8_E4M3_fn, MXFP8_E4M3_fn)
+        first = layer(x, offsets_of([5, 6]))
+        assert torch.equal(layer(x, offsets_of([5, 6]), out=torch.zeros_like(first)), first)
+    layer.w_elements.zero_()
+    twin = copy.deepcopy(layer)
+    for one in (layer, twin):
+        assert torch.equal(one(x, offsets_of([5, 6]))[:5], one.bias[0].expand(5, 64))
+    a = torch.ones(11, 64, dtype=torch.bfloat16, device=DEV)
+    before = a._version
+    layer(torch.zeros(11, 64, dtype=torch.bfloat16, device=DEV), offsets_of([5, 6]), out=a)
+    assert a._version > before
+
+
 def test_buffers_around_the_output_are_untouched(lib):
     counts = [17, 0, 130]
     layer, _, _, x = grouped_case(counts, 33, 64, MXFP8_E4M3_fn, MXFP8_E4M3_fn)

@@ -155,5 +155,5 @@ def test_c_entry_refuses_before_it_launches():
         assert L.mxq_mx_grouped_linear(*(good | bad).values()) == -1, bad
     for bad in (dict(groups=L.mxq_mx_max_groups() + 1, offsets=p), dict(nbytes=64), dict(rows=1 << 31, rows_in=1 << 31)):
         assert L.mxq_mx_grouped_linear(*(good | bad).values()) == -3, bad
-    assert L.mxq_mx_grouped_scratch_bytes(2, 2, 48) == -1 and L.mxq_mx_grouped_scratch_bytes(2, 2, 64) > 0
+    assert L.mxq_mx_grouped_scratch_bytes(2, 2, 48, 1) == -1 and L.mxq_mx_grouped_scratch_bytes(2, 2, 64, 1) > 0
     assert SimpleNamespace(**good).K == 64
