@@ -47,12 +47,13 @@ template <int MH_, int BT_, int STAGES_, bool MXF4_> struct Cfg {
     static constexpr int SF_STEP_BYTES = (MH + X_CHUNKS) * 512;
     static constexpr int STAGE_BYTES = W_BYTES + X_BYTES + SF_STEPS * SF_STEP_BYTES;
     // Two accumulators of BT columns.  MH = 2: the two halves of one tile.  MH = 1: two tiles in turn, so that one is read
-    // while the next is computed.  They begin at multiples of 32 columns; the scales take the columns behind them.
+    // while the next is computed.  They begin at multiples of 32 columns; the scales take the columns behind them, where there is
+    // room two sets in turn (a copy into the columns that the products before it read waits for their end).
     static constexpr int ACC_STRIDE = (BT + 31) / 32 * 32;
-    static constexpr int SFW_COL = ACC_STRIDE > BT ? BT : 2 * ACC_STRIDE;
-    static constexpr int SFX_COL = ACC_STRIDE > BT ? ACC_STRIDE + BT : SFW_COL + SF_STEPS * 8;
-    static_assert(ACC_STRIDE == BT || SFW_COL + SF_STEPS * 8 <= ACC_STRIDE, "tensor memory");
-    static_assert(SFX_COL + SF_STEPS * 8 <= 512, "tensor memory");
+    static constexpr int SF_SETS = MH == 2 && MXF4 ? 1 : 2, SF_COLS = SF_STEPS * 8;
+    static constexpr int SFW_COL = MH == 2 ? BT : 2 * ACC_STRIDE, SFX_COL = MH == 2 ? ACC_STRIDE + BT : SFW_COL + SF_SETS * SF_COLS;
+    static_assert(MH == 1 || BT + SF_SETS * SF_COLS <= ACC_STRIDE, "tensor memory");
+    static_assert(SFX_COL + SF_SETS * SF_COLS <= 512, "tensor memory");
     static_assert(STAGE_BYTES % 1024 == 0, "the 128-byte swizzle repeats every 1024 bytes");
     // behind the ring: barriers, the group table, the epilogue's 2 KiB per warp
     static constexpr int TABLE_END = (256 + 2 * (MAX_GROUPS + 1) * 4 + 15) / 16 * 16;
@@ -85,7 +86,7 @@ template <class T> union Four {
     __device__ __forceinline__ Four() {}
 };
 template <class T> __device__ __forceinline__ void load_four(const T* at, int left, int vector, Four<T>& o) {
-    if (vector) { if (left > 0) o.w = *reinterpret_cast<const typename Words<T>::V*>(at); return; }
+    if (vector) { if (left > 0) o.w = __ldcg(reinterpret_cast<const typename Words<T>::V*>(at)); return; }
 #pragma unroll
     for (int k = 0; k < 4; ++k) if (k < left) o.v[k] = at[k];
 }
@@ -97,14 +98,38 @@ template <class T> __device__ __forceinline__ void store_four(T* at, int left, i
 
 // z * sigmoid(2u) is 0.5 z (1 + tanh u); exp overflows to Inf for very negative arguments and the quotient is then 0
 __device__ __forceinline__ float sigmoid_times(float z, float a) { return __fdividef(z, 1.0f + __expf(-a)); }
-__device__ __forceinline__ float activate(float z, int act) {
-    switch (act) {
-        case MXQ_ACT_RELU: return z < 0.0f ? 0.0f : z;                       // NaN stays NaN
-        case MXQ_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-        case MXQ_ACT_GELU_TANH: return sigmoid_times(z, 1.5957691216057308f * (z + 0.044715f * z * z * z));
-        case MXQ_ACT_SILU: return sigmoid_times(z, z);
-        default: return z;
+template <int ACT> __device__ __forceinline__ float activate(float z) {
+    if constexpr (ACT == MXQ_ACT_RELU) return z < 0.0f ? 0.0f : z;                       // NaN stays NaN
+    else if constexpr (ACT == MXQ_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    else if constexpr (ACT == MXQ_ACT_GELU_TANH) return sigmoid_times(z, 1.5957691216057308f * (z + 0.044715f * z * z * z));
+    else if constexpr (ACT == MXQ_ACT_SILU) return sigmoid_times(z, z);
+    else return z;
+}
+// The epilogue of one lane's 4 x 4 values: rows at, at + 4 * pitch, ... (`rows` of them exist, at most four), four features each.
+// The choices are made once for all sixteen: a switch per value costs more than the values.
+template <int ACT, class T>
+__device__ __forceinline__ void finish(const float* slot, int lane, const float (&bias)[4], const Four<T> (&extra)[4], int extra_mode, T* at, int64_t pitch, int rows,
+                                       int left, int vector) {
+    float y[16];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float4 v = reinterpret_cast<const float4*>(slot)[i * 32 + lane];
+        y[4 * i] = v.x; y[4 * i + 1] = v.y; y[4 * i + 2] = v.z; y[4 * i + 3] = v.w;
     }
+#pragma unroll
+    for (int k = 0; k < 16; ++k) y[k] = activate<ACT>(y[k] + bias[k & 3]);
+    if (extra_mode == X_MUL) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) y[k] *= widen(extra[k >> 2].v[k & 3]);
+    } else if (extra_mode == X_ADD) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) y[k] += widen(extra[k >> 2].v[k & 3]);
+    }
+    Four<T> o[4];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) narrow(y[k], o[k >> 2].v[k & 3]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) if (i < rows) store_four(at + i * 4 * pitch, left, vector, o[i]);
 }
 
 // where a unit of work lies: features [f0, f0 + FEATURES) of group g for rows [row, row + rows)
@@ -324,6 +349,8 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                 ok = mbar_wait(full_bar(s), (it / STAGES) & 1, p.status, ST_MMA_TIMEOUT);
                 const uint32_t st = ring + s * C::STAGE_BYTES, sf = st + C::W_BYTES + C::X_BYTES;
                 const uint64_t x_desc = smem_desc(st + C::W_BYTES, 16, 1024, LAYOUT_SW128);
+                const uint32_t set = C::SF_SETS == 2 ? (it & 1u) * C::SF_COLS : 0u;
+                const uint32_t sfw_at = tmem + C::SFW_COL + set, sfx_at = tmem + C::SFX_COL + set;
                 for (int h = 0; h < halves; ++h) {
                     const int a = MH == 1 ? buf : h;
                     // the first product into an accumulator overwrites it: the epilogue must have read what it held
@@ -338,10 +365,10 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                             for (int c = 0; c < C::SF_STEPS; ++c) {
                                 const uint32_t src = sf + c * C::SF_STEP_BYTES;
                                 for (int hh = 0; hh < halves; ++hh)
-                                    tmem_cp_32x128b(tmem + C::SFW_COL + 8 * c + 4 * hh, smem_desc(src + 512 * hh, 0, 128, LAYOUT_NONE));
-                                tmem_cp_32x128b(tmem + C::SFX_COL + 8 * c, smem_desc(src + MH * 512, 0, 128, LAYOUT_NONE));
+                                    tmem_cp_32x128b(sfw_at + 8 * c + 4 * hh, smem_desc(src + 512 * hh, 0, 128, LAYOUT_NONE));
+                                tmem_cp_32x128b(sfx_at + 8 * c, smem_desc(src + MH * 512, 0, 128, LAYOUT_NONE));
                                 if (C::X_CHUNKS == 2 && n > 128)
-                                    tmem_cp_32x128b(tmem + C::SFX_COL + 8 * c + 4, smem_desc(src + MH * 512 + 512, 0, 128, LAYOUT_NONE));
+                                    tmem_cp_32x128b(sfx_at + 8 * c + 4, smem_desc(src + MH * 512 + 512, 0, 128, LAYOUT_NONE));
                             }
                         }
                         const uint64_t w_desc = smem_desc(st + h * 16384, 16, 1024, LAYOUT_SW128);
@@ -352,10 +379,10 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                             if constexpr (C::MXF4) {
                                 const uint32_t id = (k & 1u) * 2u;                 // 64 elements: scale bytes (0, 1) or (2, 3) of step k / 2
                                 mma_mxf4(d, w_desc + 2 * k, x_desc + 2 * k, idesc_n | (id << 29) | (id << 4),
-                                         tmem + C::SFW_COL + 8 * (k >> 1) + 4 * h, tmem + C::SFX_COL + 8 * (k >> 1), acc);
+                                         sfw_at + 8 * (k >> 1) + 4 * h, sfx_at + 8 * (k >> 1), acc);
                             } else {
                                 mma_mxf8f6f4(d, w_desc + 2 * k, x_desc + 2 * k, idesc_n | (k << 29) | (k << 4),
-                                             tmem + C::SFW_COL + 4 * h, tmem + C::SFX_COL, acc);
+                                             sfw_at + 4 * h, sfx_at, acc);
                             }
                         }
                         if (h == halves - 1) mma_commit(empty_bar(s));
@@ -400,6 +427,13 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                     if (r < t.rows) load_four(extra + (size_t)(t.row + r) * p.N + f, p.N - f, p.vector, e[i]);
                 }
             };
+            if (p.extra_mode != X_NONE) {
+                // the whole tile of the second operand on its way to L2 while the products are formed: 128-byte lines, rows dealt to the threads
+                const int bytes = min(C::FEATURES, p.N - t.f0) * (int)sizeof(T), lines = (bytes + 127) >> 7;
+                for (int i = threadIdx.x - FIRST_EPI_WARP * 32; i < t.rows * lines; i += EPI_WARPS * 32)
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char*>(extra + (size_t)(t.row + i / lines) * p.N + t.f0) +
+                                                                  min(i % lines * 128, bytes - 1)));
+            }
             if (side < chunks) request(0, side);
             ok = mbar_wait(accum_full(buf), MH == 1 ? (count >> 1) & 1 : count & 1, p.status, ST_EPILOGUE_TIMEOUT);
             tc_fence_after();
@@ -431,22 +465,14 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                         for (int i = 0; i < 4; ++i) now[i].w = e[i].w;
                         if (c + 2 < chunks) request(h, c + 2);
                         else if (h + 1 < halves) request(h + 1, side);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float4 v = reinterpret_cast<const float4*>(slot)[i * 32 + lane];
-                            const int row = c * 16 + i * 4 + er;
-                            if (row < t.rows) {
-                                float y[4] = {v.x, v.y, v.z, v.w};
-                                Four<T> o;
-#pragma unroll
-                                for (int k = 0; k < 4; ++k) {
-                                    y[k] = activate(y[k] + bias[k], p.act);
-                                    if (p.extra_mode == X_MUL) y[k] *= widen(now[i].v[k]);
-                                    else if (p.extra_mode == X_ADD) y[k] += widen(now[i].v[k]);
-                                    narrow(y[k], o.v[k]);
-                                }
-                                store_four(out + (size_t)(t.row + row) * p.N + f, p.N - f, p.vector, o);
-                            }
+                        T* at = out + (size_t)(t.row + c * 16 + er) * p.N + f;
+                        const int rows = (t.rows - c * 16 - er + 3) >> 2, left = p.N - f;
+                        switch (p.act) {
+                            case MXQ_ACT_RELU: finish<MXQ_ACT_RELU>(slot, lane, bias, now, p.extra_mode, at, p.N, rows, left, p.vector); break;
+                            case MXQ_ACT_GELU: finish<MXQ_ACT_GELU>(slot, lane, bias, now, p.extra_mode, at, p.N, rows, left, p.vector); break;
+                            case MXQ_ACT_GELU_TANH: finish<MXQ_ACT_GELU_TANH>(slot, lane, bias, now, p.extra_mode, at, p.N, rows, left, p.vector); break;
+                            case MXQ_ACT_SILU: finish<MXQ_ACT_SILU>(slot, lane, bias, now, p.extra_mode, at, p.N, rows, left, p.vector); break;
+                            default: finish<MXQ_ACT_NONE>(slot, lane, bias, now, p.extra_mode, at, p.N, rows, left, p.vector); break;
                         }
                         __syncwarp();
                     }
