@@ -47,10 +47,9 @@ template <int MH_, int BT_, int STAGES_, bool MXF4_> struct Cfg {
     static constexpr int SF_STEP_BYTES = (MH + X_CHUNKS) * 512;
     static constexpr int STAGE_BYTES = W_BYTES + X_BYTES + SF_STEPS * SF_STEP_BYTES;
     // Two accumulators of BT columns.  MH = 2: the two halves of one tile.  MH = 1: two tiles in turn, so that one is read
-    // while the next is computed.  They begin at multiples of 32 columns; the scales take the columns behind them, where there is
-    // room two sets in turn (a copy into the columns that the products before it read waits for their end).
-    static constexpr int ACC_STRIDE = (BT + 31) / 32 * 32;
-    static constexpr int SF_SETS = MH == 2 && MXF4 ? 1 : 2, SF_COLS = SF_STEPS * 8;
+    // while the next is computed.  The scales take the columns behind them, two sets in turn.
+    static constexpr int ACC_STRIDE = MH == 2 ? 256 : BT;
+    static constexpr int SF_SETS = 2, SF_COLS = SF_STEPS * 8;
     static constexpr int SFW_COL = MH == 2 ? BT : 2 * ACC_STRIDE, SFX_COL = MH == 2 ? ACC_STRIDE + BT : SFW_COL + SF_SETS * SF_COLS;
     static_assert(MH == 1 || BT + SF_SETS * SF_COLS <= ACC_STRIDE, "tensor memory");
     static_assert(SFX_COL + SF_SETS * SF_COLS <= 512, "tensor memory");
@@ -61,7 +60,7 @@ template <int MH_, int BT_, int STAGES_, bool MXF4_> struct Cfg {
     static_assert(SMEM_BYTES <= 232448, "more shared memory than a CTA can have");
 };
 using Wide = Cfg<2, 240, 3, false>;
-using WideFp4 = Cfg<2, 240, 3, true>;
+using WideFp4 = Cfg<2, 224, 3, true>;
 using Narrow = Cfg<1, 128, 6, false>;
 using NarrowFp4 = Cfg<1, 128, 5, true>;
 
@@ -130,6 +129,23 @@ __device__ __forceinline__ void finish(const float* slot, int lane, const float 
     for (int k = 0; k < 16; ++k) narrow(y[k], o[k >> 2].v[k & 3]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) if (i < rows) store_four(at + i * 4 * pitch, left, vector, o[i]);
+}
+
+// one thread of a converged warp, the same one each time
+__device__ __forceinline__ bool elect_one() {
+    uint32_t pred;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(pred));
+    return pred != 0;
+}
+// whether a barrier's phase has completed, without waiting
+__device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
 }
 
 // where a unit of work lies: features [f0, f0 + FEATURES) of group g for rows [row, row + rows)
@@ -263,7 +279,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     auto accum_empty = [&](int a) { return bars + 8u * (2 * STAGES + 2 + a); };
     const uint32_t drain_bar = bars + 8u * (2 * STAGES + 4);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(~0u, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) { mbar_init(full_bar(s), 2); mbar_init(empty_bar(s), 1); }      // full: weight copies, row copies
         for (int a = 0; a < 2; ++a) { mbar_init(accum_full(a), 1); mbar_init(accum_empty(a), EPI_WARPS); }
@@ -279,7 +295,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = __shfl_sync(~0u, *tmem_slot, 0);
 
     const int KT = (p.K + C::K_STEP - 1) / C::K_STEP, KT128 = (p.K + 127) / 128;
     const int ftiles = (p.N + C::FEATURES - 1) / C::FEATURES;
@@ -336,66 +352,91 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             mbar_wait(full_bar(j % STAGES), (j / STAGES) & 1, p.status, ST_PRODUCER_TIMEOUT);
     } else if (warp == 1) {
         // ---------------- MMA issuer ----------------
-        bool ok = true;
+        // One thread's issue rate is what a narrow tile's products run at, so everything here is uniform over the warp (the
+        // instructions take their operands from uniform registers) and the thread is elected.  The scales of a stage are copied
+        // to tensor memory before the last products of the stage in front of it, into the other set of columns: behind
+        // them the copies would hold up the tensor pipe (256 x 240: 1330 -> 1060 cycles per 128 of K).
         uint32_t it = 0, count = 0;
-        for (int u = blockIdx.x; u < walk.total && ok; u += gridDim.x, ++count) {
-            const Unit t = walk.at(u, C::FEATURES);
-            const int halves = halves_of(t);
-            const uint32_t n = t.padded();
+        bool ok = true, copied = false;
+        int u = blockIdx.x;
+        Unit next = u < walk.total ? walk.at(u, C::FEATURES) : Unit{};
+        auto stage_sf = [&](uint32_t i) { return ring + (i % STAGES) * C::STAGE_BYTES + C::W_BYTES + C::X_BYTES; };
+        auto copy_scales = [&](uint32_t i, int halves, uint32_t n) {
+            const uint32_t set = (i & 1u) * C::SF_COLS, sf = stage_sf(i);
+            if (elect_one()) {
+#pragma unroll
+                for (int c = 0; c < C::SF_STEPS; ++c) {
+                    const uint32_t src = sf + c * C::SF_STEP_BYTES;
+                    tmem_cp_32x128b(tmem + C::SFW_COL + set + 8 * c, smem_desc(src, 0, 128, LAYOUT_NONE));
+                    if (MH == 2 && halves == 2) tmem_cp_32x128b(tmem + C::SFW_COL + set + 8 * c + 4, smem_desc(src + 512, 0, 128, LAYOUT_NONE));
+                    tmem_cp_32x128b(tmem + C::SFX_COL + set + 8 * c, smem_desc(src + MH * 512, 0, 128, LAYOUT_NONE));
+                    if (C::X_CHUNKS == 2 && n > 128)
+                        tmem_cp_32x128b(tmem + C::SFX_COL + set + 8 * c + 4, smem_desc(src + MH * 512 + 512, 0, 128, LAYOUT_NONE));
+                }
+            }
+            __syncwarp();
+        };
+        for (; u < walk.total && ok; u += gridDim.x, ++count) {
+            const int halves = __shfl_sync(~0u, halves_of(next), 0);
+            const uint32_t n = __shfl_sync(~0u, next.padded(), 0);
+            const bool more = u + (int)gridDim.x < walk.total;
+            if (more) next = walk.at(u + gridDim.x, C::FEATURES);
+            const int next_halves = __shfl_sync(~0u, halves_of(next), 0);
+            const uint32_t next_n = __shfl_sync(~0u, next.padded(), 0);
             const uint32_t idesc_n = p.idesc | ((n >> 3) << 17);
             const int buf = MH == 1 ? (int)(count & 1u) : 0;
             for (int kt = 0; kt < KT && ok; ++kt, ++it) {
                 const int s = it % STAGES;
-                ok = mbar_wait(full_bar(s), (it / STAGES) & 1, p.status, ST_MMA_TIMEOUT);
-                const uint32_t st = ring + s * C::STAGE_BYTES, sf = st + C::W_BYTES + C::X_BYTES;
-                const uint64_t x_desc = smem_desc(st + C::W_BYTES, 16, 1024, LAYOUT_SW128);
-                const uint32_t set = C::SF_SETS == 2 ? (it & 1u) * C::SF_COLS : 0u;
-                const uint32_t sfw_at = tmem + C::SFW_COL + set, sfx_at = tmem + C::SFX_COL + set;
-                for (int h = 0; h < halves; ++h) {
-                    const int a = MH == 1 ? buf : h;
-                    // the first product into an accumulator overwrites it: the epilogue must have read what it held
-                    if (kt == 0 && ok) {
-                        if constexpr (MH == 1) { if (count >= 2) ok = mbar_wait(accum_empty(a), ((count >> 1) - 1) & 1, p.status, ST_MMA_TIMEOUT); }
-                        else { if (count >= 1) ok = mbar_wait(accum_empty(a), (count - 1) & 1, p.status, ST_MMA_TIMEOUT); }
-                    }
+                const uint32_t st = ring + s * C::STAGE_BYTES;
+                const uint32_t set = (it & 1u) * C::SF_COLS;
+                if (!copied) {
+                    ok = mbar_wait(full_bar(s), (it / STAGES) & 1, p.status, ST_MMA_TIMEOUT);
                     tc_fence_after();
-                    if (ok && lane == 0) {
-                        if (h == 0) {
-#pragma unroll
-                            for (int c = 0; c < C::SF_STEPS; ++c) {
-                                const uint32_t src = sf + c * C::SF_STEP_BYTES;
-                                for (int hh = 0; hh < halves; ++hh)
-                                    tmem_cp_32x128b(sfw_at + 8 * c + 4 * hh, smem_desc(src + 512 * hh, 0, 128, LAYOUT_NONE));
-                                tmem_cp_32x128b(sfx_at + 8 * c, smem_desc(src + MH * 512, 0, 128, LAYOUT_NONE));
-                                if (C::X_CHUNKS == 2 && n > 128)
-                                    tmem_cp_32x128b(sfx_at + 8 * c + 4, smem_desc(src + MH * 512 + 512, 0, 128, LAYOUT_NONE));
-                            }
-                        }
-                        const uint64_t w_desc = smem_desc(st + h * 16384, 16, 1024, LAYOUT_SW128);
-                        const uint32_t d = tmem + a * C::ACC_STRIDE;
+                    if (ok) copy_scales(it, halves, n);
+                }
+                copied = false;
+                auto products = [&](int h, int a) {
+                    const uint64_t w_desc = smem_desc(st + h * 16384, 16, 1024, LAYOUT_SW128), x_desc = smem_desc(st + C::W_BYTES, 16, 1024, LAYOUT_SW128);
+                    const uint32_t d = tmem + a * C::ACC_STRIDE, sfw = tmem + C::SFW_COL + set + 4 * h, sfx = tmem + C::SFX_COL + set;
+                    if (elect_one()) {
 #pragma unroll
                         for (uint32_t k = 0; k < 4; ++k) {
                             const uint32_t acc = (kt > 0 || k > 0) ? 1u : 0u;
                             if constexpr (C::MXF4) {
                                 const uint32_t id = (k & 1u) * 2u;                 // 64 elements: scale bytes (0, 1) or (2, 3) of step k / 2
-                                mma_mxf4(d, w_desc + 2 * k, x_desc + 2 * k, idesc_n | (id << 29) | (id << 4),
-                                         sfw_at + 8 * (k >> 1) + 4 * h, sfx_at + 8 * (k >> 1), acc);
+                                mma_mxf4(d, w_desc + 2 * k, x_desc + 2 * k, idesc_n | (id << 29) | (id << 4), sfw + 8 * (k >> 1), sfx + 8 * (k >> 1), acc);
                             } else {
-                                mma_mxf8f6f4(d, w_desc + 2 * k, x_desc + 2 * k, idesc_n | (k << 29) | (k << 4),
-                                             sfw_at + 4 * h, sfx_at, acc);
+                                mma_mxf8f6f4(d, w_desc + 2 * k, x_desc + 2 * k, idesc_n | (k << 29) | (k << 4), sfw, sfx, acc);
                             }
                         }
-                        if (h == halves - 1) mma_commit(empty_bar(s));
                     }
                     __syncwarp();
+                };
+                // the first product into an accumulator overwrites it: the epilogue must have read what it held
+                auto free_accumulator = [&](int a, uint32_t uses) {
+                    if (kt == 0 && uses > 0 && ok) { ok = mbar_wait(accum_empty(a), (uses - 1) & 1, p.status, ST_MMA_TIMEOUT); tc_fence_after(); }
+                    return ok;
+                };
+                if (MH == 2 && free_accumulator(0, count)) products(0, 0);
+                if (ok && (kt + 1 < KT || more) && mbar_test_wait(full_bar((it + 1) % STAGES), ((it + 1) / STAGES) & 1)) {
+                    tc_fence_after();
+                    copy_scales(it + 1, kt + 1 < KT ? halves : next_halves, kt + 1 < KT ? n : next_n);
+                    copied = true;
                 }
+                if constexpr (MH == 2) {
+                    if (halves == 2 && free_accumulator(1, count)) products(1, 1);
+                } else {
+                    if (free_accumulator(buf, count >> 1)) products(0, buf);
+                }
+                if (ok && elect_one()) mma_commit(empty_bar(s));
+                __syncwarp();
             }
-            if (lane == 0) mma_commit(accum_full(buf));
+            if (elect_one()) mma_commit(accum_full(buf));
             __syncwarp();
         }
         if (!ok) {
             // unwinding after a wait that ran out: the MMAs already issued must finish before tensor memory is freed
-            if (lane == 0) mma_commit(drain_bar);
+            if (elect_one()) mma_commit(drain_bar);
             __syncwarp();
             mbar_wait(drain_bar, 0, nullptr, 0);
         }
@@ -757,14 +798,14 @@ static int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 
 // Tile shape of a call, from the sizes that the host knows.
 struct Plan {
-    bool narrow;                 // 128 features, up to 128 rows (else 256 and 240)
+    bool narrow;                 // 128 features, up to 128 rows (else 256, and 240 or 224)
     int width;
     int chunks() const { return narrow ? 1 : 2; }
     int64_t sf_bytes(int64_t rows, int64_t groups, int64_t K) const { return (rows / width + groups + 1) * ((K + 127) / 128) * chunks() * 512; }
 };
-static Plan make_plan(int64_t rows, int64_t groups) {
+static Plan make_plan(int64_t rows, int64_t groups, bool fp4) {
     const bool narrow = rows / groups <= 128;
-    return Plan{narrow, narrow ? Narrow::BT : Wide::BT};
+    return Plan{narrow, narrow ? Narrow::BT : fp4 ? WideFp4::BT : Wide::BT};
 }
 
 }  // namespace grouped
@@ -776,7 +817,7 @@ extern "C" int mxq_mx_max_groups(void) { return grouped::MAX_GROUPS; }
 
 extern "C" int64_t mxq_mx_grouped_scratch_bytes(int64_t rows_in, int64_t rows, int64_t K, int64_t groups) {
     if (rows_in < 0 || rows < 0 || groups <= 0 || K <= 0 || K % 32 != 0) return MXQ_EINVAL;
-    return grouped::align256(rows * K) + grouped::align256(grouped::make_plan(rows, groups).sf_bytes(rows, groups, K)) + grouped::align256(rows_in * K) +
+    return grouped::align256(rows * K) + grouped::align256(grouped::make_plan(rows, groups, true).sf_bytes(rows, groups, K)) + grouped::align256(rows_in * K) +
            grouped::align256(rows_in * K / 32);
 }
 
@@ -804,7 +845,7 @@ extern "C" int mxq_mx_grouped_linear(const void* x, int x_dtype, int64_t rows_in
     if (!grouped::valid_mx_preset(x_exp_bits, x_frac_bits) || x_round_mode < MXQ_RN || x_round_mode > MXQ_RZ) return MXQ_EINVAL;
     const int x_fmt = x_exp_bits == 5 ? 1 : 0;
 
-    const grouped::Plan plan = grouped::make_plan(rows, groups);
+    const grouped::Plan plan = grouped::make_plan(rows, groups, fp4);
     const grouped::Groups g{offsets, offsets64, (int)rows, (int)groups, plan.width};
     uint8_t* codes = static_cast<uint8_t*>(scratch);
     uint8_t* sf = codes + grouped::align256(rows * K);
