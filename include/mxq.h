@@ -374,11 +374,12 @@ int mxq_mx_max_groups(void);
  *               clamped to [0, rows] and one that lies below an earlier one counts as that one, so that no content
  *               of the array reaches outside the buffers.  NULL: one group of all rows (groups == 1).
  *   zero_rest : rows of out outside every group are set to zero; otherwise they are left as they are.
- *   scratch   : 256-byte aligned, at least mxq_mx_grouped_scratch_bytes(rows_in, rows, K, groups) bytes, of this call alone.
+ *   scratch   : 256-byte aligned, at least mxq_mx_grouped_scratch_bytes(...) bytes, of this call alone; that is 0, and scratch may
+ *               be NULL, for a few rows per group on 16 bytes (one kernel that keeps the quantised rows on the chip).
  * `extra` may be the same buffer as `out`.  K % 32 == 0, w_hw_format / w_codes / w_sf from mxq_mx_pack_experts.
  * `status` as for mxq_mx_gemm.
  */
-int64_t mxq_mx_grouped_scratch_bytes(int64_t rows_in, int64_t rows, int64_t K, int64_t groups);
+int64_t mxq_mx_grouped_scratch_bytes(const void* x, int x_round_mode, int64_t rows_in, int64_t rows, int64_t K, int64_t groups);
 int mxq_mx_grouped_linear(const void* x, int x_dtype, int64_t rows_in, int64_t rows, int64_t K, int x_exp_bits,
                           int x_frac_bits, int x_round_mode, const void* row_index, int index64,
                           const uint8_t* w_codes, const uint8_t* w_sf, int w_hw_format, int64_t groups, int64_t N,

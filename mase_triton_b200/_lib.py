@@ -50,7 +50,7 @@ SIGNATURES = {
     "mxq_version": [],
 }
 _I64_FUNCS = {"mxq_mx_sf_bytes": [_i64, _i64, _i, _i], "mxq_packed_bytes": [_i64, _i], "mxq_mx_linear_scratch_bytes": [_i64, _i64],
-              "mxq_mx_linear_static_capacity": [], "mxq_mx_grouped_scratch_bytes": [_i64, _i64, _i64, _i64]}
+              "mxq_mx_linear_static_capacity": [], "mxq_mx_grouped_scratch_bytes": [_p, _i, _i64, _i64, _i64, _i64]}
 _STRING_FUNCS = {"mxq_status_string": [_i], "mxq_last_cuda_error": []}
 
 _lib = None
@@ -97,6 +97,10 @@ def require_cuda(t: torch.Tensor, what: str) -> None:
 
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+# the current stream's handle by device index; torch.cuda.current_stream builds a Stream object for it (1.3 us)
+raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def fmt_args(meta) -> tuple[int, int, int, int]:

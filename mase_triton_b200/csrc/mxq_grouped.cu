@@ -20,20 +20,14 @@
 //            ([ceil(N / 256)][ceil(K / 128)][2][512] bytes);
 //   rows:    codes [rows, K], scales [tile slot][ceil(K / 128)][chunks][512] bytes.  With tiles of at most `width` rows, tile t of a
 //            group that begins at row f has slot f / width + group + t: no two tiles share one, and no sum over the groups before is needed.
-#include "mxq_device.cuh"
-#include "mxq_tc.cuh"
+#include "mxq_grouped.cuh"
 
 namespace mxq {
 namespace grouped {
 
-using namespace tc;
-
-constexpr int MAX_GROUPS = MX_MAX_GROUPS;
 constexpr int EPI_WARPS = 8;                     // two per TMEM lane quadrant
 constexpr int FIRST_EPI_WARP = 4;                // warps 0, 1, 3: weight copies, MMA issuer, row copies
 constexpr int THREADS = (FIRST_EPI_WARP + EPI_WARPS) * 32;
-
-enum : int { X_NONE = MXQ_EXTRA_NONE, X_MUL = MXQ_EXTRA_MULTIPLY, X_ADD = MXQ_EXTRA_ADD };
 
 // MH: 128-feature halves of a tile; BT: widest row tile; MXF4: both operands packed E2M1 nibbles (256 elements of K per 128 bytes)
 template <int MH_, int BT_, int STAGES_, bool MXF4_> struct Cfg {
@@ -63,202 +57,6 @@ using Wide = Cfg<2, 240, 3, false>;
 using WideFp4 = Cfg<2, 224, 3, true>;
 using Narrow = Cfg<1, 128, 6, false>;
 using NarrowFp4 = Cfg<1, 128, 5, true>;
-
-template <int DT> struct Elem;
-template <> struct Elem<MXQ_F32> { typedef float T; };
-template <> struct Elem<MXQ_BF16> { typedef __nv_bfloat16 T; };
-template <> struct Elem<MXQ_F16> { typedef __half T; };
-__device__ __forceinline__ float widen(float v) { return v; }
-__device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float widen(__half v) { return __half2float(v); }
-__device__ __forceinline__ void narrow(float v, float& o) { o = v; }
-__device__ __forceinline__ void narrow(float v, __nv_bfloat16& o) { o = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void narrow(float v, __half& o) { o = __float2half_rn(v); }
-
-// Four consecutive features of a row as one 8-byte (fp32: 16-byte) access; `left` of the row's features begin here, `vector`: rows and
-// base are aligned to four.  Held as words: a struct of four 16-bit values is copied member by member, i.e. in 2-byte accesses.
-template <class T> struct Words { typedef uint2 V; };
-template <> struct Words<float> { typedef uint4 V; };
-template <class T> union Four {
-    typename Words<T>::V w;
-    T v[4];
-    __device__ __forceinline__ Four() {}
-};
-template <class T> __device__ __forceinline__ void load_four(const T* at, int left, int vector, Four<T>& o) {
-    if (vector) { if (left > 0) o.w = __ldcg(reinterpret_cast<const typename Words<T>::V*>(at)); return; }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) if (k < left) o.v[k] = at[k];
-}
-template <class T> __device__ __forceinline__ void store_four(T* at, int left, int vector, const Four<T>& o) {
-    if (vector) { if (left > 0) *reinterpret_cast<typename Words<T>::V*>(at) = o.w; return; }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) if (k < left) at[k] = o.v[k];
-}
-
-// z * sigmoid(2u) is 0.5 z (1 + tanh u); exp overflows to Inf for very negative arguments and the quotient is then 0
-__device__ __forceinline__ float sigmoid_times(float z, float a) { return __fdividef(z, 1.0f + __expf(-a)); }
-template <int ACT> __device__ __forceinline__ float activate(float z) {
-    if constexpr (ACT == MXQ_ACT_RELU) return z < 0.0f ? 0.0f : z;                       // NaN stays NaN
-    else if constexpr (ACT == MXQ_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-    else if constexpr (ACT == MXQ_ACT_GELU_TANH) return sigmoid_times(z, 1.5957691216057308f * (z + 0.044715f * z * z * z));
-    else if constexpr (ACT == MXQ_ACT_SILU) return sigmoid_times(z, z);
-    else return z;
-}
-// The epilogue of one lane's 4 x 4 values: rows at, at + 4 * pitch, ... (`rows` of them exist, at most four), four features each.
-// The choices are made once for all sixteen: a switch per value costs more than the values.
-template <int ACT, class T>
-__device__ __forceinline__ void finish(const float* slot, int lane, const float (&bias)[4], const Four<T> (&extra)[4], int extra_mode, T* at, int64_t pitch, int rows,
-                                       int left, int vector) {
-    float y[16];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float4 v = reinterpret_cast<const float4*>(slot)[i * 32 + lane];
-        y[4 * i] = v.x; y[4 * i + 1] = v.y; y[4 * i + 2] = v.z; y[4 * i + 3] = v.w;
-    }
-#pragma unroll
-    for (int k = 0; k < 16; ++k) y[k] = activate<ACT>(y[k] + bias[k & 3]);
-    if (extra_mode == X_MUL) {
-#pragma unroll
-        for (int k = 0; k < 16; ++k) y[k] *= widen(extra[k >> 2].v[k & 3]);
-    } else if (extra_mode == X_ADD) {
-#pragma unroll
-        for (int k = 0; k < 16; ++k) y[k] += widen(extra[k >> 2].v[k & 3]);
-    }
-    Four<T> o[4];
-#pragma unroll
-    for (int k = 0; k < 16; ++k) narrow(y[k], o[k >> 2].v[k & 3]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) if (i < rows) store_four(at + i * 4 * pitch, left, vector, o[i]);
-}
-
-// one thread of a converged warp, the same one each time
-__device__ __forceinline__ bool elect_one() {
-    uint32_t pred;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(pred));
-    return pred != 0;
-}
-// whether a barrier's phase has completed, without waiting
-__device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-    return ok != 0;
-}
-
-// where a unit of work lies: features [f0, f0 + FEATURES) of group g for rows [row, row + rows)
-struct Unit {
-    int g, f0, ftile, row, rows, slot;
-    __device__ __forceinline__ uint32_t padded() const { return (uint32_t)(rows + 15) & ~15u; }
-};
-
-// Rows per tile of a group of n rows cut into tt = ceil(n / width) tiles: equal, a multiple of 16, at most `width`; the last tile is never empty.
-__device__ __forceinline__ int tile_rows(int n, int tt) { return ((n + tt - 1) / tt + 15) & ~15; }
-
-// The group table (tile counts summed over the groups, first rows) and the walk over the units of one CTA.
-struct Walk {
-    const int *tiles, *first;
-    int g, ftiles, width, total;
-    __device__ __forceinline__ Walk(const int* t, const int* f, int groups, int ftiles_, int width_)
-        : tiles(t), first(f), g(0), ftiles(ftiles_), width(width_), total(t[groups] * ftiles_) {}
-    __device__ __forceinline__ Unit at(int u, int features) {
-        while (u >= tiles[g + 1] * ftiles) ++g;                              // units are visited in rising order
-        const int tt = tiles[g + 1] - tiles[g], begin = first[g], n = first[g + 1] - begin;
-        int ti, fi;
-        tile_coords(u - tiles[g] * ftiles, tt, ftiles, ti, fi);
-        const int w = tile_rows(n, tt);
-        return Unit{g, fi * features, fi, begin + ti * w, min(w, n - ti * w), begin / width + g + ti};
-    }
-};
-
-// The rows of a call and how they are grouped.
-struct Groups {
-    const void* offsets;         // [groups + 1], or null: one group of all rows
-    int offsets64, rows, groups;
-    int width;                   // rows per tile at most (a multiple of 16)
-    __device__ __forceinline__ int offset(int i) const {
-        if (offsets == nullptr) return i == 0 ? 0 : rows;
-        const int64_t v = offsets64 ? reinterpret_cast<const long long*>(offsets)[i] : (int64_t)reinterpret_cast<const int*>(offsets)[i];
-        return (int)min(max(v, (int64_t)0), (int64_t)rows);
-    }
-};
-
-// One warp: first[i] = the largest of offsets[0 .. i] (offsets that fall back leave an empty group and never an overlap),
-// tiles[i] = row tiles of the groups before i.
-__device__ __forceinline__ void build_table(const Groups& g, int* tiles, int* first, int lane) {
-    int high = 0, sum = 0;
-    for (int base = 0; base <= g.groups; base += 32) {
-        const int i = base + lane;
-        int v = i <= g.groups ? g.offset(i) : 0;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) { const int up = __shfl_up_sync(~0u, v, o); if (lane >= o) v = max(v, up); }
-        v = max(v, high);
-        const int before = __shfl_up_sync(~0u, v, 1);
-        // rows of group i - 1, which the running sum at i counts
-        int t = (i == 0 || i > g.groups) ? 0 : ((v - (lane == 0 ? high : before)) + g.width - 1) / g.width;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) { const int up = __shfl_up_sync(~0u, t, o); if (lane >= o) t += up; }
-        t += sum;
-        if (i <= g.groups) { first[i] = v; tiles[i] = t; }
-        high = __shfl_sync(~0u, v, 31);
-        sum = __shfl_sync(~0u, t, 31);
-    }
-}
-
-// Where the scales of one row lie: its tile's slot and its row in the tile.
-struct Place {
-    int slot, r;
-    __device__ __forceinline__ Place() : slot(-1), r(0) {}
-    __device__ __forceinline__ Place(const Groups& g, int group, int begin, int end, int row) {
-        const int n = end - begin, w = tile_rows(n, (n + g.width - 1) / g.width), t = (row - begin) / w;
-        slot = begin / g.width + group + t;
-        r = row - begin - t * w;
-    }
-    // byte of K block kb: chunk r / 128 of its 128-element step, (r % 32) * 16 + (r % 128 / 32) * 4 + kb % 4 within
-    __device__ __forceinline__ int64_t at(int kb, int KT128, int chunks) const {
-        return (((int64_t)slot * KT128 + (kb >> 2)) * chunks + (r >> 7)) * 512 + (r & 31) * 16 + ((r & 127) >> 5) * 4 + (kb & 3);
-    }
-};
-
-// The whole CTA: place of one row, slot -1 for a row of no group.  The group is the first whose end lies behind the row (in the
-// running maximum of the offsets, that is the first offset behind it), its begin the largest offset up to there.
-__device__ __forceinline__ Place find_row(const Groups& g, int row, int* s_two) {
-    if (g.offsets == nullptr) return Place(g, 0, 0, g.rows, row);
-    if (threadIdx.x == 0) { s_two[0] = g.groups; s_two[1] = 0; }
-    __syncthreads();
-    int group = g.groups;
-    for (int e = threadIdx.x; e < g.groups && group == g.groups; e += blockDim.x) if (g.offset(e + 1) > row) group = e;
-    group = __reduce_min_sync(~0u, group);
-    if ((threadIdx.x & 31) == 0) atomicMin(&s_two[0], group);
-    __syncthreads();
-    group = s_two[0];
-    if (group == g.groups) return Place();
-    int begin = 0;
-    for (int e = threadIdx.x; e <= group; e += blockDim.x) begin = max(begin, g.offset(e));
-    begin = __reduce_max_sync(~0u, begin);
-    if ((threadIdx.x & 31) == 0) atomicMax(&s_two[1], begin);
-    __syncthreads();
-    begin = s_two[1];
-    return begin > row ? Place() : Place(g, group, begin, g.offset(group + 1), row);
-}
-
-struct Params {
-    const uint8_t* w_sf;         // weight scales, w_sf_group bytes per group
-    int64_t w_sf_group;
-    const uint8_t* x_sf;         // row scales
-    void* out;
-    const void* bias;            // [groups, N] or null
-    const void* extra;           // [rows, N] or null
-    Groups rows;
-    int N, K;
-    int act, extra_mode;
-    int zero_rest;               // write zeros into the rows that belong to no group
-    int vector;                  // out, extra and their rows are aligned to four elements
-    uint32_t idesc;              // instruction descriptor without the width
-    int* status;
-};
 
 template <class C, int DT>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -508,13 +306,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                         else if (h + 1 < halves) request(h + 1, side);
                         T* at = out + (size_t)(t.row + c * 16 + er) * p.N + f;
                         const int rows = (t.rows - c * 16 - er + 3) >> 2, left = p.N - f;
-                        switch (p.act) {
-                            case MXQ_ACT_RELU: finish<MXQ_ACT_RELU>(slot, lane, bias, now, p.extra_mode, at, p.N, rows, left, p.vector); break;
-                            case MXQ_ACT_GELU: finish<MXQ_ACT_GELU>(slot, lane, bias, now, p.extra_mode, at, p.N, rows, left, p.vector); break;
-                            case MXQ_ACT_GELU_TANH: finish<MXQ_ACT_GELU_TANH>(slot, lane, bias, now, p.extra_mode, at, p.N, rows, left, p.vector); break;
-                            case MXQ_ACT_SILU: finish<MXQ_ACT_SILU>(slot, lane, bias, now, p.extra_mode, at, p.N, rows, left, p.vector); break;
-                            default: finish<MXQ_ACT_NONE>(slot, lane, bias, now, p.extra_mode, at, p.N, rows, left, p.vector); break;
-                        }
+                        finish_any(p.act, slot, lane, bias, now, p.extra_mode, at, p.N, rows, left, p.vector);
                         __syncwarp();
                     }
                 } else {
@@ -524,15 +316,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                 }
             }
         }
-        if (p.zero_rest) {
-            // rows before the first group and behind the last one
-            const int lo = first[0], hi = first[p.rows.groups];
-            const int64_t rest = (int64_t)(lo + p.rows.rows - hi) * p.N;
-            for (int64_t i = (int64_t)blockIdx.x * (EPI_WARPS * 32) + (threadIdx.x - FIRST_EPI_WARP * 32); i < rest; i += (int64_t)gridDim.x * (EPI_WARPS * 32)) {
-                const int64_t before = (int64_t)lo * p.N;
-                narrow(0.0f, out[i < before ? i : i - before + (int64_t)hi * p.N]);
-            }
-        }
+        if (p.zero_rest) zero_rows_outside(out, first[0], first[p.rows.groups], p.rows.rows, p.N, threadIdx.x - FIRST_EPI_WARP * 32, EPI_WARPS * 32);
     }
     tc_fence_before();
     __syncthreads();
@@ -612,11 +396,8 @@ __global__ void __launch_bounds__(256) pack_rows_kernel(const uint8_t* __restric
     *sf_at = (uint8_t)((any_bad && scale < 255u) ? scale + 1u : scale);
 }
 
-// One pass from x to the operand (built-in round-to-nearest formats, 16-byte aligned rows): 8 elements per lane, the 4 lanes of a
-// block agree on its maximum by shuffles, every lane derives the scale, quantises (the dequantised quotient in fp32, as the
-// fused quantise-dequantise kernel forms it) and converts to the hardware's codes, which is exact.  A block with a value that
-// the hardware's format lacks is stored as (scale + 1, elements / 2).  One CTA per row segment: the row is looked up once.
-// OUT: the operand's format, 0 = E4M3 bytes, 1 = E5M2 bytes, 5 = E2M1 nibbles.
+// One pass from x to the operand (built-in round-to-nearest formats, 16-byte aligned rows): 8 elements per lane and access.  One
+// CTA per row segment: the row's group and place are looked up once.
 // Bound by memory (x read once, gathered rows mostly from L2) and integer issue about equally.
 constexpr int QUANT_ACCESSES = 2;                // accesses of 8 elements per lane
 template <class KIn, class F, int OUT>
@@ -626,7 +407,6 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restri
     // everything before this kernel has completed; then the product may start: until it waits for this kernel it only reads what is older
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (early) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const F f{};
     constexpr int BYTES = 8 * KIn::size;
     const int K = o_.K;
     const int row = (int)(blockIdx.x / (unsigned)segments);
@@ -651,52 +431,13 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restri
 #pragma unroll
     for (int a = 0; a < QUANT_ACCESSES; ++a) {
         const int k = first + a * (int)blockDim.x * 8;
-        uint32_t b[8], amax = 0;
+        uint32_t b[8], o[OUT == 5 ? 1 : 2];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             if constexpr (KIn::size == 4) b[i] = raw[a][i];
             else b[i] = KIn::to_bits(i & 1 ? raw[a][i >> 1] >> 16 : raw[a][i >> 1] & 0xFFFFu);
-            amax = max(amax, b[i] & 0x7FFFFFFFu);
         }
-        amax = max(amax, __shfl_xor_sync(~0u, amax, 1));
-        amax = max(amax, __shfl_xor_sync(~0u, amax, 2));
-        uint32_t sbyte = 0;
-        const uint32_t header = block_header(amax, f);                       // 2^-se, the scale byte, and whether the block holds Inf / NaN
-        sbyte = (header >> 8) & 0xFFu;
-        const float inv = __uint_as_float(header & 0x7F800000u);
-        const bool special = header & 1u;
-        float v[8];
-        bool bad = false;
-        constexpr float hw_max = OUT == 0 ? 448.0f : OUT == 1 ? 57344.0f : 6.0f;
-        constexpr float fmt_max = F{}.eb() == 4 ? 480.0f : F{}.eb() == 5 ? 114688.0f : 0.0f;     // the formats whose largest value the hardware lacks
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint32_t qb = mx_quotient_bits(b[i], inv);
-            const uint32_t y = special ? 0u : qdq_mag_bits(qb, f);
-            if constexpr (fmt_max > hw_max) bad |= __uint_as_float(y) > hw_max;
-            v[i] = __uint_as_float(y | (qb & 0x80000000u));
-        }
-        if constexpr (fmt_max > hw_max) {
-            uint32_t any = bad ? 1u : 0u;
-            any |= __shfl_xor_sync(~0u, any, 1);
-            any |= __shfl_xor_sync(~0u, any, 2);
-            if (any) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] *= 0.5f;
-                sbyte += sbyte < 255u ? 1u : 0u;
-            }
-        }
-        if (special) sbyte = 255u;                                           // NaN to the tensor cores, whatever the codes
-        uint32_t o[2] = {0u, 0u};
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-            uint16_t two;
-            if constexpr (OUT == 0) asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(v[i + 1]), "f"(v[i]));
-            else if constexpr (OUT == 1) asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(two) : "f"(v[i + 1]), "f"(v[i]));
-            else asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %1, %2;\n\tcvt.u16.u8 %0, t;\n\t}" : "=h"(two) : "f"(v[i + 1]), "f"(v[i]));
-            if constexpr (OUT == 5) o[0] |= (uint32_t)two << (4 * i);
-            else o[i >> 2] |= (uint32_t)two << (8 * (i & 2));
-        }
+        const uint32_t sbyte = quantise_part<F, OUT, 8>(b, o);
         if (k < K) {
             if constexpr (OUT == 5) *reinterpret_cast<uint32_t*>(o_.codes + ((int64_t)row * K + k) / 2) = o[0];
             else *reinterpret_cast<uint2*>(o_.codes + (int64_t)row * K + k) = make_uint2(o[0], o[1]);
@@ -709,23 +450,6 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restri
         }
     }
     if (!early) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
-
-template <class... KArgs, class... Args>
-static int launch_after(void (*kernel)(KArgs...), unsigned grid, unsigned block, unsigned smem, cudaStream_t st, Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(block);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
-    if (e != cudaSuccess) { set_last_cuda_error(e); return MXQ_ELAUNCH; }
-    return check_launch();
 }
 
 // MXQ_ESIZE: not covered (a rounding mode other than to nearest, unaligned rows), take extract + pack_rows_kernel
@@ -741,30 +465,12 @@ static int quantize_rows(const void* x, int x_dtype, const void* row_index, int 
     int rc = MXQ_ESIZE;
     with_kind(x_dtype, [&](auto kin) {
         using KIn = decltype(kin);
-        with_preset(eb, fb, 1, rm, [&](auto fmt) {
-            using F = decltype(fmt);
-            auto go = [&](auto out) {
-                rc = launch_after(quantize_rows_kernel<KIn, F, decltype(out)::value>, (unsigned)(rows * segments), (unsigned)block, 0, st, x, row_index, index64,
-                                  rows_in, g, o, (int)segments, early);
-            };
-            if constexpr (F{}.eb() == 5) go(std::integral_constant<int, 1>{});
-            else if constexpr (F{}.eb() == 2 && F{}.fb() == 1) { if (o.nibbles) go(std::integral_constant<int, 5>{}); else go(std::integral_constant<int, 0>{}); }
-            else go(std::integral_constant<int, 0>{});
+        with_row_format(eb, fb, o.nibbles, [&](auto fmt, auto out) {
+            rc = launch_after(quantize_rows_kernel<KIn, decltype(fmt), decltype(out)::value>, (unsigned)(rows * segments), (unsigned)block, 0, st, x, row_index,
+                              index64, rows_in, g, o, (int)segments, early);
         });
     });
     return rc;
-}
-
-// box of `box_rows` rows x 128 bytes of a [rows, K] operand
-static bool make_map(CUtensorMap* map, const void* codes, int64_t rows, int64_t K, int box_rows, bool nibbles) {
-    EncodeTiledFn fn = encode_tiled_fn();
-    if (!fn) return false;
-    const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)(nibbles ? K / 2 : K)};
-    const cuuint32_t box[2] = {(cuuint32_t)(nibbles ? 256 : 128), (cuuint32_t)box_rows};
-    const cuuint32_t estr[2] = {1, 1};
-    return fn(map, nibbles ? CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN8B : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, box, estr,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <class C, int DT>
@@ -776,10 +482,8 @@ static int launch(const Params& p, const uint8_t* w_codes, const uint8_t* x_code
     const Groups& g = p.rows;
     if (!make_map(&mw, w_codes, (int64_t)g.groups * p.N, p.K, 128, C::MXF4) || !make_map(&mx64, x_codes, g.rows, p.K, 64, C::MXF4) ||
         !make_map(&mx16, x_codes, g.rows, p.K, 16, C::MXF4)) return MXQ_ELAUNCH;
-    // units at most: every group may end in a partial tile; what the groups leave is known on the device only
-    const int64_t ftiles = (p.N + C::FEATURES - 1) / C::FEATURES;
-    const int64_t most = (int64_t)(g.rows / g.width + (g.groups < g.rows ? g.groups : g.rows)) * ftiles;
-    const int grid = (int)(most < sm_count() ? most : sm_count());
+    const int64_t units = most_units(g, p.N, C::FEATURES);
+    const int grid = (int)(units < sm_count() ? units : sm_count());
     return launch_after(grouped_kernel<C, DT>, (unsigned)grid, THREADS, C::SMEM_BYTES, st, mw, mx64, mx16, p);
 }
 
@@ -796,8 +500,9 @@ static bool valid_mx_preset(int eb, int fb) {
 }
 static int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 
-// Tile shape of a call, from the sizes that the host knows.
+// Kernel and tile shape of a call, from the sizes that the host knows.
 struct Plan {
+    bool decode;                 // a few rows per group: mxq_grouped_decode.cu, where x and its format allow
     bool narrow;                 // 128 features, up to 128 rows (else 256, and 240 or 224)
     int width;
     int chunks() const { return narrow ? 1 : 2; }
@@ -805,7 +510,7 @@ struct Plan {
 };
 static Plan make_plan(int64_t rows, int64_t groups, bool fp4) {
     const bool narrow = rows / groups <= 128;
-    return Plan{narrow, narrow ? Narrow::BT : fp4 ? WideFp4::BT : Wide::BT};
+    return Plan{groups == 1 ? rows <= decode_rows() : rows / groups <= decode_rows() / 2, narrow, narrow ? Narrow::BT : fp4 ? WideFp4::BT : Wide::BT};
 }
 
 }  // namespace grouped
@@ -815,10 +520,16 @@ using namespace mxq;
 
 extern "C" int mxq_mx_max_groups(void) { return grouped::MAX_GROUPS; }
 
-extern "C" int64_t mxq_mx_grouped_scratch_bytes(int64_t rows_in, int64_t rows, int64_t K, int64_t groups) {
+// the decode kernel quantises by itself: no operand in memory
+static bool takes_decode(const grouped::Plan& plan, const void* x, int round_mode) {
+    return plan.decode && round_mode == MXQ_RN && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+}
+
+extern "C" int64_t mxq_mx_grouped_scratch_bytes(const void* x, int round_mode, int64_t rows_in, int64_t rows, int64_t K, int64_t groups) {
     if (rows_in < 0 || rows < 0 || groups <= 0 || K <= 0 || K % 32 != 0) return MXQ_EINVAL;
-    return grouped::align256(rows * K) + grouped::align256(grouped::make_plan(rows, groups, true).sf_bytes(rows, groups, K)) + grouped::align256(rows_in * K) +
-           grouped::align256(rows_in * K / 32);
+    const grouped::Plan plan = grouped::make_plan(rows, groups, true);
+    if (rows == 0 || takes_decode(plan, x, round_mode)) return 0;
+    return grouped::align256(rows * K) + grouped::align256(plan.sf_bytes(rows, groups, K)) + grouped::align256(rows_in * K) + grouped::align256(rows_in * K / 32);
 }
 
 extern "C" int mxq_mx_grouped_linear(const void* x, int x_dtype, int64_t rows_in, int64_t rows, int64_t K, int x_exp_bits, int x_frac_bits,
@@ -834,9 +545,11 @@ extern "C" int mxq_mx_grouped_linear(const void* x, int x_dtype, int64_t rows_in
     if (groups > grouped::MAX_GROUPS || rows > (1 << 30) || N > (1 << 30) || K > (1 << 30) || groups * N > (1ll << 31) - 1) return MXQ_ESIZE;
     if (rows * ((K + 127) / 128 * 4) > (1ll << 31) * 255 || rows_in > (1 << 30)) return MXQ_ESIZE;
     if (rows == 0) return MXQ_OK;
-    if ((!x && rows_in > 0) || !w_codes || !w_sf || !out || !scratch || (extra_mode != MXQ_EXTRA_NONE && !extra)) return MXQ_EINVAL;
+    if ((!x && rows_in > 0) || !w_codes || !w_sf || !out || (extra_mode != MXQ_EXTRA_NONE && !extra)) return MXQ_EINVAL;
     if ((reinterpret_cast<uintptr_t>(w_codes) | reinterpret_cast<uintptr_t>(w_sf)) % 16 != 0 || reinterpret_cast<uintptr_t>(scratch) % 256 != 0) return MXQ_EINVAL;
-    if (scratch_bytes < mxq_mx_grouped_scratch_bytes(rows_in, rows, K, groups)) return MXQ_ESIZE;
+    const int64_t needed = mxq_mx_grouped_scratch_bytes(x, x_round_mode, rows_in, rows, K, groups);
+    if (needed > 0 && !scratch) return MXQ_EINVAL;
+    if (scratch_bytes < needed) return MXQ_ESIZE;
     // both operands E2M1 and the weight kept as nibbles: the 4-bit kind
     const bool x_e2m1 = x_exp_bits == 2 && x_frac_bits == 1;
     const bool fp4 = w_hw_format == 5;
@@ -846,14 +559,30 @@ extern "C" int mxq_mx_grouped_linear(const void* x, int x_dtype, int64_t rows_in
     const int x_fmt = x_exp_bits == 5 ? 1 : 0;
 
     const grouped::Plan plan = grouped::make_plan(rows, groups, fp4);
-    const grouped::Groups g{offsets, offsets64, (int)rows, (int)groups, plan.width};
+    grouped::Params p{};
+    p.w_sf = w_sf;
+    p.w_sf_group = mxq_mx_sf_bytes(N, K, MXQ_OPERAND_A, 0);
+    p.out = out; p.bias = bias; p.extra = extra;
+    p.rows = grouped::Groups{offsets, offsets64, (int)rows, (int)groups, plan.width};
+    p.N = (int)N; p.K = (int)K;
+    const uintptr_t four = x_dtype == MXQ_F32 ? 16 : 8;
+    p.vector = N % 4 == 0 && reinterpret_cast<uintptr_t>(out) % four == 0 && reinterpret_cast<uintptr_t>(extra) % four == 0;
+    p.act = activation; p.extra_mode = extra_mode; p.zero_rest = zero_rest; p.status = status;
+    // formats of left (weight) and right (rows) operand, K-major both, E8M0 scales, M >> 4; E2M1 is 1 in the 4-bit kind's encoding
+    p.idesc = (fp4 ? (1u << 7) | (1u << 10) : ((uint32_t)w_hw_format << 7) | ((uint32_t)x_fmt << 10)) | (1u << 23) | ((uint32_t)(128 >> 4) << 24);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (takes_decode(plan, x, x_round_mode)) {
+        p.rows.width = grouped::decode_rows();
+        return grouped::launch_decode(p, x_dtype, x, row_index, index64, rows_in, x_exp_bits, x_frac_bits, fp4, w_codes, st);
+    }
+
     uint8_t* codes = static_cast<uint8_t*>(scratch);
     uint8_t* sf = codes + grouped::align256(rows * K);
     uint8_t* ref_codes = sf + grouped::align256(plan.sf_bytes(rows, groups, K));
     uint8_t* ref_scales = ref_codes + grouped::align256(rows_in * K);
+    p.x_sf = sf;
     const grouped::RowOperand operand{codes, sf, (int)K, plan.chunks(), fp4};
-    cudaStream_t st = (cudaStream_t)stream;
-    int rc = grouped::quantize_rows(x, x_dtype, row_index, index64, rows_in, g, x_exp_bits, x_frac_bits, x_round_mode, operand, st);
+    int rc = grouped::quantize_rows(x, x_dtype, row_index, index64, rows_in, p.rows, x_exp_bits, x_frac_bits, x_round_mode, operand, st);
     if (rc == MXQ_ESIZE) {
         if (rows_in > 0) {
             rc = mxq_mxfp_extract(x, x_dtype, ref_scales, ref_codes, rows_in * K, 32, x_exp_bits, x_frac_bits, 1, x_round_mode, stream);
@@ -863,22 +592,10 @@ extern "C" int mxq_mx_grouped_linear(const void* x, int x_dtype, int64_t rows_in
         int fmt;
         if (!hw_code_tables(x_exp_bits, x_frac_bits, tables.plain, tables.halved, tables.bad, &fmt)) return MXQ_EINVAL;
         const int64_t threads = rows * ((K + 127) / 128 * 4);
-        grouped::pack_rows_kernel<<<(unsigned)((threads + 255) / 256), 256, 0, st>>>(ref_scales, ref_codes, row_index, index64, rows_in, g, operand, tables);
+        grouped::pack_rows_kernel<<<(unsigned)((threads + 255) / 256), 256, 0, st>>>(ref_scales, ref_codes, row_index, index64, rows_in, p.rows, operand, tables);
         rc = check_launch();
     }
     if (rc != MXQ_OK) return rc;
-
-    grouped::Params p{};
-    p.w_sf = w_sf;
-    p.w_sf_group = mxq_mx_sf_bytes(N, K, MXQ_OPERAND_A, 0);
-    p.x_sf = sf;
-    p.out = out; p.bias = bias; p.extra = extra; p.rows = g;
-    p.N = (int)N; p.K = (int)K;
-    const uintptr_t four = x_dtype == MXQ_F32 ? 16 : 8;
-    p.vector = N % 4 == 0 && reinterpret_cast<uintptr_t>(out) % four == 0 && reinterpret_cast<uintptr_t>(extra) % four == 0;
-    p.act = activation; p.extra_mode = extra_mode; p.zero_rest = zero_rest; p.status = status;
-    // formats of left (weight) and right (rows) operand, K-major both, E8M0 scales, M >> 4; E2M1 is 1 in the 4-bit kind's encoding
-    p.idesc = (fp4 ? (1u << 7) | (1u << 10) : ((uint32_t)w_hw_format << 7) | ((uint32_t)x_fmt << 10)) | (1u << 23) | ((uint32_t)(128 >> 4) << 24);
     if (fp4) return plan.narrow ? grouped::launch_dt<grouped::NarrowFp4>(p, x_dtype, w_codes, codes, st) : grouped::launch_dt<grouped::WideFp4>(p, x_dtype, w_codes, codes, st);
     return plan.narrow ? grouped::launch_dt<grouped::Narrow>(p, x_dtype, w_codes, codes, st) : grouped::launch_dt<grouped::Wide>(p, x_dtype, w_codes, codes, st);
 }

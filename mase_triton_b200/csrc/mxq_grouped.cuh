@@ -1,0 +1,331 @@
+// Pieces shared by the kernels of the grouped products (mxq_grouped.cu, mxq_grouped_decode.cu): the group table and the walk over
+// the units of work, the epilogue's arithmetic, launches that may overlap the kernel before them.
+#pragma once
+#include "mxq_device.cuh"
+#include "mxq_tc.cuh"
+
+namespace mxq {
+namespace grouped {
+
+using namespace tc;
+
+constexpr int MAX_GROUPS = MX_MAX_GROUPS;
+enum : int { X_NONE = MXQ_EXTRA_NONE, X_MUL = MXQ_EXTRA_MULTIPLY, X_ADD = MXQ_EXTRA_ADD };
+
+template <int DT> struct Elem;
+template <> struct Elem<MXQ_F32> { typedef float T; };
+template <> struct Elem<MXQ_BF16> { typedef __nv_bfloat16 T; };
+template <> struct Elem<MXQ_F16> { typedef __half T; };
+__device__ __forceinline__ float widen(float v) { return v; }
+__device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float widen(__half v) { return __half2float(v); }
+__device__ __forceinline__ void narrow(float v, float& o) { o = v; }
+__device__ __forceinline__ void narrow(float v, __nv_bfloat16& o) { o = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void narrow(float v, __half& o) { o = __float2half_rn(v); }
+
+// Four consecutive features of a row as one 8-byte (fp32: 16-byte) access; `left` of the row's features begin here, `vector`: rows and
+// base are aligned to four.  Held as words: a struct of four 16-bit values is copied member by member, i.e. in 2-byte accesses.
+template <class T> struct Words { typedef uint2 V; };
+template <> struct Words<float> { typedef uint4 V; };
+template <class T> union Four {
+    typename Words<T>::V w;
+    T v[4];
+    __device__ __forceinline__ Four() {}
+};
+template <class T> __device__ __forceinline__ void load_four(const T* at, int left, int vector, Four<T>& o) {
+    if (vector) { if (left > 0) o.w = __ldcg(reinterpret_cast<const typename Words<T>::V*>(at)); return; }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) if (k < left) o.v[k] = at[k];
+}
+template <class T> __device__ __forceinline__ void store_four(T* at, int left, int vector, const Four<T>& o) {
+    if (vector) { if (left > 0) *reinterpret_cast<typename Words<T>::V*>(at) = o.w; return; }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) if (k < left) at[k] = o.v[k];
+}
+
+// z * sigmoid(2u) is 0.5 z (1 + tanh u); exp overflows to Inf for very negative arguments and the quotient is then 0
+__device__ __forceinline__ float sigmoid_times(float z, float a) { return __fdividef(z, 1.0f + __expf(-a)); }
+template <int ACT> __device__ __forceinline__ float activate(float z) {
+    if constexpr (ACT == MXQ_ACT_RELU) return z < 0.0f ? 0.0f : z;                       // NaN stays NaN
+    else if constexpr (ACT == MXQ_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    else if constexpr (ACT == MXQ_ACT_GELU_TANH) return sigmoid_times(z, 1.5957691216057308f * (z + 0.044715f * z * z * z));
+    else if constexpr (ACT == MXQ_ACT_SILU) return sigmoid_times(z, z);
+    else return z;
+}
+// The epilogue of one lane's 4 x 4 values: rows at, at + 4 * pitch, ... (`rows` of them exist, at most four), four features each.
+// The choices are made once for all sixteen: a switch per value costs more than the values.
+template <int ACT, class T>
+__device__ __forceinline__ void finish(const float* slot, int lane, const float (&bias)[4], const Four<T> (&extra)[4], int extra_mode, T* at, int64_t pitch, int rows,
+                                       int left, int vector) {
+    float y[16];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float4 v = reinterpret_cast<const float4*>(slot)[i * 32 + lane];
+        y[4 * i] = v.x; y[4 * i + 1] = v.y; y[4 * i + 2] = v.z; y[4 * i + 3] = v.w;
+    }
+#pragma unroll
+    for (int k = 0; k < 16; ++k) y[k] = activate<ACT>(y[k] + bias[k & 3]);
+    if (extra_mode == X_MUL) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) y[k] *= widen(extra[k >> 2].v[k & 3]);
+    } else if (extra_mode == X_ADD) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) y[k] += widen(extra[k >> 2].v[k & 3]);
+    }
+    Four<T> o[4];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) narrow(y[k], o[k >> 2].v[k & 3]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) if (i < rows) store_four(at + i * 4 * pitch, left, vector, o[i]);
+}
+
+// one thread of a converged warp, the same one each time
+__device__ __forceinline__ bool elect_one() {
+    uint32_t pred;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(pred));
+    return pred != 0;
+}
+// whether a barrier's phase has completed, without waiting
+__device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+
+template <class T>
+__device__ __forceinline__ void finish_any(int act, const float* slot, int lane, const float (&bias)[4], const Four<T> (&extra)[4], int extra_mode, T* at,
+                                           int64_t pitch, int rows, int left, int vector) {
+    switch (act) {
+        case MXQ_ACT_RELU: finish<MXQ_ACT_RELU>(slot, lane, bias, extra, extra_mode, at, pitch, rows, left, vector); break;
+        case MXQ_ACT_GELU: finish<MXQ_ACT_GELU>(slot, lane, bias, extra, extra_mode, at, pitch, rows, left, vector); break;
+        case MXQ_ACT_GELU_TANH: finish<MXQ_ACT_GELU_TANH>(slot, lane, bias, extra, extra_mode, at, pitch, rows, left, vector); break;
+        case MXQ_ACT_SILU: finish<MXQ_ACT_SILU>(slot, lane, bias, extra, extra_mode, at, pitch, rows, left, vector); break;
+        default: finish<MXQ_ACT_NONE>(slot, lane, bias, extra, extra_mode, at, pitch, rows, left, vector); break;
+    }
+}
+// zeros into the rows before the first group (begin) and behind the last one (end), by `threads` threads of every CTA
+template <class T>
+__device__ __forceinline__ void zero_rows_outside(T* out, int begin, int end, int rows, int N, int thread, int threads) {
+    const int64_t before = (int64_t)begin * N, rest = before + (int64_t)(rows - end) * N;
+    for (int64_t i = (int64_t)blockIdx.x * threads + thread; i < rest; i += (int64_t)gridDim.x * threads)
+        narrow(0.0f, out[i < before ? i : i - before + (int64_t)end * N]);
+}
+
+// E elements of a 32-element block per lane (fp32 bits; the 32 / E lanes of the block are neighbours) -> the tensor cores' codes, and
+// the block's scale byte as the result.  The lanes agree on the block's maximum by shuffles; every lane derives the scale,
+// quantises (the dequantised quotient in fp32, as the fused quantise-dequantise kernel forms it) and converts, which is exact.  A block
+// with a value that the hardware's format lacks becomes (scale + 1, elements / 2).  All lanes of the warp take part.
+// OUT: 0 = E4M3 bytes, 1 = E5M2 bytes, 5 = E2M1 nibbles.
+template <class F, int OUT, int E>
+__device__ __forceinline__ uint32_t quantise_part(const uint32_t (&b)[E], uint32_t (&codes)[OUT == 5 ? E / 8 : E / 4]) {
+    const F f{};
+    uint32_t amax = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) amax = max(amax, b[i] & 0x7FFFFFFFu);
+#pragma unroll
+    for (int o = 1; o < 32 / E; o <<= 1) amax = max(amax, __shfl_xor_sync(~0u, amax, o));
+    const uint32_t header = block_header(amax, f);                       // 2^-se, the scale byte, and whether the block holds Inf / NaN
+    uint32_t sbyte = (header >> 8) & 0xFFu;
+    const float inv = __uint_as_float(header & 0x7F800000u);
+    const bool special = header & 1u;
+    float v[E];
+    bool bad = false;
+    constexpr float hw_max = OUT == 0 ? 448.0f : OUT == 1 ? 57344.0f : 6.0f;
+    constexpr float fmt_max = F{}.eb() == 4 ? 480.0f : F{}.eb() == 5 ? 114688.0f : 0.0f;     // the formats whose largest value the hardware lacks
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const uint32_t qb = mx_quotient_bits(b[i], inv);
+        const uint32_t y = special ? 0u : qdq_mag_bits(qb, f);
+        if constexpr (fmt_max > hw_max) bad |= __uint_as_float(y) > hw_max;
+        v[i] = __uint_as_float(y | (qb & 0x80000000u));
+    }
+    if constexpr (fmt_max > hw_max) {
+        uint32_t any = bad ? 1u : 0u;
+#pragma unroll
+        for (int o = 1; o < 32 / E; o <<= 1) any |= __shfl_xor_sync(~0u, any, o);
+        if (any) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) v[i] *= 0.5f;
+            sbyte += sbyte < 255u ? 1u : 0u;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < E; i += 2) {
+        uint16_t two;
+        if constexpr (OUT == 0) asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(v[i + 1]), "f"(v[i]));
+        else if constexpr (OUT == 1) asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(two) : "f"(v[i + 1]), "f"(v[i]));
+        else asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %1, %2;\n\tcvt.u16.u8 %0, t;\n\t}" : "=h"(two) : "f"(v[i + 1]), "f"(v[i]));
+        constexpr int PER = OUT == 5 ? 8 : 4, BITS = 32 / PER;
+        if (i % PER == 0) codes[i / PER] = two;
+        else codes[i / PER] |= (uint32_t)two << (BITS * (i % PER));
+    }
+    return special ? 255u : sbyte;                                       // 255 is NaN to the tensor cores, whatever the codes
+}
+
+// fn(F, the operand's format) for a built-in round-to-nearest format; `nibbles`: E2M1 stays packed in four bits
+template <class Fn> static void with_row_format(int eb, int fb, bool nibbles, Fn&& fn) {
+    with_preset(eb, fb, 1, MXQ_RN, [&](auto fmt) {
+        using F = decltype(fmt);
+        if constexpr (F{}.eb() == 5) fn(fmt, std::integral_constant<int, 1>{});
+        else if constexpr (F{}.eb() == 2 && F{}.fb() == 1) { if (nibbles) fn(fmt, std::integral_constant<int, 5>{}); else fn(fmt, std::integral_constant<int, 0>{}); }
+        else fn(fmt, std::integral_constant<int, 0>{});
+    });
+}
+
+// where a unit of work lies: features [f0, f0 + FEATURES) of group g for rows [row, row + rows)
+struct Unit {
+    int g, f0, ftile, row, rows, slot;
+    __device__ __forceinline__ uint32_t padded() const { return (uint32_t)(rows + 15) & ~15u; }
+};
+
+// Rows per tile of a group of n rows cut into tt = ceil(n / width) tiles: equal, a multiple of 16, at most `width`; the last tile is never empty.
+__device__ __forceinline__ int tile_rows(int n, int tt) { return ((n + tt - 1) / tt + 15) & ~15; }
+
+// The group table (tile counts summed over the groups, first rows) and the walk over the units of one CTA.
+struct Walk {
+    const int *tiles, *first;
+    int g, ftiles, width, total;
+    __device__ __forceinline__ Walk(const int* t, const int* f, int groups, int ftiles_, int width_)
+        : tiles(t), first(f), g(0), ftiles(ftiles_), width(width_), total(t[groups] * ftiles_) {}
+    __device__ __forceinline__ Unit at(int u, int features) {
+        while (u >= tiles[g + 1] * ftiles) ++g;                              // units are visited in rising order
+        const int tt = tiles[g + 1] - tiles[g], begin = first[g], n = first[g + 1] - begin;
+        int ti, fi;
+        tile_coords(u - tiles[g] * ftiles, tt, ftiles, ti, fi);
+        const int w = tile_rows(n, tt);
+        return Unit{g, fi * features, fi, begin + ti * w, min(w, n - ti * w), begin / width + g + ti};
+    }
+};
+
+// The rows of a call and how they are grouped.
+struct Groups {
+    const void* offsets;         // [groups + 1], or null: one group of all rows
+    int offsets64, rows, groups;
+    int width;                   // rows per tile at most (a multiple of 16)
+    __device__ __forceinline__ int offset(int i) const {
+        if (offsets == nullptr) return i == 0 ? 0 : rows;
+        const int64_t v = offsets64 ? reinterpret_cast<const long long*>(offsets)[i] : (int64_t)reinterpret_cast<const int*>(offsets)[i];
+        return (int)min(max(v, (int64_t)0), (int64_t)rows);
+    }
+};
+
+// One warp: first[i] = the largest of offsets[0 .. i] (offsets that fall back leave an empty group and never an overlap),
+// tiles[i] = row tiles of the groups before i.
+__device__ __forceinline__ void build_table(const Groups& g, int* tiles, int* first, int lane) {
+    int high = 0, sum = 0;
+    for (int base = 0; base <= g.groups; base += 32) {
+        const int i = base + lane;
+        int v = i <= g.groups ? g.offset(i) : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const int up = __shfl_up_sync(~0u, v, o); if (lane >= o) v = max(v, up); }
+        v = max(v, high);
+        const int before = __shfl_up_sync(~0u, v, 1);
+        // rows of group i - 1, which the running sum at i counts
+        int t = (i == 0 || i > g.groups) ? 0 : ((v - (lane == 0 ? high : before)) + g.width - 1) / g.width;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const int up = __shfl_up_sync(~0u, t, o); if (lane >= o) t += up; }
+        t += sum;
+        if (i <= g.groups) { first[i] = v; tiles[i] = t; }
+        high = __shfl_sync(~0u, v, 31);
+        sum = __shfl_sync(~0u, t, 31);
+    }
+}
+
+// Where the scales of one row lie: its tile's slot and its row in the tile.
+struct Place {
+    int slot, r;
+    __device__ __forceinline__ Place() : slot(-1), r(0) {}
+    __device__ __forceinline__ Place(const Groups& g, int group, int begin, int end, int row) {
+        const int n = end - begin, w = tile_rows(n, (n + g.width - 1) / g.width), t = (row - begin) / w;
+        slot = begin / g.width + group + t;
+        r = row - begin - t * w;
+    }
+    // byte of K block kb: chunk r / 128 of its 128-element step, (r % 32) * 16 + (r % 128 / 32) * 4 + kb % 4 within
+    __device__ __forceinline__ int64_t at(int kb, int KT128, int chunks) const {
+        return (((int64_t)slot * KT128 + (kb >> 2)) * chunks + (r >> 7)) * 512 + (r & 31) * 16 + ((r & 127) >> 5) * 4 + (kb & 3);
+    }
+};
+
+// The whole CTA: place of one row, slot -1 for a row of no group.  The group is the first whose end lies behind the row (in the
+// running maximum of the offsets, that is the first offset behind it), its begin the largest offset up to there.
+__device__ __forceinline__ Place find_row(const Groups& g, int row, int* s_two) {
+    if (g.offsets == nullptr) return Place(g, 0, 0, g.rows, row);
+    if (threadIdx.x == 0) { s_two[0] = g.groups; s_two[1] = 0; }
+    __syncthreads();
+    int group = g.groups;
+    for (int e = threadIdx.x; e < g.groups && group == g.groups; e += blockDim.x) if (g.offset(e + 1) > row) group = e;
+    group = __reduce_min_sync(~0u, group);
+    if ((threadIdx.x & 31) == 0) atomicMin(&s_two[0], group);
+    __syncthreads();
+    group = s_two[0];
+    if (group == g.groups) return Place();
+    int begin = 0;
+    for (int e = threadIdx.x; e <= group; e += blockDim.x) begin = max(begin, g.offset(e));
+    begin = __reduce_max_sync(~0u, begin);
+    if ((threadIdx.x & 31) == 0) atomicMax(&s_two[1], begin);
+    __syncthreads();
+    begin = s_two[1];
+    return begin > row ? Place() : Place(g, group, begin, g.offset(group + 1), row);
+}
+
+struct Params {
+    const uint8_t* w_sf;         // weight scales, w_sf_group bytes per group
+    int64_t w_sf_group;
+    const uint8_t* x_sf;         // row scales
+    void* out;
+    const void* bias;            // [groups, N] or null
+    const void* extra;           // [rows, N] or null
+    Groups rows;
+    int N, K;
+    int act, extra_mode;
+    int zero_rest;               // write zeros into the rows that belong to no group
+    int vector;                  // out, extra and their rows are aligned to four elements
+    uint32_t idesc;              // instruction descriptor without the width
+    int* status;
+};
+
+// units of work at most: every group may end in a partial tile; what the groups leave is known on the device only
+static int64_t most_units(const Groups& g, int64_t N, int features) {
+    return (int64_t)(g.rows / g.width + (g.groups < g.rows ? g.groups : g.rows)) * ((N + features - 1) / features);
+}
+
+// mxq_grouped_decode.cu: rows that fit tiles of decode_rows(); x on 16 bytes, a built-in round-to-nearest format
+int decode_rows();
+int launch_decode(const Params& p, int dt, const void* x, const void* row_index, int index64, int64_t rows_in, int eb, int fb, bool nibbles,
+                  const uint8_t* w_codes, cudaStream_t st);
+
+template <class... KArgs, class... Args>
+static int launch_after(void (*kernel)(KArgs...), unsigned grid, unsigned block, unsigned smem, cudaStream_t st, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+    if (e != cudaSuccess) { set_last_cuda_error(e); return MXQ_ELAUNCH; }
+    return check_launch();
+}
+
+// box of `box_rows` rows x 128 bytes of a [rows, K] operand
+static bool make_map(CUtensorMap* map, const void* codes, int64_t rows, int64_t K, int box_rows, bool nibbles) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)(nibbles ? K / 2 : K)};
+    const cuuint32_t box[2] = {(cuuint32_t)(nibbles ? 256 : 128), (cuuint32_t)box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    return fn(map, nibbles ? CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN8B : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace grouped
+}  // namespace mxq

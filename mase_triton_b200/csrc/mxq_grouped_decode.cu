@@ -1,0 +1,427 @@
+// The grouped products for few rows (a decoding step): one kernel, in which the rows are quantised by the CTAs that multiply them.
+//
+// What bounds such a call is one read of the weights and, below some 20 us, everything in front of and behind it: launches, the
+// ramp of the grid, a second kernel's hand-over.  So
+//   * eight warps of every CTA quantise the rows of its tile (16 at most) as they go along K, straight into the ring of
+//     shared memory that the tensor cores read, a stage each in turn: one warp's way through a stage (a load, the block
+//     maximum, the rounding, a proxy fence) takes far longer than the stage's products.  Every CTA repeats this for its own features,
+//     out of L2 and beside the weights' copies, which take longer; there is no second launch, no operand in memory and no workspace;
+//   * the ring holds ten stages of 128 features x 128 elements: 160 KB of weights in flight per SM;
+//   * where the features leave SMs idle, K is split over a cluster of 2 or 4 CTAs.  Each sums its part in tensor memory; the
+//     partial sums go to the CTA that finishes those features through distributed shared memory and are added in the
+//     order of the CTAs, so that results do not depend on which comes first.
+// The layout of weights, the walk over the units and the epilogue are those of mxq_grouped.cu.
+#include "mxq_grouped.cuh"
+
+namespace mxq {
+namespace grouped {
+namespace decode {
+
+constexpr int ROWS = 16;                         // widest row tile: the narrowest the instruction takes
+constexpr int FEATURES = 128;
+constexpr int STAGES = 10;
+constexpr int EPI_WARP = 4, QUANT_WARP = 8, QUANT_WARPS = 8;
+constexpr int THREADS = 512;                     // warps 0, 1: weight copies, MMA issuer; 4..7: epilogue; 8..15: quantisers
+constexpr int W_BYTES = FEATURES * 128, X_BYTES = ROWS * 128;
+constexpr int TMEM_COLS = 128;
+constexpr int ACC_STRIDE = 32, SFW_COL = 64, SFX_COL = 96;
+
+template <bool MXF4> struct Cfg {
+    static constexpr int K_STEP = MXF4 ? 256 : 128, SF_STEPS = MXF4 ? 2 : 1;
+    static constexpr int STAGE_BYTES = W_BYTES + X_BYTES + SF_STEPS * 1024;          // scales: 512 bytes of either operand per 128 elements of K
+    static constexpr int TABLE_END = (256 + 2 * (MAX_GROUPS + 1) * 4 + 15) / 16 * 16;
+    static constexpr int SLOTS = 4 * 2048, EXCHANGE = 3 * 2048;                      // 32 features x 16 rows per epilogue warp, and per part received
+    static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + TABLE_END + SLOTS + EXCHANGE;
+    static_assert(STAGE_BYTES % 1024 == 0, "the 128-byte swizzle repeats every 1024 bytes");
+    static_assert(SMEM_BYTES <= 232448, "more shared memory than a CTA can have");
+};
+
+struct Source {
+    const void* x;
+    const void* row_index;
+    int index64;
+    int64_t rows_in;
+};
+
+__device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// bounded wait for a phase that other CTAs of the cluster complete
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, int* status, int code) {
+    for (uint32_t i = 0; i < SPIN_LIMIT; ++i) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if (ok) return true;
+        if (i > 64) __nanosleep(32);
+    }
+    if (status) *reinterpret_cast<volatile int*>(status) = code;
+    return false;
+}
+
+// DT: type of x, out, bias and extra; F, OUT: element format of the rows and what the tensor cores read of it
+template <int DT, class F, int OUT>
+__global__ void __launch_bounds__(THREADS, 1)
+decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ Params p, const __grid_constant__ Source src, int split) {
+    constexpr bool MXF4 = OUT == 5;
+    using C = Cfg<MXF4>;
+    typedef typename Elem<DT>::T T;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t ring = (raw + 1023u) & ~1023u;
+    uint8_t* ring_ptr = smem_raw + (ring - raw);
+    const uint32_t bars = ring + STAGES * C::STAGE_BYTES;            // full[S], empty[S], accum_full[2], accum_empty[2], drain, parts, tmem slot
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ring_ptr + STAGES * C::STAGE_BYTES + 8 * (2 * STAGES + 6));
+    int* tiles = reinterpret_cast<int*>(ring_ptr + STAGES * C::STAGE_BYTES + 256);
+    int* first = tiles + MAX_GROUPS + 1;
+    float* slots = reinterpret_cast<float*>(ring_ptr + STAGES * C::STAGE_BYTES + C::TABLE_END);
+    float* exchange = slots + C::SLOTS / 4;
+    auto full_bar = [&](int s) { return bars + 8u * s; };
+    auto empty_bar = [&](int s) { return bars + 8u * (STAGES + s); };
+    auto accum_full = [&](int a) { return bars + 8u * (2 * STAGES + a); };
+    auto accum_empty = [&](int a) { return bars + 8u * (2 * STAGES + 2 + a); };
+    const uint32_t drain_bar = bars + 8u * (2 * STAGES + 4), parts_bar = bars + 8u * (2 * STAGES + 5);
+
+    const int warp = __shfl_sync(~0u, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    const int rank = split > 1 ? (int)(blockIdx.x % (unsigned)split) : 0;           // clusters are consecutive CTAs
+    const int quads = 4 / split;                                                     // lane quadrants whose features a CTA finishes
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) { mbar_init(full_bar(s), 2); mbar_init(empty_bar(s), 1); }
+        for (int a = 0; a < 2; ++a) { mbar_init(accum_full(a), 1); mbar_init(accum_empty(a), 4); }
+        mbar_init(drain_bar, 1);
+        mbar_init(parts_bar, (split - 1) * quads + (split == 1 ? 1 : 0));
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    // what the kernels before this one write (rows, offsets, perhaps the weights) is read behind this line only
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (warp == 3) build_table(p.rows, tiles, first, lane);
+    tc_fence_before();
+    __syncthreads();
+    if (split > 1) cluster_barrier();                                // every CTA's barriers exist before another one arrives there
+    tc_fence_after();
+    const uint32_t tmem = __shfl_sync(~0u, *tmem_slot, 0);
+
+    const int KT_all = (p.K + C::K_STEP - 1) / C::K_STEP, KT128 = (p.K + 127) / 128;
+    const int k_begin = rank * KT_all / split, KT = (rank + 1) * KT_all / split - k_begin;     // this CTA's steps of K, one at least
+    const int ftiles = (p.N + FEATURES - 1) / FEATURES;
+    const int u_begin = blockIdx.x / split, u_step = gridDim.x / split;
+    Walk walk(tiles, first, p.rows.groups, ftiles, p.rows.width);
+
+    if (warp == 0) {
+        // ---------------- weight copies ----------------
+        bool ok = true;
+        uint32_t it = 0;
+        for (int u = u_begin; u < walk.total && ok; u += u_step) {
+            const Unit t = walk.at(u, FEATURES);
+            const uint8_t* sf = p.w_sf + (size_t)t.g * p.w_sf_group + (size_t)(t.ftile >> 1) * KT128 * 1024 + (t.ftile & 1) * 512;
+            const int w_row = t.g * p.N + t.f0;
+            for (int kt = k_begin; kt < k_begin + KT && ok; ++kt, ++it) {
+                const int s = it % STAGES;
+                if (it >= STAGES) ok = mbar_wait(empty_bar(s), ((it / STAGES) & 1) ^ 1, p.status, ST_PRODUCER_TIMEOUT);
+                if (!ok) break;
+                if (lane == 0) {
+                    const uint32_t st = ring + s * C::STAGE_BYTES;
+                    mbar_expect_tx(full_bar(s), W_BYTES + C::SF_STEPS * 512u);
+                    tma_load_2d(st, &map_w, kt * C::K_STEP, w_row, full_bar(s));
+#pragma unroll
+                    for (int c = 0; c < C::SF_STEPS; ++c)
+                        bulk_load(st + W_BYTES + X_BYTES + c * 1024, sf + (size_t)(kt * C::SF_STEPS + c) * 1024, 512, full_bar(s));
+                }
+                __syncwarp();
+            }
+        }
+        // every copy must have landed before the CTA gives its shared memory back (returns at once in a run that went well)
+        for (uint32_t j = it > (uint32_t)STAGES ? it - STAGES : 0u; j < it; ++j)
+            mbar_wait(full_bar(j % STAGES), (j / STAGES) & 1, p.status, ST_PRODUCER_TIMEOUT);
+    } else if (warp == 1) {
+        // ---------------- MMA issuer: uniform over the warp, scales one stage ahead (see mxq_grouped.cu) ----------------
+        uint32_t it = 0, count = 0;
+        bool ok = true, copied = false;
+        const uint32_t idesc = p.idesc | ((uint32_t)(ROWS >> 3) << 17);
+        auto copy_scales = [&](uint32_t i) {
+            const uint32_t set = (i & 1u) * (C::SF_STEPS * 8), sf = ring + (i % STAGES) * C::STAGE_BYTES + W_BYTES + X_BYTES;
+            if (elect_one()) {
+#pragma unroll
+                for (int c = 0; c < C::SF_STEPS; ++c) {
+                    tmem_cp_32x128b(tmem + SFW_COL + set + 8 * c, smem_desc(sf + c * 1024, 0, 128, LAYOUT_NONE));
+                    tmem_cp_32x128b(tmem + SFX_COL + set + 8 * c, smem_desc(sf + c * 1024 + 512, 0, 128, LAYOUT_NONE));
+                }
+            }
+            __syncwarp();
+        };
+        for (int u = u_begin; u < walk.total && ok; u += u_step, ++count) {
+            const bool more = u + u_step < walk.total;
+            const int a = (int)(count & 1u);
+            if (count >= 2) ok = mbar_wait(accum_empty(a), ((count >> 1) - 1) & 1, p.status, ST_MMA_TIMEOUT);
+            tc_fence_after();
+            for (int kt = 0; kt < KT && ok; ++kt, ++it) {
+                const int s = it % STAGES;
+                const uint32_t st = ring + s * C::STAGE_BYTES, set = (it & 1u) * (C::SF_STEPS * 8);
+                if (!copied) {
+                    ok = mbar_wait(full_bar(s), (it / STAGES) & 1, p.status, ST_MMA_TIMEOUT);
+                    tc_fence_after();
+                    if (ok) copy_scales(it);
+                }
+                copied = false;
+                if (!ok) break;
+                if ((kt + 1 < KT || more) && mbar_test_wait(full_bar((it + 1) % STAGES), ((it + 1) / STAGES) & 1)) {
+                    tc_fence_after();
+                    copy_scales(it + 1);
+                    copied = true;
+                }
+                const uint64_t w_desc = smem_desc(st, 16, 1024, LAYOUT_SW128), x_desc = smem_desc(st + W_BYTES, 16, 1024, LAYOUT_SW128);
+                const uint32_t d = tmem + a * ACC_STRIDE, sfw = tmem + SFW_COL + set, sfx = tmem + SFX_COL + set;
+                if (elect_one()) {
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k) {
+                        const uint32_t acc = (kt > 0 || k > 0) ? 1u : 0u;
+                        if constexpr (MXF4) {
+                            const uint32_t id = (k & 1u) * 2u;
+                            mma_mxf4(d, w_desc + 2 * k, x_desc + 2 * k, idesc | (id << 29) | (id << 4), sfw + 8 * (k >> 1), sfx + 8 * (k >> 1), acc);
+                        } else {
+                            mma_mxf8f6f4(d, w_desc + 2 * k, x_desc + 2 * k, idesc | (k << 29) | (k << 4), sfw, sfx, acc);
+                        }
+                    }
+                    mma_commit(empty_bar(s));
+                }
+                __syncwarp();
+            }
+            if (elect_one()) mma_commit(accum_full(a));
+            __syncwarp();
+        }
+        if (!ok) {
+            // unwinding after a wait that ran out: the MMAs already issued must finish before tensor memory is freed
+            if (elect_one()) mma_commit(drain_bar);
+            __syncwarp();
+            mbar_wait(drain_bar, 0, nullptr, 0);
+        }
+    } else if (warp >= QUANT_WARP) {
+        // ---------------- rows: a warp takes every eighth stage, 16 lanes a row, two rows at a time ----------------
+        constexpr int E = MXF4 ? 16 : 8, WORDS = E * (int)sizeof(T) / 4;                 // elements and words per lane and row
+        constexpr int BATCH = 32 / WORDS;                                                // row pairs whose loads are issued together (32 registers)
+        constexpr int PAIRS = ROWS / 2;
+        using KIn = typename std::conditional<DT == MXQ_F32, KF32, typename std::conditional<DT == MXQ_BF16, KBF16, KF16>::type>::type;
+        const int kl = (lane & 15) * E;                                                  // this lane's first element of a step
+        int u = u_begin, kt = warp - QUANT_WARP;
+        uint32_t it = kt;
+        bool fresh = true, ok = true;
+        Unit t{};
+        int from[PAIRS];                                                                 // rows of x, -1: zeros
+        while (ok) {
+            while (kt >= KT && u < walk.total) { kt -= KT; u += u_step; fresh = true; }
+            if (u >= walk.total) break;
+            if (fresh) {
+                fresh = false;
+                t = walk.at(u, FEATURES);
+#pragma unroll
+                for (int i = 0; i < PAIRS; ++i) {
+                    const int r = 2 * i + (lane >> 4);
+                    from[i] = -1;
+                    if (r < t.rows) {
+                        int64_t row = t.row + r;
+                        if (src.row_index != nullptr)
+                            row = src.index64 ? reinterpret_cast<const long long*>(src.row_index)[row] : (int64_t)reinterpret_cast<const int*>(src.row_index)[row];
+                        if (row >= 0 && row < src.rows_in) from[i] = (int)row;
+                    }
+                }
+            }
+            const int s = it % STAGES, k = (k_begin + kt) * C::K_STEP + kl;
+            uint8_t* st = ring_ptr + s * C::STAGE_BYTES;
+            bool first_batch = true;
+#pragma unroll
+            for (int i0 = 0; i0 < PAIRS; i0 += BATCH) {
+                if (2 * i0 >= t.rows) break;
+                uint32_t w[BATCH][WORDS];
+#pragma unroll
+                for (int i = 0; i < BATCH; ++i)
+#pragma unroll
+                    for (int j = 0; j < WORDS; j += 4) {
+                        uint4 q = make_uint4(0u, 0u, 0u, 0u);
+                        if (from[i0 + i] >= 0 && k < p.K)
+                            q = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(src.x) + (int64_t)from[i0 + i] * p.K + k) + j / 4);
+                        w[i][j] = q.x; w[i][j + 1] = q.y; w[i][j + 2] = q.z; w[i][j + 3] = q.w;
+                    }
+                if (first_batch) {
+                    first_batch = false;
+                    if (it >= STAGES) ok = mbar_wait(empty_bar(s), ((it / STAGES) & 1) ^ 1, p.status, ST_PRODUCER_TIMEOUT);
+                    if (!ok) break;
+                }
+#pragma unroll
+                for (int i = 0; i < BATCH; ++i) {
+                    if (2 * (i0 + i) >= t.rows) break;                                   // uniform: neither row of the pair exists
+                    uint32_t b[E], codes[2];
+#pragma unroll
+                    for (int j = 0; j < E; ++j) {
+                        if constexpr (KIn::size == 4) b[j] = w[i][j];
+                        else b[j] = KIn::to_bits(j & 1 ? w[i][j >> 1] >> 16 : w[i][j >> 1] & 0xFFFFu);
+                    }
+                    const uint32_t sbyte = quantise_part<F, OUT, E>(b, codes);
+                    const int r = 2 * (i0 + i) + (lane >> 4);
+                    if (r < t.rows) {
+                        // 8 of the row's 128 bytes: 16-byte unit j lies at j ^ (r % 8)
+                        const uint32_t j = (lane & 15) >> 1;
+                        *reinterpret_cast<uint2*>(st + W_BYTES + r * 128 + ((j ^ (r & 7)) << 4) + (lane & 1) * 8) = make_uint2(codes[0], codes[1]);
+                        if (lane % (32 / E) == 0) {
+                            // scale of row r and block b at r * 16 + b; blocks behind K are 2^0 (their codes are zero)
+                            const int blk = kl / 32;
+                            st[W_BYTES + X_BYTES + (blk >> 2) * 1024 + 512 + r * 16 + (blk & 3)] = (uint8_t)(k < p.K ? sbyte : 127u);
+                        }
+                    }
+                }
+            }
+            if (!ok) break;
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full_bar(s));
+            it += QUANT_WARPS;
+            kt += QUANT_WARPS;
+        }
+    } else if (warp >= EPI_WARP) {
+        // ---------------- epilogue: 32 features of 16 rows per warp ----------------
+        const int q = warp - EPI_WARP;
+        const int er = lane >> 3, ef = q * 32 + (lane & 7) * 4;
+        float* slot = slots + q * 512;
+        T* out = reinterpret_cast<T*>(p.out);
+        const T* extra = reinterpret_cast<const T*>(p.extra);
+        const int owner = q / quads;                                                     // the CTA of the cluster that finishes these features
+        bool ok = true;
+        uint32_t count = 0;
+        for (int u = u_begin; u < walk.total && ok; u += u_step, ++count) {
+            const Unit t = walk.at(u, FEATURES);
+            const int a = (int)(count & 1u), f = t.f0 + ef;
+            Four<T> e[4];
+            float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (owner == rank) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = i * 4 + er;
+                    if (p.extra_mode != X_NONE && r < t.rows) load_four(extra + (size_t)(t.row + r) * p.N + f, p.N - f, p.vector, e[i]);
+                }
+                if (p.bias != nullptr) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) if (f + i < p.N) bias[i] = widen(reinterpret_cast<const T*>(p.bias)[(size_t)t.g * p.N + f + i]);
+                }
+            }
+            ok = mbar_wait(accum_full(a), (count >> 1) & 1, p.status, ST_EPILOGUE_TIMEOUT);
+            tc_fence_after();
+            if (!ok) break;
+            uint32_t v[32];
+            tmem_ld_32x32b_x16(tmem + ((uint32_t)(q * 32) << 16) + a * ACC_STRIDE, v);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(accum_empty(a));
+            if (split > 1) {
+                // a cluster works on one unit: parts are received once.  Part of CTA c for this quadrant: slot c, own one left out
+                float* mine = exchange + (q % quads) * 512;
+                if (owner != rank) {
+                    const int place = rank < owner ? rank : rank - 1;
+                    const uint32_t to = map_to_rank(smem_u32(mine + place * quads * 512 + lane), (uint32_t)owner);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to + j * 128), "r"(v[j]) : "memory");
+                    asm volatile("fence.acq_rel.cluster;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0)
+                        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(map_to_rank(parts_bar, (uint32_t)owner)) : "memory");
+                    continue;
+                }
+                ok = mbar_wait_cluster(parts_bar, 0, p.status, ST_EPILOGUE_TIMEOUT);
+                if (!ok) break;
+                float sum[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) sum[j] = 0.0f;
+                for (int c = 0; c < split; ++c) {                                        // in the order of the CTAs
+                    const float* part = mine + (c < rank ? c : c - 1) * quads * 512;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) sum[j] += c == rank ? __uint_as_float(v[j]) : part[j * 32 + lane];
+                }
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(sum[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) slot[j * 32 + lane] = __uint_as_float(v[j]);
+            __syncwarp();
+            T* at = out + (size_t)(t.row + er) * p.N + f;
+            const int rows = (t.rows - er + 3) >> 2, left = p.N - f;
+            finish_any(p.act, slot, lane, bias, e, p.extra_mode, at, p.N, rows, left, p.vector);
+            __syncwarp();
+        }
+        if (p.zero_rest) zero_rows_outside(out, first[0], first[p.rows.groups], p.rows.rows, p.N, threadIdx.x - EPI_WARP * 32, 128);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+    }
+    if (split > 1) cluster_barrier();                                // no CTA leaves while another may still write to it
+}
+
+template <int DT, class F, int OUT>
+static int launch(const Params& p, const Source& src, const uint8_t* w_codes, int split, cudaStream_t st) {
+    using C = Cfg<OUT == 5>;
+    static bool attr_done[MAX_DEVICES] = {false};
+    cudaError_t e = raise_smem_limit(decode_kernel<DT, F, OUT>, C::SMEM_BYTES, attr_done);
+    if (e != cudaSuccess) { set_last_cuda_error(e); return MXQ_ELAUNCH; }
+    CUtensorMap mw;
+    if (!make_map(&mw, w_codes, (int64_t)p.rows.groups * p.N, p.K, FEATURES, OUT == 5)) return MXQ_ELAUNCH;
+    const int64_t units = most_units(p.rows, p.N, FEATURES);
+    cudaLaunchConfig_t cfg = {};
+    // a cluster works on one unit; without clusters the CTAs stay and walk over theirs
+    cfg.gridDim = dim3((unsigned)(split > 1 ? units * split : units < sm_count() ? units : sm_count()));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = C::SMEM_BYTES;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)split;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = split > 1 ? 2 : 1;
+    e = cudaLaunchKernelEx(&cfg, decode_kernel<DT, F, OUT>, mw, p, src, split);
+    if (e != cudaSuccess) { set_last_cuda_error(e); return MXQ_ELAUNCH; }
+    return check_launch();
+}
+
+}  // namespace decode
+
+int decode_rows() { return decode::ROWS; }
+
+int launch_decode(const Params& p, int dt, const void* x, const void* row_index, int index64, int64_t rows_in, int eb, int fb, bool nibbles,
+                  const uint8_t* w_codes, cudaStream_t st) {
+    // CTAs that share a unit: as many as the SMs hold, the steps of K allow, and 4 at most (a lane quadrant each)
+    const int64_t units = most_units(p.rows, p.N, decode::FEATURES);
+    const int steps = (p.K + (nibbles ? 255 : 127)) / (nibbles ? 256 : 128);
+    int split = 1;
+    while (split < 4 && units * split * 2 <= sm_count() && steps >= split * 2 * 4) split *= 2;
+    const decode::Source src{x, row_index, index64, rows_in};
+    int rc = MXQ_ESIZE;
+    with_row_format(eb, fb, nibbles, [&](auto fmt, auto out) {
+        using F = decltype(fmt);
+        constexpr int OUT = decltype(out)::value;
+        if (dt == MXQ_F32) rc = decode::launch<MXQ_F32, F, OUT>(p, src, w_codes, split, st);
+        else if (dt == MXQ_BF16) rc = decode::launch<MXQ_BF16, F, OUT>(p, src, w_codes, split, st);
+        else rc = decode::launch<MXQ_F16, F, OUT>(p, src, w_codes, split, st);
+    });
+    return rc;
+}
+
+}  // namespace grouped
+}  // namespace mxq

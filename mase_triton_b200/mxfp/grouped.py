@@ -30,6 +30,9 @@ class PackedExperts:
     N: int
     K: int
 
+    def __post_init__(self):
+        self.device_index, self.codes_ptr, self.sf_ptr = self.codes.get_device(), self.codes.data_ptr(), self.sf.data_ptr()
+
 
 def check_formats(x_meta: MXFPMeta | None, w_meta: MXFPMeta | None, K: int) -> None:
     if not (supported(x_meta) and supported(w_meta)):
@@ -116,7 +119,7 @@ def grouped_linear(x: Tensor, x_meta: MXFPMeta, w: PackedExperts, offsets: Tenso
         raise ValueError(f"input of shape {tuple(x.shape)}: expected [tokens, {K}]")
     if not supported(x_meta) or (w.hw_format == 5 and not is_e2m1(x_meta)):
         raise ValueError(f"the weight was packed for another activation format than {x_meta}")
-    if w.codes.get_device() != dev:
+    if w.device_index != dev:
         raise ValueError(f"the weight is on {w.codes.device}, the input on {x.device}")
     x = x.contiguous()
     tokens = rows = x.shape[0]
@@ -148,7 +151,7 @@ def grouped_linear(x: Tensor, x_meta: MXFPMeta, w: PackedExperts, offsets: Tenso
     zero_rest = 0
     if out is None:
         zero_rest = int(offsets is not None)
-        out = torch.empty((rows, N), dtype=dtype, device=x.device)
+        out = x.new_empty(rows, N)
     else:
         if out.dtype != dtype or out.shape != (rows, N) or out.get_device() != dev:
             raise _operand_error(out, "out", (rows, N), x)
@@ -160,12 +163,13 @@ def grouped_linear(x: Tensor, x_meta: MXFPMeta, w: PackedExperts, offsets: Tenso
         return out
     status = status_address(dev)
     L = _lib.load()
-    nbytes = L.mxq_mx_grouped_scratch_bytes(tokens, rows, K, groups)
+    x_ptr, round_id = x.data_ptr(), _lib.ROUND_ID[x_meta.round_mode]
+    nbytes = L.mxq_mx_grouped_scratch_bytes(x_ptr, round_id, tokens, rows, K, groups)
     # of this call alone: two captured graphs, or two streams, never share it
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-    args = (x.data_ptr(), dtype_id, tokens, rows, K, x_meta.element_exp_bits, x_meta.element_frac_bits, _lib.ROUND_ID[x_meta.round_mode], index_ptr, index64,
-            w.codes.data_ptr(), w.sf.data_ptr(), w.hw_format, groups, N, offsets_ptr, offsets64, out.data_ptr(), bias_ptr, act, extra_ptr, extra_mode, zero_rest,
-            scratch.data_ptr(), nbytes, status, torch.cuda.current_stream(dev).cuda_stream)
+    scratch = None if nbytes == 0 else torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    args = (x_ptr, dtype_id, tokens, rows, K, x_meta.element_exp_bits, x_meta.element_frac_bits, round_id, index_ptr, index64, w.codes_ptr, w.sf_ptr, w.hw_format,
+            groups, N, offsets_ptr, offsets64, out.data_ptr(), bias_ptr, act, extra_ptr, extra_mode, zero_rest,
+            None if scratch is None else scratch.data_ptr(), nbytes, status, _lib.raw_stream(dev))
     if torch.cuda.current_device() == dev:
         rc = L.mxq_mx_grouped_linear(*args)
     else:

@@ -136,11 +136,14 @@ class MXFPLinearPTQ(PTQLinearBase):
 
         return import_packed(record, device, backend)
 
-    @torch.no_grad()
     def forward(self, input: Tensor, activation: str | None = None, multiplier: Tensor | None = None, residual: Tensor | None = None) -> Tensor:
         """``act(linear(input)) * multiplier`` or ``act(linear(input)) + residual``; see ``mxfp_linear``."""
         if activation is not None or multiplier is not None or residual is not None:
             return self._forward_with_epilogue(input, activation, multiplier, residual)
+        return self._forward(input)
+
+    @torch.no_grad()
+    def _forward(self, input: Tensor) -> Tensor:
         if (self.backend == "fused" and "Xq" in self.layer_type and "Wq" in self.layer_type
                 and MXFP_F.linear.block_scaled_ok(input, self.x_mxfp_meta, self.w_tensor_meta)):
             # both operands stay quantised: the module's own tensor-core form of the weight, no per-call packing.
@@ -160,6 +163,10 @@ class MXFPLinearPTQ(PTQLinearBase):
             if self._row_weight is None:
                 MXFP_F.linear.require_epilogue(self.x_mxfp_meta, self.w_tensor_meta, parse_layer_type(self.layer_type))
             return MXFP_F.linear.linear_with_epilogue(input, self.x_mxfp_meta, self.row_weight(), self.bias, activation, multiplier, residual)
+        return self._separate_with_epilogue(input, activation, multiplier, residual)
+
+    @torch.no_grad()
+    def _separate_with_epilogue(self, input: Tensor, activation: str | None, multiplier: Tensor | None, residual: Tensor | None) -> Tensor:
         return MXFP_F.mxfp_linear(
             x=input, x_meta=self.x_mxfp_meta,
             w=self.weight, w_scales=self.w_scales, w_elements=self.w_elements, w_tensor_meta=self.w_tensor_meta,
@@ -278,7 +285,6 @@ class MXFPGroupedLinearPTQ(PTQLinearBase):
                                                       self.w_tensor_meta.meta, self.x_mxfp_meta))
         return self._row_weight[2]
 
-    @torch.no_grad()
     def forward(self, input: Tensor, offsets: Tensor, activation: str | None = None, multiplier: Tensor | None = None,
                 residual: Tensor | None = None, row_index: Tensor | None = None, out: Tensor | None = None) -> Tensor:
         """``mxfp_grouped_linear`` with this layer's weights."""

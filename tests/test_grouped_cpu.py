@@ -150,10 +150,12 @@ def test_c_entry_refuses_before_it_launches():
                 offsets64=0, out=p, bias=None, act=0, extra=None, mode=0, zero=0, scratch=p, nbytes=1 << 16, status=None, stream=None)
     assert L.mxq_mx_grouped_linear(*(good | dict(rows=0, rows_in=0)).values()) == 0
     for bad in (dict(K=48), dict(K=0), dict(N=0), dict(groups=0), dict(groups=2), dict(rows=3), dict(rows=-1), dict(x_dtype=3), dict(act=5), dict(act=-1), dict(mode=3),
-                dict(mode=1), dict(x=None), dict(w_codes=None), dict(w_sf=p + 8), dict(out=None), dict(scratch=None), dict(scratch=p + 16), dict(fmt=3), dict(fmt=5),
+                dict(mode=1), dict(x=None), dict(w_codes=None), dict(w_sf=p + 8), dict(out=None), dict(scratch=None, rm=1), dict(scratch=p + 16), dict(fmt=3), dict(fmt=5),
                 dict(eb=3, fb=3)):
         assert L.mxq_mx_grouped_linear(*(good | bad).values()) == -1, bad
-    for bad in (dict(groups=L.mxq_mx_max_groups() + 1, offsets=p), dict(nbytes=64), dict(rows=1 << 31, rows_in=1 << 31)):
+    for bad in (dict(groups=L.mxq_mx_max_groups() + 1, offsets=p), dict(nbytes=64, rm=1), dict(rows=1 << 31, rows_in=1 << 31)):
         assert L.mxq_mx_grouped_linear(*(good | bad).values()) == -3, bad
-    assert L.mxq_mx_grouped_scratch_bytes(2, 2, 48, 1) == -1 and L.mxq_mx_grouped_scratch_bytes(2, 2, 64, 1) > 0
+    assert L.mxq_mx_grouped_scratch_bytes(p, 0, 2, 2, 48, 1) == -1 and L.mxq_mx_grouped_scratch_bytes(p, 0, 2, 2, 64, 1) == 0
+    assert L.mxq_mx_grouped_scratch_bytes(p + 2, 0, 2, 2, 64, 1) > 0 and L.mxq_mx_grouped_scratch_bytes(p, 1, 2, 2, 64, 1) > 0
+    assert L.mxq_mx_grouped_scratch_bytes(p, 0, 500, 500, 64, 1) > 0
     assert SimpleNamespace(**good).K == 64
