@@ -416,13 +416,14 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restri
         src = index64 ? reinterpret_cast<const long long*>(row_index)[row] : (int64_t)reinterpret_cast<const int*>(row_index)[row];
     const bool there = src >= 0 && src < rows_in;                            // a row index outside x gives a row of zeros
     const char* from = reinterpret_cast<const char*>(x) + src * K * KIn::size;
+    const uint32_t fill = there ? one_bits<KIn>() : 0u;                       // lanes behind K do not hold up the others' short form
     uint32_t raw[QUANT_ACCESSES][BYTES / 4];
 #pragma unroll
     for (int a = 0; a < QUANT_ACCESSES; ++a) {
         const int k = first + a * (int)blockDim.x * 8;
 #pragma unroll
         for (int i = 0; i < BYTES / 16; ++i) {
-            const uint4 v = there && k < K ? __ldg(reinterpret_cast<const uint4*>(from + (int64_t)k * KIn::size) + i) : make_uint4(0, 0, 0, 0);
+            const uint4 v = there && k < K ? __ldg(reinterpret_cast<const uint4*>(from + (int64_t)k * KIn::size) + i) : make_uint4(fill, fill, fill, fill);
             raw[a][4 * i] = v.x; raw[a][4 * i + 1] = v.y; raw[a][4 * i + 2] = v.z; raw[a][4 * i + 3] = v.w;
         }
     }
@@ -431,13 +432,8 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restri
 #pragma unroll
     for (int a = 0; a < QUANT_ACCESSES; ++a) {
         const int k = first + a * (int)blockDim.x * 8;
-        uint32_t b[8], o[OUT == 5 ? 1 : 2];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if constexpr (KIn::size == 4) b[i] = raw[a][i];
-            else b[i] = KIn::to_bits(i & 1 ? raw[a][i >> 1] >> 16 : raw[a][i >> 1] & 0xFFFFu);
-        }
-        const uint32_t sbyte = quantise_part<F, OUT, 8>(b, o);
+        uint32_t o[OUT == 5 ? 1 : 2];
+        const uint32_t sbyte = quantise_part<KIn, F, OUT, 8>(raw[a], o);
         if (k < K) {
             if constexpr (OUT == 5) *reinterpret_cast<uint32_t*>(o_.codes + ((int64_t)row * K + k) / 2) = o[0];
             else *reinterpret_cast<uint2*>(o_.codes + (int64_t)row * K + k) = make_uint2(o[0], o[1]);

@@ -1,7 +1,7 @@
 // Pieces shared by the kernels of the grouped products (mxq_grouped.cu, mxq_grouped_decode.cu): the group table and the walk over
 // the units of work, the epilogue's arithmetic, launches that may overlap the kernel before them.
 #pragma once
-#include "mxq_device.cuh"
+#include "mxq_quant.cuh"
 #include "mxq_tc.cuh"
 
 namespace mxq {
@@ -115,53 +115,124 @@ __device__ __forceinline__ void zero_rows_outside(T* out, int begin, int end, in
         narrow(0.0f, out[i < before ? i : i - before + (int64_t)end * N]);
 }
 
-// E elements of a 32-element block per lane (fp32 bits; the 32 / E lanes of the block are neighbours) -> the tensor cores' codes, and
-// the block's scale byte as the result.  The lanes agree on the block's maximum by shuffles; every lane derives the scale,
-// quantises (the dequantised quotient in fp32, as the fused quantise-dequantise kernel forms it) and converts, which is exact.  A block
-// with a value that the hardware's format lacks becomes (scale + 1, elements / 2).  All lanes of the warp take part.
-// OUT: 0 = E4M3 bytes, 1 = E5M2 bytes, 5 = E2M1 nibbles.
-template <class F, int OUT, int E>
-__device__ __forceinline__ uint32_t quantise_part(const uint32_t (&b)[E], uint32_t (&codes)[OUT == 5 ? E / 8 : E / 4]) {
-    const F f{};
-    uint32_t amax = 0;
-#pragma unroll
-    for (int i = 0; i < E; ++i) amax = max(amax, b[i] & 0x7FFFFFFFu);
-#pragma unroll
-    for (int o = 1; o < 32 / E; o <<= 1) amax = max(amax, __shfl_xor_sync(~0u, amax, o));
-    const uint32_t header = block_header(amax, f);                       // 2^-se, the scale byte, and whether the block holds Inf / NaN
-    uint32_t sbyte = (header >> 8) & 0xFFu;
-    const float inv = __uint_as_float(header & 0x7F800000u);
-    const bool special = header & 1u;
-    float v[E];
-    bool bad = false;
-    constexpr float hw_max = OUT == 0 ? 448.0f : OUT == 1 ? 57344.0f : 6.0f;
-    constexpr float fmt_max = F{}.eb() == 4 ? 480.0f : F{}.eb() == 5 ? 114688.0f : 0.0f;     // the formats whose largest value the hardware lacks
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-        const uint32_t qb = mx_quotient_bits(b[i], inv);
-        const uint32_t y = special ? 0u : qdq_mag_bits(qb, f);
-        if constexpr (fmt_max > hw_max) bad |= __uint_as_float(y) > hw_max;
-        v[i] = __uint_as_float(y | (qb & 0x80000000u));
+// 1.0 (two of them for the 16-bit types) as a word
+template <class KIn> __device__ __forceinline__ constexpr uint32_t one_bits() {
+    return KIn::size == 4 ? 0x3F800000u : std::is_same<KIn, KBF16>::value ? 0x3F803F80u : 0x3C003C00u;
+}
+
+// Codes of a narrower element format, one per byte, as the E4M3 bytes of the same values (exact).
+template <class F> __device__ __forceinline__ uint32_t widen_codes4(uint32_t w) {
+    if constexpr (F{}.eb() == 2 && F{}.fb() == 1) {
+        // the magnitudes 0, 0.5, 1, 1.5, 2, 3, 4, 6 looked up by the three low bits
+        const uint32_t pick = (w & 0x7u) | ((w >> 4) & 0x70u) | ((w >> 8) & 0x700u) | ((w >> 12) & 0x7000u);
+        return __byte_perm(0x3C383000u, 0x4C484440u, pick) | ((w & 0x08080808u) << 4);
+    } else {
+        uint32_t lo, hi;
+        if constexpr (F{}.eb() == 2) {
+            asm("cvt.rn.f16x2.e2m3x2 %0, %1;" : "=r"(lo) : "h"((uint16_t)w));
+            asm("cvt.rn.f16x2.e2m3x2 %0, %1;" : "=r"(hi) : "h"((uint16_t)(w >> 16)));
+        } else {
+            asm("cvt.rn.f16x2.e3m2x2 %0, %1;" : "=r"(lo) : "h"((uint16_t)w));
+            asm("cvt.rn.f16x2.e3m2x2 %0, %1;" : "=r"(hi) : "h"((uint16_t)(w >> 16)));
+        }
+        uint16_t a, b;
+        asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(a) : "r"(lo));
+        asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(b) : "r"(hi));
+        return (uint32_t)a | ((uint32_t)b << 16);
     }
-    if constexpr (fmt_max > hw_max) {
-        uint32_t any = bad ? 1u : 0u;
+}
+
+// E (8 or 16) elements of a 32-element block per lane, as they lie in memory (the 32 / E lanes of the block are neighbours) -> the
+// tensor cores' codes, and the block's scale byte as the result.  The lanes agree on the block's maximum by shuffles and every lane
+// derives the scale; bf16 inputs take the packed quantisers, the 8-bit element formats their short form where no element of the warp lies
+// below its block's normal range (so lanes without a row should hold ones, not zeros).  A block with a code that the hardware reads
+// as Inf / NaN becomes (scale + 1, elements / 2).  All lanes of the warp take part.
+// OUT: 0 = E4M3 bytes, 1 = E5M2 bytes, 5 = E2M1 nibbles.
+template <class KIn, class F, int OUT, int E>
+__device__ __forceinline__ uint32_t quantise_part(const uint32_t (&raw)[E * KIn::size / 4], uint32_t (&codes)[OUT == 5 ? E / 8 : E / 4]) {
+    const F f{};
+    constexpr int LANES = 32 / E;
+    uint32_t o[E / 4], sbyte;
+    bool special;
+    if constexpr (std::is_same<KIn, KBF16>::value) {
+        uint32_t mx2, mn2;
+        Pack<16> p[E / 8];
 #pragma unroll
-        for (int o = 1; o < 32 / E; o <<= 1) any |= __shfl_xor_sync(~0u, any, o);
-        if (any) {
+        for (int i = 0; i < E / 8; ++i) {
+            uint32_t hi, lo;
 #pragma unroll
-            for (int i = 0; i < E; ++i) v[i] *= 0.5f;
+            for (int j = 0; j < 4; ++j) p[i].w[j] = raw[4 * i + j];
+            bf16_abs_range(p[i], hi, lo);
+            mx2 = i == 0 ? hi : bf2_bits(__hmax2_nan(bf2(mx2), bf2(hi)));
+            mn2 = i == 0 ? lo : bf2_bits(__hmin2(bf2(mn2), bf2(lo)));
+        }
+#pragma unroll
+        for (int d = 1; d < LANES; d <<= 1) mx2 = bf2_bits(__hmax2_nan(bf2(mx2), bf2(__shfl_xor_sync(~0u, mx2, d))));
+        const uint32_t header = block_header_bf16(bf16x2_max_bits(mx2), f), word = bf16_block_word<F>(header);
+#pragma unroll
+        for (int i = 0; i < E / 8; ++i) bf16_quantise_access<F, false>(p[i], word, mn2, header, 0u, o + 2 * i);
+        sbyte = (header >> 8) & 0xFFu;
+        special = header & 1u;
+    } else {
+        uint32_t b[E], amax = 0, amin = ~0u;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            if constexpr (KIn::size == 4) b[i] = raw[i];
+            else b[i] = KIn::to_bits(i & 1 ? raw[i >> 1] >> 16 : raw[i >> 1] & 0xFFFFu);
+            amax = max(amax, b[i] & 0x7FFFFFFFu);
+            amin = min(amin, b[i] & 0x7FFFFFFFu);
+        }
+#pragma unroll
+        for (int d = 1; d < LANES; d <<= 1) amax = max(amax, __shfl_xor_sync(~0u, amax, d));
+        const uint32_t header = block_header(amax, f);
+        const float inv = __uint_as_float(header & 0x7F800000u);
+        bool short_form = false;
+        if constexpr (PkFmt<F>::RARE_SUBRANGE) short_form = !__any_sync(~0u, amin < short_form_limit_bits<F>(header));
+        if (short_form) {
+            if constexpr (PkFmt<F>::RARE_SUBRANGE) {
+#pragma unroll
+                for (int i = 0; i < E / 4; ++i) o[i] = f32_codes4_normal(b + 4 * i, inv, f);
+            }
+        } else {
+            uint32_t qb[E], mag[E];
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                qb[i] = mx_quotient_bits(b[i], inv);
+                mag[i] = (uint32_t)encode_mag_fp(qb[i], f);
+            }
+#pragma unroll
+            for (int i = 0; i < E / 4; ++i) o[i] = pack4_codes(mag + 4 * i, qb + 4 * i, f);
+        }
+        sbyte = (header >> 8) & 0xFFu;
+        special = header & 1u;
+    }
+    if constexpr (F{}.eb() >= 4) {
+        // carry out of the magnitude byte: a code the hardware reads as Inf / NaN
+        constexpr uint32_t probe = F{}.eb() == 4 ? 0x01010101u : 0x04040404u;
+        uint32_t bad = 0;
+#pragma unroll
+        for (int i = 0; i < E / 4; ++i) bad |= ((o[i] & 0x7F7F7F7Fu) + probe) & 0x80808080u;
+#pragma unroll
+        for (int d = 1; d < LANES; d <<= 1) bad |= __shfl_xor_sync(~0u, bad, d);
+        if (bad != 0u) {
+#pragma unroll
+            for (int i = 0; i < E / 4; ++i) o[i] = halve_codes4<F{}.fb()>(o[i]);
             sbyte += sbyte < 255u ? 1u : 0u;
         }
     }
 #pragma unroll
-    for (int i = 0; i < E; i += 2) {
-        uint16_t two;
-        if constexpr (OUT == 0) asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(v[i + 1]), "f"(v[i]));
-        else if constexpr (OUT == 1) asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(two) : "f"(v[i + 1]), "f"(v[i]));
-        else asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %1, %2;\n\tcvt.u16.u8 %0, t;\n\t}" : "=h"(two) : "f"(v[i + 1]), "f"(v[i]));
-        constexpr int PER = OUT == 5 ? 8 : 4, BITS = 32 / PER;
-        if (i % PER == 0) codes[i / PER] = two;
-        else codes[i / PER] |= (uint32_t)two << (BITS * (i % PER));
+    for (int i = 0; i < E / 4; ++i) {
+        if (special) o[i] = 0u;
+        if constexpr (OUT == 5) {
+            uint32_t t = o[i] & 0x0F0F0F0Fu;                              // element 2i in the low nibble of byte i
+            t |= t >> 4;
+            t = (t & 0xFFu) | ((t >> 8) & 0xFF00u);
+            if (i % 2 == 0) codes[i / 2] = t; else codes[i / 2] |= t << 16;
+        } else if constexpr (F{}.eb() >= 4) {
+            codes[i] = o[i];
+        } else {
+            codes[i] = widen_codes4<F>(o[i]);
+        }
     }
     return special ? 255u : sbyte;                                       // 255 is NaN to the tensor cores, whatever the codes
 }

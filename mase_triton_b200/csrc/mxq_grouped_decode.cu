@@ -220,7 +220,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         uint32_t it = kt;
         bool fresh = true, ok = true;
         Unit t{};
-        int from[PAIRS];                                                                 // rows of x, -1: zeros
+        int from[PAIRS];                                                                 // rows of x; -1: a row of zeros, -2: none
         while (ok) {
             while (kt >= KT && u < walk.total) { kt -= KT; u += u_step; fresh = true; }
             if (u >= walk.total) break;
@@ -230,7 +230,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
 #pragma unroll
                 for (int i = 0; i < PAIRS; ++i) {
                     const int r = 2 * i + (lane >> 4);
-                    from[i] = -1;
+                    from[i] = r < t.rows ? -1 : -2;
                     if (r < t.rows) {
                         int64_t row = t.row + r;
                         if (src.row_index != nullptr)
@@ -250,7 +250,9 @@ decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
                 for (int i = 0; i < BATCH; ++i)
 #pragma unroll
                     for (int j = 0; j < WORDS; j += 4) {
-                        uint4 q = make_uint4(0u, 0u, 0u, 0u);
+                        // a row that does not exist reads as ones (it does not hold up the short form), one outside x as zeros
+                        const uint32_t fill = from[i0 + i] == -2 ? one_bits<KIn>() : 0u;
+                        uint4 q = make_uint4(fill, fill, fill, fill);
                         if (from[i0 + i] >= 0 && k < p.K)
                             q = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(src.x) + (int64_t)from[i0 + i] * p.K + k) + j / 4);
                         w[i][j] = q.x; w[i][j + 1] = q.y; w[i][j + 2] = q.z; w[i][j + 3] = q.w;
@@ -263,13 +265,8 @@ decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
 #pragma unroll
                 for (int i = 0; i < BATCH; ++i) {
                     if (2 * (i0 + i) >= t.rows) break;                                   // uniform: neither row of the pair exists
-                    uint32_t b[E], codes[2];
-#pragma unroll
-                    for (int j = 0; j < E; ++j) {
-                        if constexpr (KIn::size == 4) b[j] = w[i][j];
-                        else b[j] = KIn::to_bits(j & 1 ? w[i][j >> 1] >> 16 : w[i][j >> 1] & 0xFFFFu);
-                    }
-                    const uint32_t sbyte = quantise_part<F, OUT, E>(b, codes);
+                    uint32_t codes[2];
+                    const uint32_t sbyte = quantise_part<KIn, F, OUT, E>(w[i], codes);
                     const int r = 2 * (i0 + i) + (lane >> 4);
                     if (r < t.rows) {
                         // 8 of the row's 128 bytes: 16-byte unit j lies at j ^ (r % 8)
