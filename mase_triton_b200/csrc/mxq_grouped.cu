@@ -85,19 +85,19 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
+    if (warp == 0 && elect_one()) { prefetch_map(map_w); prefetch_map(map_x16); prefetch_map(map_x64); }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    if (warp == 3) build_table(p.rows, tiles, first, lane);
     tc_fence_before();
-    __syncthreads();
+    build_table(p.rows, tiles, first);
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(~0u, *tmem_slot, 0);
 
     const int KT = (p.K + C::K_STEP - 1) / C::K_STEP, KT128 = (p.K + 127) / 128;
     const int ftiles = (p.N + C::FEATURES - 1) / C::FEATURES;
-    Walk walk(tiles, first, p.rows.groups, ftiles, p.rows.width);
+    Walk walk(tiles, first, p.rows.groups, ftiles);
     auto halves_of = [&](const Unit& t) { return MH == 2 && p.N - t.f0 > 128 ? 2 : 1; };
 
     // The kernel before this one quantises the rows.  It lets this one start when everything before it has completed, so that
@@ -109,44 +109,44 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     if (warp == 0 || warp == 3) {
         // ---------------- copies: weights and their scales (warp 0), rows (warp 3) ----------------
         bool ok = true;
-        uint32_t it = 0;
+        RingAt<STAGES> at;
+        uint32_t issued = 0;
         for (int u = blockIdx.x; u < walk.total && ok; u += gridDim.x) {
             const Unit t = walk.at(u, C::FEATURES);
-            const int halves = halves_of(t);
-            const uint32_t n = t.padded();
-            const uint8_t* sf = p.w_sf + (size_t)t.g * p.w_sf_group +
-                                (MH == 2 ? (size_t)t.ftile * KT128 * 1024 : (size_t)(t.ftile >> 1) * KT128 * 1024 + (t.ftile & 1) * 512);
-            const int w_row = t.g * p.N + t.f0;
-            const uint8_t* x_sf = p.x_sf + (size_t)t.slot * KT128 * (C::X_CHUNKS * 512);
+            const int halves = uniform(halves_of(t)), row = uniform(t.row), w_row = uniform(t.g * p.N + t.f0);
+            const uint32_t n = uniform(t.padded());
+            const uint8_t* w_sf = p.w_sf + (size_t)uniform(t.g) * p.w_sf_group +
+                                  (MH == 2 ? (size_t)uniform(t.ftile) * KT128 * 1024 : (size_t)uniform(t.ftile >> 1) * KT128 * 1024 + uniform(t.ftile & 1) * 512);
+            const uint8_t* x_sf = p.x_sf + (size_t)uniform(t.begin / p.rows.width + t.g + t.tile) * KT128 * (C::X_CHUNKS * 512);
             const uint32_t x_chunks = n > 128 ? 2 : 1;
-            for (int kt = 0; kt < KT && ok; ++kt, ++it) {
-                const int s = it % STAGES;
-                if (it >= STAGES) ok = mbar_wait(empty_bar(s), ((it / STAGES) & 1) ^ 1, p.status, ST_PRODUCER_TIMEOUT);
+            for (int kt = 0; kt < KT; ++kt, ++issued, at.step()) {
+                ok = mbar_wait(empty_bar(at.s), at.phase ^ 1u, p.status, ST_PRODUCER_TIMEOUT);      // (a fresh barrier's phase before counts as complete)
                 if (!ok) break;
-                if (lane == 0) {
-                    const uint32_t st = ring + s * C::STAGE_BYTES;
+                const uint32_t st = ring + at.s * C::STAGE_BYTES, full = full_bar(at.s);
+                if (elect_one()) {
                     if (warp == 0) {
-                        mbar_expect_tx(full_bar(s), (uint32_t)halves * (16384u + C::SF_STEPS * 512u));
-                        for (int h = 0; h < halves; ++h) tma_load_2d(st + h * 16384, &map_w, kt * C::K_STEP, w_row + h * 128, full_bar(s));
+                        mbar_expect_tx(full, (uint32_t)halves * (16384u + C::SF_STEPS * 512u));
+                        tma_load_2d(st, &map_w, kt * C::K_STEP, w_row, full);
+                        if (MH == 2 && halves == 2) tma_load_2d(st + 16384, &map_w, kt * C::K_STEP, w_row + 128, full);
 #pragma unroll
                         for (int c = 0; c < C::SF_STEPS; ++c)
-                            bulk_load(st + C::W_BYTES + C::X_BYTES + c * C::SF_STEP_BYTES, sf + (size_t)(kt * C::SF_STEPS + c) * 1024, halves * 512, full_bar(s));
+                            bulk_load(st + C::W_BYTES + C::X_BYTES + c * C::SF_STEP_BYTES, w_sf + (size_t)(kt * C::SF_STEPS + c) * 1024, halves * 512, full);
                     } else {
-                        mbar_expect_tx(full_bar(s), n * 128u + C::SF_STEPS * x_chunks * 512u);
+                        mbar_expect_tx(full, n * 128u + C::SF_STEPS * x_chunks * 512u);
                         uint32_t r = 0;
-                        for (; r + 64 <= n; r += 64) tma_load_2d(st + C::W_BYTES + r * 128, &map_x64, kt * C::K_STEP, t.row + r, full_bar(s));
-                        for (; r < n; r += 16) tma_load_2d(st + C::W_BYTES + r * 128, &map_x16, kt * C::K_STEP, t.row + r, full_bar(s));
+                        for (; r + 64 <= n; r += 64) tma_load_2d(st + C::W_BYTES + r * 128, &map_x64, kt * C::K_STEP, row + r, full);
+                        for (; r < n; r += 16) tma_load_2d(st + C::W_BYTES + r * 128, &map_x16, kt * C::K_STEP, row + r, full);
 #pragma unroll
                         for (int c = 0; c < C::SF_STEPS; ++c)
                             bulk_load(st + C::W_BYTES + C::X_BYTES + c * C::SF_STEP_BYTES + MH * 512, x_sf + (size_t)(kt * C::SF_STEPS + c) * (C::X_CHUNKS * 512),
-                                      x_chunks * 512u, full_bar(s));
+                                      x_chunks * 512u, full);
                     }
                 }
                 __syncwarp();
             }
         }
         // every copy this warp started must have landed before the CTA gives its shared memory back (returns at once in a run that went well)
-        for (uint32_t j = it > (uint32_t)STAGES ? it - STAGES : 0u; j < it; ++j)
+        for (uint32_t j = issued > (uint32_t)STAGES ? issued - STAGES : 0u; j < issued; ++j)
             mbar_wait(full_bar(j % STAGES), (j / STAGES) & 1, p.status, ST_PRODUCER_TIMEOUT);
     } else if (warp == 1) {
         // ---------------- MMA issuer ----------------
@@ -154,46 +154,44 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         // instructions take their operands from uniform registers) and the thread is elected.  The scales of a stage are copied
         // to tensor memory before the last products of the stage in front of it, into the other set of columns: behind
         // them the copies would hold up the tensor pipe (256 x 240: 1330 -> 1060 cycles per 128 of K).
-        uint32_t it = 0, count = 0;
+        uint32_t count = 0, set = 0;
         bool ok = true, copied = false;
+        RingAt<STAGES> at;
         int u = blockIdx.x;
         Unit next = u < walk.total ? walk.at(u, C::FEATURES) : Unit{};
-        auto stage_sf = [&](uint32_t i) { return ring + (i % STAGES) * C::STAGE_BYTES + C::W_BYTES + C::X_BYTES; };
-        auto copy_scales = [&](uint32_t i, int halves, uint32_t n) {
-            const uint32_t set = (i & 1u) * C::SF_COLS, sf = stage_sf(i);
+        auto copy_scales = [&](int s, uint32_t into, int halves, uint32_t n) {
+            const uint32_t sf = ring + s * C::STAGE_BYTES + C::W_BYTES + C::X_BYTES, sfw = tmem + C::SFW_COL + into, sfx = tmem + C::SFX_COL + into;
             if (elect_one()) {
 #pragma unroll
                 for (int c = 0; c < C::SF_STEPS; ++c) {
                     const uint32_t src = sf + c * C::SF_STEP_BYTES;
-                    tmem_cp_32x128b(tmem + C::SFW_COL + set + 8 * c, smem_desc(src, 0, 128, LAYOUT_NONE));
-                    if (MH == 2 && halves == 2) tmem_cp_32x128b(tmem + C::SFW_COL + set + 8 * c + 4, smem_desc(src + 512, 0, 128, LAYOUT_NONE));
-                    tmem_cp_32x128b(tmem + C::SFX_COL + set + 8 * c, smem_desc(src + MH * 512, 0, 128, LAYOUT_NONE));
-                    if (C::X_CHUNKS == 2 && n > 128)
-                        tmem_cp_32x128b(tmem + C::SFX_COL + set + 8 * c + 4, smem_desc(src + MH * 512 + 512, 0, 128, LAYOUT_NONE));
+                    tmem_cp_32x128b(sfw + 8 * c, smem_desc(src, 0, 128, LAYOUT_NONE));
+                    if (MH == 2 && halves == 2) tmem_cp_32x128b(sfw + 8 * c + 4, smem_desc(src + 512, 0, 128, LAYOUT_NONE));
+                    tmem_cp_32x128b(sfx + 8 * c, smem_desc(src + MH * 512, 0, 128, LAYOUT_NONE));
+                    if (C::X_CHUNKS == 2 && n > 128) tmem_cp_32x128b(sfx + 8 * c + 4, smem_desc(src + MH * 512 + 512, 0, 128, LAYOUT_NONE));
                 }
             }
             __syncwarp();
         };
         for (; u < walk.total && ok; u += gridDim.x, ++count) {
-            const int halves = __shfl_sync(~0u, halves_of(next), 0);
-            const uint32_t n = __shfl_sync(~0u, next.padded(), 0);
+            const int halves = uniform(halves_of(next));
+            const uint32_t n = uniform(next.padded());
             const bool more = u + (int)gridDim.x < walk.total;
             if (more) next = walk.at(u + gridDim.x, C::FEATURES);
-            const int next_halves = __shfl_sync(~0u, halves_of(next), 0);
-            const uint32_t next_n = __shfl_sync(~0u, next.padded(), 0);
+            const int next_halves = uniform(halves_of(next));
+            const uint32_t next_n = uniform(next.padded());
             const uint32_t idesc_n = p.idesc | ((n >> 3) << 17);
             const int buf = MH == 1 ? (int)(count & 1u) : 0;
-            for (int kt = 0; kt < KT && ok; ++kt, ++it) {
-                const int s = it % STAGES;
-                const uint32_t st = ring + s * C::STAGE_BYTES;
-                const uint32_t set = (it & 1u) * C::SF_COLS;
+            for (int kt = 0; kt < KT; ++kt, set ^= C::SF_COLS) {
+                const uint32_t st = ring + at.s * C::STAGE_BYTES, empty = empty_bar(at.s);
                 if (!copied) {
-                    ok = mbar_wait(full_bar(s), (it / STAGES) & 1, p.status, ST_MMA_TIMEOUT);
+                    ok = mbar_wait(full_bar(at.s), at.phase, p.status, ST_MMA_TIMEOUT);
                     tc_fence_after();
-                    if (ok) copy_scales(it, halves, n);
+                    if (!ok) break;
+                    copy_scales(at.s, set, halves, n);
                 }
                 copied = false;
-                auto products = [&](int h, int a) {
+                auto products = [&](int h, int a, bool last) {
                     const uint64_t w_desc = smem_desc(st + h * 16384, 16, 1024, LAYOUT_SW128), x_desc = smem_desc(st + C::W_BYTES, 16, 1024, LAYOUT_SW128);
                     const uint32_t d = tmem + a * C::ACC_STRIDE, sfw = tmem + C::SFW_COL + set + 4 * h, sfx = tmem + C::SFX_COL + set;
                     if (elect_one()) {
@@ -207,27 +205,28 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                                 mma_mxf8f6f4(d, w_desc + 2 * k, x_desc + 2 * k, idesc_n | (k << 29) | (k << 4), sfw, sfx, acc);
                             }
                         }
+                        if (last) mma_commit(empty);                               // frees the stage once these products have read it
                     }
                     __syncwarp();
                 };
                 // the first product into an accumulator overwrites it: the epilogue must have read what it held
                 auto free_accumulator = [&](int a, uint32_t uses) {
-                    if (kt == 0 && uses > 0 && ok) { ok = mbar_wait(accum_empty(a), (uses - 1) & 1, p.status, ST_MMA_TIMEOUT); tc_fence_after(); }
+                    if (kt == 0 && uses > 0) { ok = mbar_wait(accum_empty(a), (uses - 1) & 1, p.status, ST_MMA_TIMEOUT); tc_fence_after(); }
                     return ok;
                 };
-                if (MH == 2 && free_accumulator(0, count)) products(0, 0);
-                if (ok && (kt + 1 < KT || more) && mbar_test_wait(full_bar((it + 1) % STAGES), ((it + 1) / STAGES) & 1)) {
+                at.step();
+                if (MH == 2 && free_accumulator(0, count)) products(0, 0, halves == 1);
+                if (ok && (kt + 1 < KT || more) && mbar_test_wait(full_bar(at.s), at.phase)) {
                     tc_fence_after();
-                    copy_scales(it + 1, kt + 1 < KT ? halves : next_halves, kt + 1 < KT ? n : next_n);
+                    copy_scales(at.s, set ^ C::SF_COLS, kt + 1 < KT ? halves : next_halves, kt + 1 < KT ? n : next_n);
                     copied = true;
                 }
                 if constexpr (MH == 2) {
-                    if (halves == 2 && free_accumulator(1, count)) products(1, 1);
+                    if (halves == 2 && ok && free_accumulator(1, count)) products(1, 1, true);
                 } else {
-                    if (free_accumulator(buf, count >> 1)) products(0, buf);
+                    if (ok && free_accumulator(buf, count >> 1)) products(0, buf, true);
                 }
-                if (ok && elect_one()) mma_commit(empty_bar(s));
-                __syncwarp();
+                if (!ok) break;
             }
             if (elect_one()) mma_commit(accum_full(buf));
             __syncwarp();
@@ -350,8 +349,7 @@ __global__ void __launch_bounds__(256) pack_rows_kernel(const uint8_t* __restric
     __shared__ int s_tiles[MAX_GROUPS + 1], s_first[MAX_GROUPS + 1];
     s_plain[threadIdx.x] = t.plain[threadIdx.x];
     s_halved[threadIdx.x] = t.halved[threadIdx.x];
-    if (threadIdx.x < 32) build_table(g, s_tiles, s_first, threadIdx.x);
-    __syncthreads();
+    build_table(g, s_tiles, s_first);
     const int K = o_.K, blocks = (K + 127) / 128 * 4;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= (int64_t)g.rows * blocks) return;

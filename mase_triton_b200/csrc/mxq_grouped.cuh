@@ -79,6 +79,10 @@ __device__ __forceinline__ void finish(const float* slot, int lane, const float 
     for (int i = 0; i < 4; ++i) if (i < rows) store_four(at + i * 4 * pitch, left, vector, o[i]);
 }
 
+// a value that every lane holds, in a uniform register
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(~0u, v, 0); }
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(~0u, v, 0); }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap& m) { asm volatile("prefetch.tensormap [%0];" ::"l"(&m) : "memory"); }
 // one thread of a converged warp, the same one each time
 __device__ __forceinline__ bool elect_one() {
     uint32_t pred;
@@ -249,26 +253,42 @@ template <class Fn> static void with_row_format(int eb, int fb, bool nibbles, Fn
 
 // where a unit of work lies: features [f0, f0 + FEATURES) of group g for rows [row, row + rows)
 struct Unit {
-    int g, f0, ftile, row, rows, slot;
+    int g, f0, ftile, row, rows;
+    int begin, tile;             // first row of the group, row tile within it
     __device__ __forceinline__ uint32_t padded() const { return (uint32_t)(rows + 15) & ~15u; }
 };
 
-// Rows per tile of a group of n rows cut into tt = ceil(n / width) tiles: equal, a multiple of 16, at most `width`; the last tile is never empty.
-__device__ __forceinline__ int tile_rows(int n, int tt) { return ((n + tt - 1) / tt + 15) & ~15; }
+// Position in a ring of STAGES stages, and the parity of its barriers' current phase.
+template <int STAGES> struct RingAt {
+    int s = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void step() { if (++s == STAGES) { s = 0; phase ^= 1u; } }
+    __device__ __forceinline__ void step(int n) { s += n; if (s >= STAGES) { s -= STAGES; phase ^= 1u; } }       // n <= STAGES
+};
 
-// The group table (tile counts summed over the groups, first rows) and the walk over the units of one CTA.
+// Rows per tile of a group of n rows cut into tt = ceil(n / width) tiles: equal, a multiple of 16, at most `width`; the last tile is never empty.
+__device__ __forceinline__ int tile_rows(int n, int tt) { return tt == 1 ? (n + 15) & ~15 : ((n + tt - 1) / tt + 15) & ~15; }
+
+// The group table (tile counts summed over the groups, first rows) and the walk over the units of one CTA.  Called by whole warps.
 struct Walk {
     const int *tiles, *first;
-    int g, ftiles, width, total;
-    __device__ __forceinline__ Walk(const int* t, const int* f, int groups, int ftiles_, int width_)
-        : tiles(t), first(f), g(0), ftiles(ftiles_), width(width_), total(t[groups] * ftiles_) {}
+    int g, groups, ftiles, total;
+    __device__ __forceinline__ Walk(const int* t, const int* f, int groups_, int ftiles_)
+        : tiles(t), first(f), g(0), groups(groups_), ftiles(ftiles_), total(t[groups_] * ftiles_) {}
     __device__ __forceinline__ Unit at(int u, int features) {
-        while (u >= tiles[g + 1] * ftiles) ++g;                              // units are visited in rising order
-        const int tt = tiles[g + 1] - tiles[g], begin = first[g], n = first[g + 1] - begin;
-        int ti, fi;
-        tile_coords(u - tiles[g] * ftiles, tt, ftiles, ti, fi);
+        // units are visited in rising order: the first group from g on that ends behind u, 32 groups a step
+        if (groups > 1) {
+            for (;; g += 32) {
+                const int i = g + (threadIdx.x & 31);
+                const uint32_t behind = __ballot_sync(~0u, i < groups && u < tiles[min(i, groups - 1) + 1] * ftiles);
+                if (behind != 0u) { g += __ffs(behind) - 1; break; }
+            }
+        }
+        const int tt = tiles[g + 1] - tiles[g], begin = first[g], n = first[g + 1] - begin, local = u - tiles[g] * ftiles;
+        int ti = 0, fi = local;
+        if (tt > 1) tile_coords(local, tt, ftiles, ti, fi);
         const int w = tile_rows(n, tt);
-        return Unit{g, fi * features, fi, begin + ti * w, min(w, n - ti * w), begin / width + g + ti};
+        return Unit{g, fi * features, fi, begin + ti * w, min(w, n - ti * w), begin, ti};
     }
 };
 
@@ -284,26 +304,32 @@ struct Groups {
     }
 };
 
-// One warp: first[i] = the largest of offsets[0 .. i] (offsets that fall back leave an empty group and never an overlap),
-// tiles[i] = row tiles of the groups before i.
-__device__ __forceinline__ void build_table(const Groups& g, int* tiles, int* first, int lane) {
-    int high = 0, sum = 0;
-    for (int base = 0; base <= g.groups; base += 32) {
-        const int i = base + lane;
-        int v = i <= g.groups ? g.offset(i) : 0;
+// The group table, by the whole CTA: first[i] = the largest of offsets[0 .. i] (offsets that fall back leave an empty group and never
+// an overlap), tiles[i] = row tiles of the groups before i.  The offsets are loaded by all threads at once, one warp sums.
+__device__ __forceinline__ void build_table(const Groups& g, int* tiles, int* first) {
+    for (int i = threadIdx.x; i <= g.groups; i += blockDim.x) first[i] = g.offset(i);
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        const int lane = threadIdx.x;
+        int high = 0, sum = 0;
+        for (int base = 0; base <= g.groups; base += 32) {
+            const int i = base + lane;
+            int v = i <= g.groups ? first[i] : 0;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) { const int up = __shfl_up_sync(~0u, v, o); if (lane >= o) v = max(v, up); }
-        v = max(v, high);
-        const int before = __shfl_up_sync(~0u, v, 1);
-        // rows of group i - 1, which the running sum at i counts
-        int t = (i == 0 || i > g.groups) ? 0 : ((v - (lane == 0 ? high : before)) + g.width - 1) / g.width;
+            for (int o = 1; o < 32; o <<= 1) { const int up = __shfl_up_sync(~0u, v, o); if (lane >= o) v = max(v, up); }
+            v = max(v, high);
+            const int before = __shfl_up_sync(~0u, v, 1);
+            // rows of group i - 1, which the running sum at i counts
+            int t = (i == 0 || i > g.groups) ? 0 : ((v - (lane == 0 ? high : before)) + g.width - 1) / g.width;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) { const int up = __shfl_up_sync(~0u, t, o); if (lane >= o) t += up; }
-        t += sum;
-        if (i <= g.groups) { first[i] = v; tiles[i] = t; }
-        high = __shfl_sync(~0u, v, 31);
-        sum = __shfl_sync(~0u, t, 31);
+            for (int o = 1; o < 32; o <<= 1) { const int up = __shfl_up_sync(~0u, t, o); if (lane >= o) t += up; }
+            t += sum;
+            if (i <= g.groups) { first[i] = v; tiles[i] = t; }
+            high = __shfl_sync(~0u, v, 31);
+            sum = __shfl_sync(~0u, t, 31);
+        }
     }
+    __syncthreads();
 }
 
 // Where the scales of one row lie: its tile's slot and its row in the tile.

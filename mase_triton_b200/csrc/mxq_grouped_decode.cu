@@ -19,7 +19,7 @@ namespace decode {
 
 constexpr int ROWS = 16;                         // widest row tile: the narrowest the instruction takes
 constexpr int FEATURES = 128;
-constexpr int STAGES = 10;
+constexpr int STAGES = 10;                       // (not fewer than the quantising warps)
 constexpr int EPI_WARP = 4, QUANT_WARP = 8, QUANT_WARPS = 8;
 constexpr int THREADS = 512;                     // warps 0, 1: weight copies, MMA issuer; 4..7: epilogue; 8..15: quantisers
 constexpr int W_BYTES = FEATURES * 128, X_BYTES = ROWS * 128;
@@ -101,6 +101,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
+    if (warp == 0 && elect_one()) prefetch_map(map_w);
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -108,9 +109,8 @@ decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     // what the kernels before this one write (rows, offsets, perhaps the weights) is read behind this line only
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (warp == 3) build_table(p.rows, tiles, first, lane);
     tc_fence_before();
-    __syncthreads();
+    build_table(p.rows, tiles, first);
     if (split > 1) cluster_barrier();                                // every CTA's barriers exist before another one arrives there
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(~0u, *tmem_slot, 0);
@@ -119,46 +119,48 @@ decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     const int k_begin = rank * KT_all / split, KT = (rank + 1) * KT_all / split - k_begin;     // this CTA's steps of K, one at least
     const int ftiles = (p.N + FEATURES - 1) / FEATURES;
     const int u_begin = blockIdx.x / split, u_step = gridDim.x / split;
-    Walk walk(tiles, first, p.rows.groups, ftiles, p.rows.width);
+    Walk walk(tiles, first, p.rows.groups, ftiles);
 
     if (warp == 0) {
         // ---------------- weight copies ----------------
         bool ok = true;
-        uint32_t it = 0;
+        RingAt<STAGES> at;
+        uint32_t issued = 0;
         for (int u = u_begin; u < walk.total && ok; u += u_step) {
             const Unit t = walk.at(u, FEATURES);
-            const uint8_t* sf = p.w_sf + (size_t)t.g * p.w_sf_group + (size_t)(t.ftile >> 1) * KT128 * 1024 + (t.ftile & 1) * 512;
-            const int w_row = t.g * p.N + t.f0;
-            for (int kt = k_begin; kt < k_begin + KT && ok; ++kt, ++it) {
-                const int s = it % STAGES;
-                if (it >= STAGES) ok = mbar_wait(empty_bar(s), ((it / STAGES) & 1) ^ 1, p.status, ST_PRODUCER_TIMEOUT);
+            const uint8_t* sf = p.w_sf + (size_t)uniform(t.g) * p.w_sf_group + (size_t)uniform(t.ftile >> 1) * KT128 * 1024 + uniform(t.ftile & 1) * 512;
+            const int w_row = uniform(t.g * p.N + t.f0);
+            for (int kt = k_begin; kt < k_begin + KT; ++kt, ++issued, at.step()) {
+                ok = mbar_wait(empty_bar(at.s), at.phase ^ 1u, p.status, ST_PRODUCER_TIMEOUT);      // (a fresh barrier's phase before counts as complete)
                 if (!ok) break;
-                if (lane == 0) {
-                    const uint32_t st = ring + s * C::STAGE_BYTES;
-                    mbar_expect_tx(full_bar(s), W_BYTES + C::SF_STEPS * 512u);
-                    tma_load_2d(st, &map_w, kt * C::K_STEP, w_row, full_bar(s));
+                const uint32_t st = ring + at.s * C::STAGE_BYTES, full = full_bar(at.s);
+                if (elect_one()) {
+                    mbar_expect_tx(full, W_BYTES + C::SF_STEPS * 512u);
+                    tma_load_2d(st, &map_w, kt * C::K_STEP, w_row, full);
 #pragma unroll
                     for (int c = 0; c < C::SF_STEPS; ++c)
-                        bulk_load(st + W_BYTES + X_BYTES + c * 1024, sf + (size_t)(kt * C::SF_STEPS + c) * 1024, 512, full_bar(s));
+                        bulk_load(st + W_BYTES + X_BYTES + c * 1024, sf + (size_t)(kt * C::SF_STEPS + c) * 1024, 512, full);
                 }
                 __syncwarp();
             }
         }
         // every copy must have landed before the CTA gives its shared memory back (returns at once in a run that went well)
-        for (uint32_t j = it > (uint32_t)STAGES ? it - STAGES : 0u; j < it; ++j)
+        for (uint32_t j = issued > (uint32_t)STAGES ? issued - STAGES : 0u; j < issued; ++j)
             mbar_wait(full_bar(j % STAGES), (j / STAGES) & 1, p.status, ST_PRODUCER_TIMEOUT);
     } else if (warp == 1) {
         // ---------------- MMA issuer: uniform over the warp, scales one stage ahead (see mxq_grouped.cu) ----------------
-        uint32_t it = 0, count = 0;
+        uint32_t count = 0, set = 0;
         bool ok = true, copied = false;
+        RingAt<STAGES> at;
+        constexpr uint32_t SF_COLS = C::SF_STEPS * 8;
         const uint32_t idesc = p.idesc | ((uint32_t)(ROWS >> 3) << 17);
-        auto copy_scales = [&](uint32_t i) {
-            const uint32_t set = (i & 1u) * (C::SF_STEPS * 8), sf = ring + (i % STAGES) * C::STAGE_BYTES + W_BYTES + X_BYTES;
+        auto copy_scales = [&](int s, uint32_t into) {
+            const uint32_t sf = ring + s * C::STAGE_BYTES + W_BYTES + X_BYTES, sfw = tmem + SFW_COL + into, sfx = tmem + SFX_COL + into;
             if (elect_one()) {
 #pragma unroll
                 for (int c = 0; c < C::SF_STEPS; ++c) {
-                    tmem_cp_32x128b(tmem + SFW_COL + set + 8 * c, smem_desc(sf + c * 1024, 0, 128, LAYOUT_NONE));
-                    tmem_cp_32x128b(tmem + SFX_COL + set + 8 * c, smem_desc(sf + c * 1024 + 512, 0, 128, LAYOUT_NONE));
+                    tmem_cp_32x128b(sfw + 8 * c, smem_desc(sf + c * 1024, 0, 128, LAYOUT_NONE));
+                    tmem_cp_32x128b(sfx + 8 * c, smem_desc(sf + c * 1024 + 512, 0, 128, LAYOUT_NONE));
                 }
             }
             __syncwarp();
@@ -168,23 +170,24 @@ decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
             const int a = (int)(count & 1u);
             if (count >= 2) ok = mbar_wait(accum_empty(a), ((count >> 1) - 1) & 1, p.status, ST_MMA_TIMEOUT);
             tc_fence_after();
-            for (int kt = 0; kt < KT && ok; ++kt, ++it) {
-                const int s = it % STAGES;
-                const uint32_t st = ring + s * C::STAGE_BYTES, set = (it & 1u) * (C::SF_STEPS * 8);
+            const uint32_t d = tmem + a * ACC_STRIDE;
+            for (int kt = 0; kt < KT && ok; ++kt, set ^= SF_COLS) {
+                const uint32_t st = ring + at.s * C::STAGE_BYTES, empty = empty_bar(at.s);
                 if (!copied) {
-                    ok = mbar_wait(full_bar(s), (it / STAGES) & 1, p.status, ST_MMA_TIMEOUT);
+                    ok = mbar_wait(full_bar(at.s), at.phase, p.status, ST_MMA_TIMEOUT);
                     tc_fence_after();
-                    if (ok) copy_scales(it);
+                    if (!ok) break;
+                    copy_scales(at.s, set);
                 }
                 copied = false;
-                if (!ok) break;
-                if ((kt + 1 < KT || more) && mbar_test_wait(full_bar((it + 1) % STAGES), ((it + 1) / STAGES) & 1)) {
+                at.step();
+                if ((kt + 1 < KT || more) && mbar_test_wait(full_bar(at.s), at.phase)) {
                     tc_fence_after();
-                    copy_scales(it + 1);
+                    copy_scales(at.s, set ^ SF_COLS);
                     copied = true;
                 }
                 const uint64_t w_desc = smem_desc(st, 16, 1024, LAYOUT_SW128), x_desc = smem_desc(st + W_BYTES, 16, 1024, LAYOUT_SW128);
-                const uint32_t d = tmem + a * ACC_STRIDE, sfw = tmem + SFW_COL + set, sfx = tmem + SFX_COL + set;
+                const uint32_t sfw = tmem + SFW_COL + set, sfx = tmem + SFX_COL + set;
                 if (elect_one()) {
 #pragma unroll
                     for (uint32_t k = 0; k < 4; ++k) {
@@ -196,7 +199,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
                             mma_mxf8f6f4(d, w_desc + 2 * k, x_desc + 2 * k, idesc | (k << 29) | (k << 4), sfw, sfx, acc);
                         }
                     }
-                    mma_commit(empty_bar(s));
+                    mma_commit(empty);
                 }
                 __syncwarp();
             }
@@ -217,7 +220,8 @@ decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         using KIn = typename std::conditional<DT == MXQ_F32, KF32, typename std::conditional<DT == MXQ_BF16, KBF16, KF16>::type>::type;
         const int kl = (lane & 15) * E;                                                  // this lane's first element of a step
         int u = u_begin, kt = warp - QUANT_WARP;
-        uint32_t it = kt;
+        RingAt<STAGES> at;
+        at.step(kt);
         bool fresh = true, ok = true;
         Unit t{};
         int from[PAIRS];                                                                 // rows of x; -1: a row of zeros, -2: none
@@ -239,8 +243,8 @@ decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
                     }
                 }
             }
-            const int s = it % STAGES, k = (k_begin + kt) * C::K_STEP + kl;
-            uint8_t* st = ring_ptr + s * C::STAGE_BYTES;
+            const int k = (k_begin + kt) * C::K_STEP + kl;
+            uint8_t* st = ring_ptr + at.s * C::STAGE_BYTES;
             bool first_batch = true;
 #pragma unroll
             for (int i0 = 0; i0 < PAIRS; i0 += BATCH) {
@@ -259,7 +263,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
                     }
                 if (first_batch) {
                     first_batch = false;
-                    if (it >= STAGES) ok = mbar_wait(empty_bar(s), ((it / STAGES) & 1) ^ 1, p.status, ST_PRODUCER_TIMEOUT);
+                    ok = mbar_wait(empty_bar(at.s), at.phase ^ 1u, p.status, ST_PRODUCER_TIMEOUT);
                     if (!ok) break;
                 }
 #pragma unroll
@@ -283,8 +287,8 @@ decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
             if (!ok) break;
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(full_bar(s));
-            it += QUANT_WARPS;
+            if (lane == 0) mbar_arrive(full_bar(at.s));
+            at.step(QUANT_WARPS);
             kt += QUANT_WARPS;
         }
     } else if (warp >= EPI_WARP) {
