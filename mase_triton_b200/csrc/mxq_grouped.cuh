@@ -263,7 +263,7 @@ template <int STAGES> struct RingAt {
     int s = 0;
     uint32_t phase = 0;
     __device__ __forceinline__ void step() { if (++s == STAGES) { s = 0; phase ^= 1u; } }
-    __device__ __forceinline__ void step(int n) { s += n; if (s >= STAGES) { s -= STAGES; phase ^= 1u; } }       // n <= STAGES
+    __device__ __forceinline__ void step(int n) { for (s += n; s >= STAGES; s -= STAGES) phase ^= 1u; }
 };
 
 // Rows per tile of a group of n rows cut into tt = ceil(n / width) tiles: equal, a multiple of 16, at most `width`; the last tile is never empty.

@@ -2,11 +2,12 @@
 //
 // What bounds such a call is one read of the weights and, below some 20 us, everything in front of and behind it: launches, the
 // ramp of the grid, a second kernel's hand-over.  So
-//   * eight warps of every CTA quantise the rows of its tile (16 at most) as they go along K, straight into the ring of
+//   * five warps of every CTA (four for 4-bit pairs) quantise the rows of its tile (16 at most) as they go along K, straight into the ring of
 //     shared memory that the tensor cores read, a stage each in turn: one warp's way through a stage (a load, the block
 //     maximum, the rounding, a proxy fence) takes far longer than the stage's products.  Every CTA repeats this for its own features,
 //     out of L2 and beside the weights' copies, which take longer; there is no second launch, no operand in memory and no workspace;
-//   * the ring holds ten stages of 128 features x 128 elements: 160 KB of weights in flight per SM;
+//   * two CTAs fit on an SM (a ring of 64 to 80 KB each): one's start and end hide behind the other's copies, within a call and, with
+//     the launch that may overlap the kernel before, between calls;
 //   * where the features leave SMs idle, K is split over a cluster of 2 or 4 CTAs.  Each sums its part in tensor memory; the
 //     partial sums go to the CTA that finishes those features through distributed shared memory and are added in the
 //     order of the CTAs, so that results do not depend on which comes first.
@@ -19,21 +20,24 @@ namespace decode {
 
 constexpr int ROWS = 16;                         // widest row tile: the narrowest the instruction takes
 constexpr int FEATURES = 128;
-constexpr int STAGES = 10;                       // (not fewer than the quantising warps)
-constexpr int EPI_WARP = 4, QUANT_WARP = 8, QUANT_WARPS = 8;
-constexpr int THREADS = 512;                     // warps 0, 1: weight copies, MMA issuer; 4..7: epilogue; 8..15: quantisers
+constexpr int EPI_WARP = 4;
+constexpr int THREADS = 352;                     // warps 0, 1: weight copies, MMA issuer; 4..7: epilogue; 2, 3, 8..10: quantisers
 constexpr int W_BYTES = FEATURES * 128, X_BYTES = ROWS * 128;
 constexpr int TMEM_COLS = 128;
 constexpr int ACC_STRIDE = 32, SFW_COL = 64, SFX_COL = 96;
 
 template <bool MXF4> struct Cfg {
     static constexpr int K_STEP = MXF4 ? 256 : 128, SF_STEPS = MXF4 ? 2 : 1;
+    static constexpr int STAGES = MXF4 ? 4 : 5;
+    // a warp that took a stage more than one turn of the ring ahead would mistake the phase its barrier is in
+    static constexpr int QUANT_WARPS = STAGES;
+    static_assert(QUANT_WARPS <= STAGES && EPI_WARP + 2 + QUANT_WARPS <= THREADS / 32, "quantising warps");
     static constexpr int STAGE_BYTES = W_BYTES + X_BYTES + SF_STEPS * 1024;          // scales: 512 bytes of either operand per 128 elements of K
-    static constexpr int TABLE_END = (256 + 2 * (MAX_GROUPS + 1) * 4 + 15) / 16 * 16;
     static constexpr int SLOTS = 4 * 2048, EXCHANGE = 3 * 2048;                      // 32 features x 16 rows per epilogue warp, and per part received
-    static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + TABLE_END + SLOTS + EXCHANGE;
+    static constexpr int FIXED_BYTES = 1024 + STAGES * STAGE_BYTES + 256 + SLOTS + EXCHANGE;
+    static int smem_bytes(int groups) { return FIXED_BYTES + 2 * (groups + 1) * 4; }  // the group table comes last
     static_assert(STAGE_BYTES % 1024 == 0, "the 128-byte swizzle repeats every 1024 bytes");
-    static_assert(SMEM_BYTES <= 232448, "more shared memory than a CTA can have");
+    static_assert(FIXED_BYTES + 2 * (MAX_GROUPS + 1) * 4 <= 232448, "more shared memory than a CTA can have");
 };
 
 struct Source {
@@ -51,6 +55,7 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
 __device__ __forceinline__ void cluster_barrier() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // bounded wait for a phase that other CTAs of the cluster complete
 __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, int* status, int code) {
     for (uint32_t i = 0; i < SPIN_LIMIT; ++i) {
@@ -69,26 +74,28 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity,
 
 // DT: type of x, out, bias and extra; F, OUT: element format of the rows and what the tensor cores read of it
 template <int DT, class F, int OUT>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(THREADS, 2)
 decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ Params p, const __grid_constant__ Source src, int split) {
     constexpr bool MXF4 = OUT == 5;
     using C = Cfg<MXF4>;
+    constexpr int STAGES = C::STAGES;
     typedef typename Elem<DT>::T T;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t ring = (raw + 1023u) & ~1023u;
     uint8_t* ring_ptr = smem_raw + (ring - raw);
-    const uint32_t bars = ring + STAGES * C::STAGE_BYTES;            // full[S], empty[S], accum_full[2], accum_empty[2], drain, parts, tmem slot
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ring_ptr + STAGES * C::STAGE_BYTES + 8 * (2 * STAGES + 6));
-    int* tiles = reinterpret_cast<int*>(ring_ptr + STAGES * C::STAGE_BYTES + 256);
-    int* first = tiles + MAX_GROUPS + 1;
-    float* slots = reinterpret_cast<float*>(ring_ptr + STAGES * C::STAGE_BYTES + C::TABLE_END);
+    const uint32_t bars = ring + STAGES * C::STAGE_BYTES;            // full[S], empty[S], accum_full[2], accum_empty[2], drain, parts, rows requested, tmem slot
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ring_ptr + STAGES * C::STAGE_BYTES + 8 * (2 * STAGES + 7));
+    float* slots = reinterpret_cast<float*>(ring_ptr + STAGES * C::STAGE_BYTES + 256);
     float* exchange = slots + C::SLOTS / 4;
+    int* tiles = reinterpret_cast<int*>(exchange + C::EXCHANGE / 4);
+    int* first = tiles + p.rows.groups + 1;
     auto full_bar = [&](int s) { return bars + 8u * s; };
     auto empty_bar = [&](int s) { return bars + 8u * (STAGES + s); };
     auto accum_full = [&](int a) { return bars + 8u * (2 * STAGES + a); };
     auto accum_empty = [&](int a) { return bars + 8u * (2 * STAGES + 2 + a); };
     const uint32_t drain_bar = bars + 8u * (2 * STAGES + 4), parts_bar = bars + 8u * (2 * STAGES + 5);
+    const uint32_t rows_bar = bars + 8u * (2 * STAGES + 6);
 
     const int warp = __shfl_sync(~0u, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int rank = split > 1 ? (int)(blockIdx.x % (unsigned)split) : 0;           // clusters are consecutive CTAs
@@ -97,6 +104,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         for (int s = 0; s < STAGES; ++s) { mbar_init(full_bar(s), 2); mbar_init(empty_bar(s), 1); }
         for (int a = 0; a < 2; ++a) { mbar_init(accum_full(a), 1); mbar_init(accum_empty(a), 4); }
         mbar_init(drain_bar, 1);
+        mbar_init(rows_bar, C::QUANT_WARPS);
         mbar_init(parts_bar, (split - 1) * quads + (split == 1 ? 1 : 0));
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -106,9 +114,10 @@ decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    // what the kernels before this one write (rows, offsets, perhaps the weights) is read behind this line only
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    // What the kernels before this one write (rows, offsets, perhaps the weights) is read behind a wait for their end only: here
+    // for offsets; without them every warp gets as far as its first access and waits there.
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (p.rows.offsets != nullptr) dependency_wait();
     tc_fence_before();
     build_table(p.rows, tiles, first);
     if (split > 1) cluster_barrier();                                // every CTA's barriers exist before another one arrives there
@@ -134,6 +143,10 @@ decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
                 ok = mbar_wait(empty_bar(at.s), at.phase ^ 1u, p.status, ST_PRODUCER_TIMEOUT);      // (a fresh barrier's phase before counts as complete)
                 if (!ok) break;
                 const uint32_t st = ring + at.s * C::STAGE_BYTES, full = full_bar(at.s);
+                // The weights that all CTAs ask for at once keep the memory busy for microseconds.  The first rows, which everything
+                // waits for, are asked for in front of all but one stage of them.
+                if (issued == 0) dependency_wait();
+                if (issued == 1) mbar_wait(rows_bar, 0, p.status, ST_PRODUCER_TIMEOUT);
                 if (elect_one()) {
                     mbar_expect_tx(full, W_BYTES + C::SF_STEPS * 512u);
                     tma_load_2d(st, &map_w, kt * C::K_STEP, w_row, full);
@@ -212,67 +225,72 @@ decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
             __syncwarp();
             mbar_wait(drain_bar, 0, nullptr, 0);
         }
-    } else if (warp >= QUANT_WARP) {
-        // ---------------- rows: a warp takes every eighth stage, 16 lanes a row, two rows at a time ----------------
+    } else if (warp < EPI_WARP || warp >= EPI_WARP + 4) {
+        // ---------------- rows: a warp takes every fifth (fourth) stage, 16 lanes a row, two rows at a time ----------------
         constexpr int E = MXF4 ? 16 : 8, WORDS = E * (int)sizeof(T) / 4;                 // elements and words per lane and row
-        constexpr int BATCH = 32 / WORDS;                                                // row pairs whose loads are issued together (32 registers)
+        constexpr int BATCH = 16 / WORDS;                                                // row pairs whose loads are issued together (16 registers)
         constexpr int PAIRS = ROWS / 2;
         using KIn = typename std::conditional<DT == MXQ_F32, KF32, typename std::conditional<DT == MXQ_BF16, KBF16, KF16>::type>::type;
         const int kl = (lane & 15) * E;                                                  // this lane's first element of a step
-        int u = u_begin, kt = warp - QUANT_WARP;
+        const int turn = warp < EPI_WARP ? warp - 2 : warp - EPI_WARP - 2;
+        int u = u_begin, kt = turn;
         RingAt<STAGES> at;
-        at.step(kt);
-        bool fresh = true, ok = true;
+        at.step(turn);
+        bool ok = true, live = turn < C::QUANT_WARPS, fresh = live;
         Unit t{};
         int from[PAIRS];                                                                 // rows of x; -1: a row of zeros, -2: none
-        while (ok) {
-            while (kt >= KT && u < walk.total) { kt -= KT; u += u_step; fresh = true; }
-            if (u >= walk.total) break;
-            if (fresh) {
-                fresh = false;
-                t = walk.at(u, FEATURES);
+        // the unit of this warp's next stage, and where its rows lie
+        auto open = [&]() {
+            while (live && kt >= KT) { kt -= KT; u += u_step; fresh = true; live = u < walk.total; }
+            live = live && u < walk.total;
+            if (!live || !fresh) return;
+            fresh = false;
+            t = walk.at(u, FEATURES);
 #pragma unroll
-                for (int i = 0; i < PAIRS; ++i) {
-                    const int r = 2 * i + (lane >> 4);
-                    from[i] = r < t.rows ? -1 : -2;
-                    if (r < t.rows) {
-                        int64_t row = t.row + r;
-                        if (src.row_index != nullptr)
-                            row = src.index64 ? reinterpret_cast<const long long*>(src.row_index)[row] : (int64_t)reinterpret_cast<const int*>(src.row_index)[row];
-                        if (row >= 0 && row < src.rows_in) from[i] = (int)row;
-                    }
+            for (int i = 0; i < PAIRS; ++i) {
+                const int r = 2 * i + (lane >> 4);
+                from[i] = r < t.rows ? -1 : -2;
+                if (r < t.rows) {
+                    int64_t row = t.row + r;
+                    if (src.row_index != nullptr)
+                        row = src.index64 ? reinterpret_cast<const long long*>(src.row_index)[row] : (int64_t)reinterpret_cast<const int*>(src.row_index)[row];
+                    if (row >= 0 && row < src.rows_in) from[i] = (int)row;
                 }
             }
+        };
+        uint32_t w[BATCH][WORDS];
+        auto request = [&](int i0) {                                                     // row pairs i0 .. i0 + BATCH - 1 of the stage
             const int k = (k_begin + kt) * C::K_STEP + kl;
-            uint8_t* st = ring_ptr + at.s * C::STAGE_BYTES;
-            bool first_batch = true;
 #pragma unroll
-            for (int i0 = 0; i0 < PAIRS; i0 += BATCH) {
-                if (2 * i0 >= t.rows) break;
-                uint32_t w[BATCH][WORDS];
+            for (int i = 0; i < BATCH; ++i)
 #pragma unroll
-                for (int i = 0; i < BATCH; ++i)
-#pragma unroll
-                    for (int j = 0; j < WORDS; j += 4) {
-                        // a row that does not exist reads as ones (it does not hold up the short form), one outside x as zeros
-                        const uint32_t fill = from[i0 + i] == -2 ? one_bits<KIn>() : 0u;
-                        uint4 q = make_uint4(fill, fill, fill, fill);
-                        if (from[i0 + i] >= 0 && k < p.K)
-                            q = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(src.x) + (int64_t)from[i0 + i] * p.K + k) + j / 4);
-                        w[i][j] = q.x; w[i][j + 1] = q.y; w[i][j + 2] = q.z; w[i][j + 3] = q.w;
-                    }
-                if (first_batch) {
-                    first_batch = false;
-                    ok = mbar_wait(empty_bar(at.s), at.phase ^ 1u, p.status, ST_PRODUCER_TIMEOUT);
-                    if (!ok) break;
+                for (int j = 0; j < WORDS; j += 4) {
+                    // a row that does not exist reads as ones (it does not hold up the short form), one outside x as zeros
+                    const uint32_t fill = from[i0 + i] == -2 ? one_bits<KIn>() : 0u;
+                    uint4 q = make_uint4(fill, fill, fill, fill);
+                    if (from[i0 + i] >= 0 && k < p.K)
+                        q = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(src.x) + (int64_t)from[i0 + i] * p.K + k) + j / 4);
+                    w[i][j] = q.x; w[i][j + 1] = q.y; w[i][j + 2] = q.z; w[i][j + 3] = q.w;
                 }
+        };
+        if (src.row_index != nullptr) dependency_wait();
+        open();
+        dependency_wait();
+        if (live) request(0);
+        if (turn < C::QUANT_WARPS && lane == 0) mbar_arrive(rows_bar);
+        while (ok && live) {
+            const int k = (k_begin + kt) * C::K_STEP + kl, rows = t.rows;
+            uint8_t* st = ring_ptr + at.s * C::STAGE_BYTES;
+            ok = mbar_wait(empty_bar(at.s), at.phase ^ 1u, p.status, ST_PRODUCER_TIMEOUT);
+            if (!ok) break;
+            auto quantise = [&](int i0) {
 #pragma unroll
                 for (int i = 0; i < BATCH; ++i) {
-                    if (2 * (i0 + i) >= t.rows) break;                                   // uniform: neither row of the pair exists
+                    if (2 * (i0 + i) >= rows) break;                                     // uniform: neither row of the pair exists
                     uint32_t codes[2];
                     const uint32_t sbyte = quantise_part<KIn, F, OUT, E>(w[i], codes);
                     const int r = 2 * (i0 + i) + (lane >> 4);
-                    if (r < t.rows) {
+                    if (r < rows) {
                         // 8 of the row's 128 bytes: 16-byte unit j lies at j ^ (r % 8)
                         const uint32_t j = (lane & 15) >> 1;
                         *reinterpret_cast<uint2*>(st + W_BYTES + r * 128 + ((j ^ (r & 7)) << 4) + (lane & 1) * 8) = make_uint2(codes[0], codes[1]);
@@ -283,13 +301,22 @@ decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
                         }
                     }
                 }
+            };
+            quantise(0);
+#pragma unroll
+            for (int i0 = BATCH; i0 < PAIRS; i0 += BATCH) {
+                if (2 * i0 >= rows) break;
+                request(i0);
+                quantise(i0);
             }
-            if (!ok) break;
+            // the next stage's first rows are on their way while this one is handed over and the ring has no room
+            kt += C::QUANT_WARPS;
+            open();
+            if (live) request(0);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(full_bar(at.s));
-            at.step(QUANT_WARPS);
-            kt += QUANT_WARPS;
+            at.step(C::QUANT_WARPS);
         }
     } else if (warp >= EPI_WARP) {
         // ---------------- epilogue: 32 features of 16 rows per warp ----------------
@@ -301,6 +328,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         const int owner = q / quads;                                                     // the CTA of the cluster that finishes these features
         bool ok = true;
         uint32_t count = 0;
+        dependency_wait();
         for (int u = u_begin; u < walk.total && ok; u += u_step, ++count) {
             const Unit t = walk.at(u, FEATURES);
             const int a = (int)(count & 1u), f = t.f0 + ef;
@@ -377,16 +405,16 @@ template <int DT, class F, int OUT>
 static int launch(const Params& p, const Source& src, const uint8_t* w_codes, int split, cudaStream_t st) {
     using C = Cfg<OUT == 5>;
     static bool attr_done[MAX_DEVICES] = {false};
-    cudaError_t e = raise_smem_limit(decode_kernel<DT, F, OUT>, C::SMEM_BYTES, attr_done);
+    cudaError_t e = raise_smem_limit(decode_kernel<DT, F, OUT>, C::smem_bytes(MAX_GROUPS), attr_done);
     if (e != cudaSuccess) { set_last_cuda_error(e); return MXQ_ELAUNCH; }
     CUtensorMap mw;
     if (!make_map(&mw, w_codes, (int64_t)p.rows.groups * p.N, p.K, FEATURES, OUT == 5)) return MXQ_ELAUNCH;
-    const int64_t units = most_units(p.rows, p.N, FEATURES);
+    const int64_t units = most_units(p.rows, p.N, FEATURES), room = 2 * sm_count();
     cudaLaunchConfig_t cfg = {};
     // a cluster works on one unit; without clusters the CTAs stay and walk over theirs
-    cfg.gridDim = dim3((unsigned)(split > 1 ? units * split : units < sm_count() ? units : sm_count()));
+    cfg.gridDim = dim3((unsigned)(split > 1 ? units * split : units < room ? units : room));
     cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = C::SMEM_BYTES;
+    cfg.dynamicSmemBytes = (size_t)C::smem_bytes(p.rows.groups);
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -407,11 +435,11 @@ int decode_rows() { return decode::ROWS; }
 
 int launch_decode(const Params& p, int dt, const void* x, const void* row_index, int index64, int64_t rows_in, int eb, int fb, bool nibbles,
                   const uint8_t* w_codes, cudaStream_t st) {
-    // CTAs that share a unit: as many as the SMs hold, the steps of K allow, and 4 at most (a lane quadrant each)
+    // CTAs that share a unit: as many as the SMs hold (two each), the steps of K allow, and 4 at most (a lane quadrant each)
     const int64_t units = most_units(p.rows, p.N, decode::FEATURES);
     const int steps = (p.K + (nibbles ? 255 : 127)) / (nibbles ? 256 : 128);
     int split = 1;
-    while (split < 4 && units * split * 2 <= sm_count() && steps >= split * 2 * 4) split *= 2;
+    while (split < 4 && units * split * 2 <= 2 * sm_count() && steps >= split * 2 * 4) split *= 2;
     const decode::Source src{x, row_index, index64, rows_in};
     int rc = MXQ_ESIZE;
     with_row_format(eb, fb, nibbles, [&](auto fmt, auto out) {
