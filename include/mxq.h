@@ -357,13 +357,13 @@ int mxq_mx_linear_static(const void* x, int x_dtype, int64_t M, int64_t K, int x
  * Q quantises to MXFP (32-element blocks along K, is_finite elements of x_exp_bits / x_frac_bits, any rounding mode);
  * products, bias, activation and the second operand in fp32, one rounding to the output's type.
  * mxq_mx_pack_experts re-encodes the weights once: scales / elements of a [groups, N, K] tensor blocked along K, as
- * mxq_mxfp_extract writes them, into hw_codes (groups * N * K bytes; half of that with `nibbles`, 32-byte aligned) and
- * hw_sf (groups * mxq_mx_sf_bytes(N, K, MXQ_OPERAND_A, 0) bytes).  `nibbles`: keep E2M1 codes two per byte for an E2M1
- * activation (K % 256 == 0), which then runs on the 4-bit x 4-bit tensor-core kind.
+ * mxq_mxfp_extract writes them, into mxq_mx_packed_experts_bytes(groups, N, K, nibbles) bytes of blocks that the kernels copy
+ * to shared memory as they are (128 features x 128 elements and their scales each; 16-byte aligned).  `nibbles`: keep E2M1
+ * codes two per byte for an E2M1 activation (K % 256 == 0), which then runs on the 4-bit x 4-bit tensor-core kind.
  */
+int64_t mxq_mx_packed_experts_bytes(int64_t groups, int64_t N, int64_t K, int nibbles);
 int mxq_mx_pack_experts(const uint8_t* scales, const uint8_t* elements, int64_t groups, int64_t N, int64_t K,
-                        int exp_bits, int frac_bits, int nibbles, uint8_t* hw_codes, uint8_t* hw_sf,
-                        int* hw_format, void* stream);
+                        int exp_bits, int frac_bits, int nibbles, uint8_t* packed, int* hw_format, void* stream);
 /* Largest number of groups (1024). */
 int mxq_mx_max_groups(void);
 /*
@@ -376,14 +376,14 @@ int mxq_mx_max_groups(void);
  *   zero_rest : rows of out outside every group are set to zero; otherwise they are left as they are.
  *   scratch   : 256-byte aligned, at least mxq_mx_grouped_scratch_bytes(...) bytes, of this call alone; that is 0, and scratch may
  *               be NULL, for a few rows per group on 16 bytes (one kernel that keeps the quantised rows on the chip).
- * `extra` may be the same buffer as `out`.  K % 32 == 0, w_hw_format / w_codes / w_sf from mxq_mx_pack_experts.
+ * `extra` may be the same buffer as `out`.  K % 32 == 0, w_packed / w_hw_format from mxq_mx_pack_experts.
  * `status` as for mxq_mx_gemm.
  */
 int64_t mxq_mx_grouped_scratch_bytes(const void* x, int x_round_mode, int64_t rows_in, int64_t rows, int64_t K, int64_t groups);
 int mxq_mx_grouped_linear(const void* x, int x_dtype, int64_t rows_in, int64_t rows, int64_t K, int x_exp_bits,
                           int x_frac_bits, int x_round_mode, const void* row_index, int index64,
-                          const uint8_t* w_codes, const uint8_t* w_sf, int w_hw_format, int64_t groups, int64_t N,
-                          const void* offsets, int offsets64, void* out, const void* bias, int activation,
+                          const uint8_t* w_packed, int w_hw_format, int64_t groups, int64_t N, const void* offsets,
+                          int offsets64, void* out, const void* bias, int activation,
                           const void* extra, int extra_mode, int zero_rest, void* scratch, int64_t scratch_bytes,
                           int* status, void* stream);
 

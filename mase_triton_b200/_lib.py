@@ -39,8 +39,8 @@ SIGNATURES = {
     "mxq_mx_gemm_gather": [_p, _p, _i, _p, _p, _i, _i, _p, _i, _i, _i64, _i64, _i, _p, _i64, _i64, _i64, _p, _p],
     "mxq_mx_linear": [_p, _i, _i64, _i64, _i, _i, _p, _p, _i, _i, _i64, _p, _i, _p, _p, _i64, _p, _p],
     "mxq_mx_linear_static": [_p, _i, _i64, _i64, _i, _i, _p, _p, _i, _i, _i64, _p, _i, _p, _p, _p],
-    "mxq_mx_pack_experts": [_p, _p, _i64, _i64, _i64, _i, _i, _i, _p, _p, _p, _p],
-    "mxq_mx_grouped_linear": [_p, _i, _i64, _i64, _i64, _i, _i, _i, _p, _i, _p, _p, _i, _i64, _i64, _p, _i, _p, _p, _i, _p, _i, _i, _p, _i64, _p, _p],
+    "mxq_mx_pack_experts": [_p, _p, _i64, _i64, _i64, _i, _i, _i, _p, _p, _p],
+    "mxq_mx_grouped_linear": [_p, _i, _i64, _i64, _i64, _i, _i, _i, _p, _i, _p, _i, _i64, _i64, _p, _i, _p, _p, _i, _p, _i, _i, _p, _i64, _p, _p],
     "mxq_mx_max_groups": [],
     "mxq_dense_linear": [_p, _p, _i, _p, _p, _i64, _i64, _i64, _p, _p],
     "mxq_mxfp_weight_linear": [_p, _i, _p, _p, _i, _i, _p, _p, _i64, _i64, _i64, _p, _p],
@@ -50,7 +50,7 @@ SIGNATURES = {
     "mxq_version": [],
 }
 _I64_FUNCS = {"mxq_mx_sf_bytes": [_i64, _i64, _i, _i], "mxq_packed_bytes": [_i64, _i], "mxq_mx_linear_scratch_bytes": [_i64, _i64],
-              "mxq_mx_linear_static_capacity": [], "mxq_mx_grouped_scratch_bytes": [_p, _i, _i64, _i64, _i64, _i64]}
+              "mxq_mx_linear_static_capacity": [], "mxq_mx_packed_experts_bytes": [_i64, _i64, _i64, _i], "mxq_mx_grouped_scratch_bytes": [_p, _i, _i64, _i64, _i64, _i64]}
 _STRING_FUNCS = {"mxq_status_string": [_i], "mxq_last_cuda_error": []}
 
 _lib = None

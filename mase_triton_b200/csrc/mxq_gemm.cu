@@ -502,11 +502,6 @@ __global__ void __launch_bounds__(256) mx_pack_kernel(const uint8_t* __restrict_
     const int64_t kb_per_row = K / 32;
     const int64_t KT = (K + 127) / 128;
     const int64_t n_tiles = (rows + tile_rows - 1) / tile_rows;
-    // matrices one after the other (the weights of an expert layer), each with scale tiles of its own
-    if (scales != nullptr) scales += blockIdx.y * rows * kb_per_row;
-    elements += blockIdx.y * rows * K;
-    if (hw_codes != nullptr) hw_codes += blockIdx.y * rows * K;
-    hw_sf += blockIdx.y * n_tiles * KT * 1024;
     // one (tile, chunk-local row, K block) per thread, padding included: every byte of hw_sf is written
     const int64_t total = n_tiles * 256 * KT * 4;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -790,24 +785,6 @@ bool hw_code_tables(int eb, int fb, uint8_t (&plain)[256], uint8_t (&halved)[256
     return true;
 }
 }  // namespace mxq
-
-extern "C" int mxq_mx_pack_experts(const uint8_t* scales, const uint8_t* elements, int64_t groups, int64_t N, int64_t K, int eb, int fb,
-                                   int nibbles, uint8_t* hw_codes, uint8_t* hw_sf, int* hw_format, void* stream) {
-    if (groups <= 0 || N <= 0 || K <= 0 || K % 32 != 0 || !scales || !elements || !hw_codes || !hw_sf || !hw_format) return MXQ_EINVAL;
-    if (groups > MX_MAX_GROUPS) return MXQ_ESIZE;
-    if ((reinterpret_cast<uintptr_t>(elements) | reinterpret_cast<uintptr_t>(hw_codes)) % 16 != 0) return MXQ_EINVAL;
-    if (nibbles && (eb != 2 || fb != 1 || K % 256 != 0 || reinterpret_cast<uintptr_t>(hw_codes) % 32 != 0)) return MXQ_ESIZE;
-    gemm::PackTables t;
-    int fmt;
-    if (!gemm::build_pack_tables(eb, fb, &t, &fmt)) return MXQ_EINVAL;
-    const int64_t total = (N + 255) / 256 * 256 * ((K + 127) / 128 * 4);
-    const dim3 grid((unsigned)((total + 255) / 256), (unsigned)groups);
-    gemm::mx_pack_kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(scales, elements, nibbles ? nullptr : hw_codes, hw_sf, N, K, gemm::A_TILE_ROWS, t);
-    int rc = check_launch();
-    if (rc == MXQ_OK && nibbles) { fmt = gemm::HW_E2M1; rc = mxq_pack_codes(elements, hw_codes, groups * N * K, 4, stream); }
-    if (rc == MXQ_OK) *hw_format = fmt;
-    return rc;
-}
 
 static int mx_gemm_impl(const uint8_t* a_codes, const uint8_t* a_sf, int a_hw_format, const uint8_t* b_codes, const uint8_t* b_sf,
                         int b_hw_format, int b_tile_rows, void* out, int out_dtype, const tc::BiasRef& bias, int64_t M, int64_t N, int64_t K,

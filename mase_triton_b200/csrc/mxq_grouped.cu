@@ -16,8 +16,7 @@
 // Which rows belong to which group is read on the device: no size but the upper bounds is known to the host.
 //
 // Operand layout in HBM:
-//   weights: codes [groups * N, K] (bytes, or nibbles for E2M1 x E2M1), scales per group as for a left operand of mxq_gemm.cu
-//            ([ceil(N / 256)][ceil(K / 128)][2][512] bytes);
+//   weights: blocks of 128 features x one step of K, see WeightTile in mxq_grouped.cuh;
 //   rows:    codes [rows, K], scales [tile slot][ceil(K / 128)][chunks][512] bytes.  With tiles of at most `width` rows, tile t of a
 //            group that begins at row f has slot f / width + group + t: no two tiles share one, and no sum over the groups before is needed.
 #include "mxq_grouped.cuh"
@@ -36,10 +35,12 @@ template <int MH_, int BT_, int STAGES_, bool MXF4_> struct Cfg {
     static constexpr int FEATURES = 128 * MH;
     static constexpr int K_STEP = MXF4 ? 256 : 128;                 // elements of K per stage
     static constexpr int SF_STEPS = MXF4 ? 2 : 1;                   // 128-element steps of scales per stage
+    using Tile = WeightTile<MXF4>;
     static constexpr int W_BYTES = FEATURES * 128, X_BYTES = BT * 128;
     static constexpr int X_CHUNKS = BT > 128 ? 2 : 1;
-    static constexpr int SF_STEP_BYTES = (MH + X_CHUNKS) * 512;
-    static constexpr int STAGE_BYTES = W_BYTES + X_BYTES + SF_STEPS * SF_STEP_BYTES;
+    // a stage: weight codes | row codes | scales: [MH][SF_STEPS][512] of the weights, [SF_STEPS][X_CHUNKS][512] of the rows
+    static constexpr int SFW = W_BYTES + X_BYTES, SFX = SFW + MH * SF_STEPS * 512;
+    static constexpr int STAGE_BYTES = SFX + SF_STEPS * X_CHUNKS * 512;
     // Two accumulators of BT columns.  MH = 2: the two halves of one tile.  MH = 1: two tiles in turn, so that one is read
     // while the next is computed.  The scales take the columns behind them, two sets in turn.
     static constexpr int ACC_STRIDE = MH == 2 ? 256 : BT;
@@ -60,7 +61,7 @@ using NarrowFp4 = Cfg<1, 128, 5, true>;
 
 template <class C, int DT>
 __global__ void __launch_bounds__(THREADS, 1)
-grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x64, const __grid_constant__ CUtensorMap map_x16,
+grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constant__ CUtensorMap map_x16,
                const __grid_constant__ Params p) {
     constexpr int MH = C::MH, STAGES = C::STAGES;
     extern __shared__ uint8_t smem_raw[];
@@ -85,7 +86,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == 0 && elect_one()) { prefetch_map(map_w); prefetch_map(map_x16); prefetch_map(map_x64); }
+    if (warp == 0 && elect_one()) { prefetch_map(map_x16); prefetch_map(map_x64); }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -113,10 +114,9 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         uint32_t issued = 0;
         for (int u = blockIdx.x; u < walk.total && ok; u += gridDim.x) {
             const Unit t = walk.at(u, C::FEATURES);
-            const int halves = uniform(halves_of(t)), row = uniform(t.row), w_row = uniform(t.g * p.N + t.f0);
+            const int halves = uniform(halves_of(t)), row = uniform(t.row);
             const uint32_t n = uniform(t.padded());
-            const uint8_t* w_sf = p.w_sf + (size_t)uniform(t.g) * p.w_sf_group +
-                                  (MH == 2 ? (size_t)uniform(t.ftile) * KT128 * 1024 : (size_t)uniform(t.ftile >> 1) * KT128 * 1024 + uniform(t.ftile & 1) * 512);
+            const uint8_t* w = p.w + (size_t)uniform(t.g) * p.w_group + (size_t)uniform(t.ftile * MH) * KT * C::Tile::BYTES;
             const uint8_t* x_sf = p.x_sf + (size_t)uniform(t.begin / p.rows.width + t.g + t.tile) * KT128 * (C::X_CHUNKS * 512);
             const uint32_t x_chunks = n > 128 ? 2 : 1;
             for (int kt = 0; kt < KT; ++kt, ++issued, at.step()) {
@@ -125,12 +125,12 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                 const uint32_t st = ring + at.s * C::STAGE_BYTES, full = full_bar(at.s);
                 if (elect_one()) {
                     if (warp == 0) {
-                        mbar_expect_tx(full, (uint32_t)halves * (16384u + C::SF_STEPS * 512u));
-                        tma_load_2d(st, &map_w, kt * C::K_STEP, w_row, full);
-                        if (MH == 2 && halves == 2) tma_load_2d(st + 16384, &map_w, kt * C::K_STEP, w_row + 128, full);
-#pragma unroll
-                        for (int c = 0; c < C::SF_STEPS; ++c)
-                            bulk_load(st + C::W_BYTES + C::X_BYTES + c * C::SF_STEP_BYTES, w_sf + (size_t)(kt * C::SF_STEPS + c) * 1024, halves * 512, full);
+                        mbar_expect_tx(full, (uint32_t)halves * C::Tile::BYTES);
+                        for (int h = 0; h < halves; ++h) {
+                            const uint8_t* block = w + ((size_t)h * KT + kt) * C::Tile::BYTES;
+                            bulk_load(st + h * 16384, block, C::Tile::CODES, full);
+                            bulk_load(st + C::SFW + h * C::SF_STEPS * 512, block + C::Tile::CODES, C::SF_STEPS * 512, full);
+                        }
                     } else {
                         mbar_expect_tx(full, n * 128u + C::SF_STEPS * x_chunks * 512u);
                         uint32_t r = 0;
@@ -138,7 +138,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                         for (; r < n; r += 16) tma_load_2d(st + C::W_BYTES + r * 128, &map_x16, kt * C::K_STEP, row + r, full);
 #pragma unroll
                         for (int c = 0; c < C::SF_STEPS; ++c)
-                            bulk_load(st + C::W_BYTES + C::X_BYTES + c * C::SF_STEP_BYTES + MH * 512, x_sf + (size_t)(kt * C::SF_STEPS + c) * (C::X_CHUNKS * 512),
+                            bulk_load(st + C::SFX + c * C::X_CHUNKS * 512, x_sf + (size_t)(kt * C::SF_STEPS + c) * (C::X_CHUNKS * 512),
                                       x_chunks * 512u, full);
                     }
                 }
@@ -160,15 +160,15 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         int u = blockIdx.x;
         Unit next = u < walk.total ? walk.at(u, C::FEATURES) : Unit{};
         auto copy_scales = [&](int s, uint32_t into, int halves, uint32_t n) {
-            const uint32_t sf = ring + s * C::STAGE_BYTES + C::W_BYTES + C::X_BYTES, sfw = tmem + C::SFW_COL + into, sfx = tmem + C::SFX_COL + into;
+            const uint32_t from = ring + s * C::STAGE_BYTES, sfw = tmem + C::SFW_COL + into, sfx = tmem + C::SFX_COL + into;
             if (elect_one()) {
 #pragma unroll
                 for (int c = 0; c < C::SF_STEPS; ++c) {
-                    const uint32_t src = sf + c * C::SF_STEP_BYTES;
-                    tmem_cp_32x128b(sfw + 8 * c, smem_desc(src, 0, 128, LAYOUT_NONE));
-                    if (MH == 2 && halves == 2) tmem_cp_32x128b(sfw + 8 * c + 4, smem_desc(src + 512, 0, 128, LAYOUT_NONE));
-                    tmem_cp_32x128b(sfx + 8 * c, smem_desc(src + MH * 512, 0, 128, LAYOUT_NONE));
-                    if (C::X_CHUNKS == 2 && n > 128) tmem_cp_32x128b(sfx + 8 * c + 4, smem_desc(src + MH * 512 + 512, 0, 128, LAYOUT_NONE));
+                    const uint32_t w = from + C::SFW + c * 512, x = from + C::SFX + c * C::X_CHUNKS * 512;
+                    tmem_cp_32x128b(sfw + 8 * c, smem_desc(w, 0, 128, LAYOUT_NONE));
+                    if (MH == 2 && halves == 2) tmem_cp_32x128b(sfw + 8 * c + 4, smem_desc(w + C::SF_STEPS * 512, 0, 128, LAYOUT_NONE));
+                    tmem_cp_32x128b(sfx + 8 * c, smem_desc(x, 0, 128, LAYOUT_NONE));
+                    if (C::X_CHUNKS == 2 && n > 128) tmem_cp_32x128b(sfx + 8 * c + 4, smem_desc(x + 512, 0, 128, LAYOUT_NONE));
                 }
             }
             __syncwarp();
@@ -334,6 +334,53 @@ struct CodeTables {
     uint32_t bad[8];        // bit c: reference code c is one that the hardware reads as Inf / NaN
 };
 
+// One thread per feature and 32-element block of a group (blockIdx.y), those that only fill up the last tile and step included
+// (codes 0, scale 2^0).
+__global__ void __launch_bounds__(256) pack_weights_kernel(const uint8_t* __restrict__ scales, const uint8_t* __restrict__ elements, int64_t N, int64_t K,
+                                                           int nibbles, uint8_t* __restrict__ packed, const __grid_constant__ CodeTables t) {
+    __shared__ uint8_t s_plain[256], s_halved[256];
+    s_plain[threadIdx.x] = t.plain[threadIdx.x];
+    s_halved[threadIdx.x] = t.halved[threadIdx.x];
+    __syncthreads();
+    const int blocks_per_step = nibbles ? 8 : 4, tile_bytes = nibbles ? WeightTile<true>::BYTES : WeightTile<false>::BYTES;
+    const int64_t steps = nibbles ? WeightTile<true>::steps(K) : WeightTile<false>::steps(K), blocks = steps * blocks_per_step, features = (N + 127) / 128 * 128;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= features * blocks) return;
+    const int64_t f = i / blocks, kb = i - f * blocks;
+    const int r = (int)(f % 128), b = (int)(kb % blocks_per_step);
+    uint8_t* tile = packed + (blockIdx.y * (features / 128 * steps) + f / 128 * steps + kb / blocks_per_step) * tile_bytes;
+    uint4 c[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    uint32_t scale = 127u;
+    if (f < N && kb * 32 < K) {
+        const int64_t block = ((int64_t)blockIdx.y * N + f) * (K / 32) + kb;
+        const uint4* from = reinterpret_cast<const uint4*>(elements + block * 32);
+        c[0] = from[0];
+        c[1] = from[1];
+        scale = scales[block];
+    }
+    const uint8_t* cb = reinterpret_cast<const uint8_t*>(c);
+    uint8_t* row = tile + r * 128;
+    if (nibbles) {
+        uint32_t o[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int j = 0; j < 32; ++j) o[j >> 3] |= (uint32_t)(cb[j] & 0xFu) << (4 * (j & 7));
+        *reinterpret_cast<uint4*>(row + ((b ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+    } else {
+        bool any_bad = false;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) any_bad |= (t.bad[cb[j] >> 5] >> (cb[j] & 31)) & 1u;
+        const uint8_t* lut = any_bad ? s_halved : s_plain;
+        uint4 o[2];
+        uint8_t* ob = reinterpret_cast<uint8_t*>(o);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) ob[j] = lut[cb[j]];
+        *reinterpret_cast<uint4*>(row + (((2 * b) ^ (r & 7)) << 4)) = o[0];
+        *reinterpret_cast<uint4*>(row + (((2 * b + 1) ^ (r & 7)) << 4)) = o[1];
+        if (any_bad && scale < 255u) ++scale;
+    }
+    tile[WeightTile<false>::CODES + (b >> 2) * 512 + (r % 32) * 16 + (r / 32) * 4 + (b & 3)] = (uint8_t)scale;
+}
+
 // Operand of the product: codes, scale chunks, chunks per 128-element step.
 struct RowOperand {
     uint8_t *codes, *sf;
@@ -468,24 +515,23 @@ static int quantize_rows(const void* x, int x_dtype, const void* row_index, int 
 }
 
 template <class C, int DT>
-static int launch(const Params& p, const uint8_t* w_codes, const uint8_t* x_codes, cudaStream_t st) {
+static int launch(const Params& p, const uint8_t* x_codes, cudaStream_t st) {
     static bool attr_done[MAX_DEVICES] = {false};
     const cudaError_t e = raise_smem_limit(grouped_kernel<C, DT>, C::SMEM_BYTES, attr_done);
     if (e != cudaSuccess) { set_last_cuda_error(e); return MXQ_ELAUNCH; }
-    CUtensorMap mw, mx64, mx16;
+    CUtensorMap mx64, mx16;
     const Groups& g = p.rows;
-    if (!make_map(&mw, w_codes, (int64_t)g.groups * p.N, p.K, 128, C::MXF4) || !make_map(&mx64, x_codes, g.rows, p.K, 64, C::MXF4) ||
-        !make_map(&mx16, x_codes, g.rows, p.K, 16, C::MXF4)) return MXQ_ELAUNCH;
+    if (!make_map(&mx64, x_codes, g.rows, p.K, 64, C::MXF4) || !make_map(&mx16, x_codes, g.rows, p.K, 16, C::MXF4)) return MXQ_ELAUNCH;
     const int64_t units = most_units(g, p.N, C::FEATURES);
     const int grid = (int)(units < sm_count() ? units : sm_count());
-    return launch_after(grouped_kernel<C, DT>, (unsigned)grid, THREADS, C::SMEM_BYTES, st, mw, mx64, mx16, p);
+    return launch_after(grouped_kernel<C, DT>, (unsigned)grid, THREADS, C::SMEM_BYTES, st, mx64, mx16, p);
 }
 
 template <class C>
-static int launch_dt(Params& p, int dt, const uint8_t* w_codes, const uint8_t* x_codes, cudaStream_t st) {
-    if (dt == MXQ_F32) return launch<C, MXQ_F32>(p, w_codes, x_codes, st);
-    if (dt == MXQ_BF16) return launch<C, MXQ_BF16>(p, w_codes, x_codes, st);
-    return launch<C, MXQ_F16>(p, w_codes, x_codes, st);
+static int launch_dt(const Params& p, int dt, const uint8_t* x_codes, cudaStream_t st) {
+    if (dt == MXQ_F32) return launch<C, MXQ_F32>(p, x_codes, st);
+    if (dt == MXQ_BF16) return launch<C, MXQ_BF16>(p, x_codes, st);
+    return launch<C, MXQ_F16>(p, x_codes, st);
 }
 
 // element formats of the tensor-core path
@@ -514,6 +560,29 @@ using namespace mxq;
 
 extern "C" int mxq_mx_max_groups(void) { return grouped::MAX_GROUPS; }
 
+extern "C" int64_t mxq_mx_packed_experts_bytes(int64_t groups, int64_t N, int64_t K, int nibbles) {
+    if (groups <= 0 || N <= 0 || K <= 0 || K % 32 != 0) return MXQ_EINVAL;
+    return groups * (nibbles ? grouped::WeightTile<true>::group_bytes(N, K) : grouped::WeightTile<false>::group_bytes(N, K));
+}
+
+extern "C" int mxq_mx_pack_experts(const uint8_t* scales, const uint8_t* elements, int64_t groups, int64_t N, int64_t K, int eb, int fb, int nibbles,
+                                   uint8_t* packed, int* hw_format, void* stream) {
+    if (groups <= 0 || N <= 0 || K <= 0 || K % 32 != 0 || !scales || !elements || !packed || !hw_format) return MXQ_EINVAL;
+    if (groups > grouped::MAX_GROUPS || groups * N > (1ll << 31) - 1 || K > (1 << 30)) return MXQ_ESIZE;
+    if ((reinterpret_cast<uintptr_t>(elements) | reinterpret_cast<uintptr_t>(packed)) % 16 != 0) return MXQ_EINVAL;
+    if (nibbles && (eb != 2 || fb != 1 || K % 256 != 0)) return MXQ_ESIZE;
+    grouped::CodeTables t;
+    int fmt;
+    if (!hw_code_tables(eb, fb, t.plain, t.halved, t.bad, &fmt)) return MXQ_EINVAL;
+    const int64_t steps = nibbles ? grouped::WeightTile<true>::steps(K) * 8 : grouped::WeightTile<false>::steps(K) * 4;
+    const int64_t threads = (N + 127) / 128 * 128 * steps;
+    if ((threads + 255) / 256 > (1ll << 31) - 1) return MXQ_ESIZE;
+    grouped::pack_weights_kernel<<<dim3((unsigned)((threads + 255) / 256), (unsigned)groups), 256, 0, (cudaStream_t)stream>>>(scales, elements, N, K, nibbles, packed, t);
+    const int rc = check_launch();
+    if (rc == MXQ_OK) *hw_format = nibbles ? 5 : fmt;
+    return rc;
+}
+
 // the decode kernel quantises by itself: no operand in memory
 static bool takes_decode(const grouped::Plan& plan, const void* x, int round_mode) {
     return plan.decode && round_mode == MXQ_RN && reinterpret_cast<uintptr_t>(x) % 16 == 0;
@@ -527,8 +596,7 @@ extern "C" int64_t mxq_mx_grouped_scratch_bytes(const void* x, int round_mode, i
 }
 
 extern "C" int mxq_mx_grouped_linear(const void* x, int x_dtype, int64_t rows_in, int64_t rows, int64_t K, int x_exp_bits, int x_frac_bits,
-                                     int x_round_mode, const void* row_index, int index64, const uint8_t* w_codes, const uint8_t* w_sf,
-                                     int w_hw_format, int64_t groups, int64_t N, const void* offsets, int offsets64, void* out, const void* bias,
+                                     int x_round_mode, const void* row_index, int index64, const uint8_t* w_packed, int w_hw_format, int64_t groups, int64_t N, const void* offsets, int offsets64, void* out, const void* bias,
                                      int activation, const void* extra, int extra_mode, int zero_rest, void* scratch, int64_t scratch_bytes,
                                      int* status, void* stream) {
     if (rows < 0 || rows_in < 0 || groups <= 0 || N <= 0 || K <= 0 || K % 32 != 0) return MXQ_EINVAL;
@@ -539,23 +607,23 @@ extern "C" int mxq_mx_grouped_linear(const void* x, int x_dtype, int64_t rows_in
     if (groups > grouped::MAX_GROUPS || rows > (1 << 30) || N > (1 << 30) || K > (1 << 30) || groups * N > (1ll << 31) - 1) return MXQ_ESIZE;
     if (rows * ((K + 127) / 128 * 4) > (1ll << 31) * 255 || rows_in > (1 << 30)) return MXQ_ESIZE;
     if (rows == 0) return MXQ_OK;
-    if ((!x && rows_in > 0) || !w_codes || !w_sf || !out || (extra_mode != MXQ_EXTRA_NONE && !extra)) return MXQ_EINVAL;
-    if ((reinterpret_cast<uintptr_t>(w_codes) | reinterpret_cast<uintptr_t>(w_sf)) % 16 != 0 || reinterpret_cast<uintptr_t>(scratch) % 256 != 0) return MXQ_EINVAL;
+    if ((!x && rows_in > 0) || !w_packed || !out || (extra_mode != MXQ_EXTRA_NONE && !extra)) return MXQ_EINVAL;
+    if (reinterpret_cast<uintptr_t>(w_packed) % 16 != 0 || reinterpret_cast<uintptr_t>(scratch) % 256 != 0) return MXQ_EINVAL;
     const int64_t needed = mxq_mx_grouped_scratch_bytes(x, x_round_mode, rows_in, rows, K, groups);
     if (needed > 0 && !scratch) return MXQ_EINVAL;
     if (scratch_bytes < needed) return MXQ_ESIZE;
     // both operands E2M1 and the weight kept as nibbles: the 4-bit kind
     const bool x_e2m1 = x_exp_bits == 2 && x_frac_bits == 1;
     const bool fp4 = w_hw_format == 5;
-    if (fp4 && (!x_e2m1 || K % 256 != 0 || reinterpret_cast<uintptr_t>(w_codes) % 32 != 0)) return MXQ_EINVAL;
+    if (fp4 && (!x_e2m1 || K % 256 != 0)) return MXQ_EINVAL;
     if (!fp4 && w_hw_format != 0 && w_hw_format != 1) return MXQ_EINVAL;
     if (!grouped::valid_mx_preset(x_exp_bits, x_frac_bits) || x_round_mode < MXQ_RN || x_round_mode > MXQ_RZ) return MXQ_EINVAL;
     const int x_fmt = x_exp_bits == 5 ? 1 : 0;
 
     const grouped::Plan plan = grouped::make_plan(rows, groups, fp4);
     grouped::Params p{};
-    p.w_sf = w_sf;
-    p.w_sf_group = mxq_mx_sf_bytes(N, K, MXQ_OPERAND_A, 0);
+    p.w = w_packed;
+    p.w_group = fp4 ? grouped::WeightTile<true>::group_bytes(N, K) : grouped::WeightTile<false>::group_bytes(N, K);
     p.out = out; p.bias = bias; p.extra = extra;
     p.rows = grouped::Groups{offsets, offsets64, (int)rows, (int)groups, plan.width};
     p.N = (int)N; p.K = (int)K;
@@ -567,7 +635,7 @@ extern "C" int mxq_mx_grouped_linear(const void* x, int x_dtype, int64_t rows_in
     cudaStream_t st = (cudaStream_t)stream;
     if (takes_decode(plan, x, x_round_mode)) {
         p.rows.width = grouped::decode_rows();
-        return grouped::launch_decode(p, x_dtype, x, row_index, index64, rows_in, x_exp_bits, x_frac_bits, fp4, w_codes, st);
+        return grouped::launch_decode(p, x_dtype, x, row_index, index64, rows_in, x_exp_bits, x_frac_bits, fp4, st);
     }
 
     uint8_t* codes = static_cast<uint8_t*>(scratch);
@@ -590,6 +658,6 @@ extern "C" int mxq_mx_grouped_linear(const void* x, int x_dtype, int64_t rows_in
         rc = check_launch();
     }
     if (rc != MXQ_OK) return rc;
-    if (fp4) return plan.narrow ? grouped::launch_dt<grouped::NarrowFp4>(p, x_dtype, w_codes, codes, st) : grouped::launch_dt<grouped::WideFp4>(p, x_dtype, w_codes, codes, st);
-    return plan.narrow ? grouped::launch_dt<grouped::Narrow>(p, x_dtype, w_codes, codes, st) : grouped::launch_dt<grouped::Wide>(p, x_dtype, w_codes, codes, st);
+    if (fp4) return plan.narrow ? grouped::launch_dt<grouped::NarrowFp4>(p, x_dtype, codes, st) : grouped::launch_dt<grouped::WideFp4>(p, x_dtype, codes, st);
+    return plan.narrow ? grouped::launch_dt<grouped::Narrow>(p, x_dtype, codes, st) : grouped::launch_dt<grouped::Wide>(p, x_dtype, codes, st);
 }

@@ -12,6 +12,17 @@ using namespace tc;
 constexpr int MAX_GROUPS = MX_MAX_GROUPS;
 enum : int { X_NONE = MXQ_EXTRA_NONE, X_MUL = MXQ_EXTRA_MULTIPLY, X_ADD = MXQ_EXTRA_ADD };
 
+// Packed weights: 128 features x one step of K (128 bytes of codes per feature: 128 elements, 256 of E2M1 pairs) are one contiguous
+// block, the codes as the 128-byte-swizzled image that the tensor cores read in shared memory, their scale chunks behind
+// them.  [group][ceil(N / 128)][steps of K] blocks: a CTA reads a sequential stream with plain bulk copies.  (Codes in rows, fetched in boxes
+// of 128 rows x 128 bytes, cost a DRAM page per line: see the measurements in mxq_grouped_decode.cu.)
+template <bool MXF4> struct WeightTile {
+    static constexpr int K_STEP = MXF4 ? 256 : 128, SF_STEPS = MXF4 ? 2 : 1;
+    static constexpr int CODES = 16384, BYTES = CODES + SF_STEPS * 512;
+    static __host__ __device__ int64_t steps(int64_t K) { return (K + K_STEP - 1) / K_STEP; }
+    static __host__ __device__ int64_t group_bytes(int64_t N, int64_t K) { return (N + 127) / 128 * steps(K) * BYTES; }
+};
+
 template <int DT> struct Elem;
 template <> struct Elem<MXQ_F32> { typedef float T; };
 template <> struct Elem<MXQ_BF16> { typedef __nv_bfloat16 T; };
@@ -370,8 +381,8 @@ __device__ __forceinline__ Place find_row(const Groups& g, int row, int* s_two) 
 }
 
 struct Params {
-    const uint8_t* w_sf;         // weight scales, w_sf_group bytes per group
-    int64_t w_sf_group;
+    const uint8_t* w;            // packed weights (WeightTile blocks)
+    int64_t w_group;             // bytes per group
     const uint8_t* x_sf;         // row scales
     void* out;
     const void* bias;            // [groups, N] or null
@@ -393,7 +404,7 @@ static int64_t most_units(const Groups& g, int64_t N, int features) {
 // mxq_grouped_decode.cu: rows that fit tiles of decode_rows(); x on 16 bytes, a built-in round-to-nearest format
 int decode_rows();
 int launch_decode(const Params& p, int dt, const void* x, const void* row_index, int index64, int64_t rows_in, int eb, int fb, bool nibbles,
-                  const uint8_t* w_codes, cudaStream_t st);
+                  cudaStream_t st);
 
 template <class... KArgs, class... Args>
 static int launch_after(void (*kernel)(KArgs...), unsigned grid, unsigned block, unsigned smem, cudaStream_t st, Args... args) {

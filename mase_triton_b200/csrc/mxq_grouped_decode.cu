@@ -22,17 +22,20 @@ constexpr int ROWS = 16;                         // widest row tile: the narrowe
 constexpr int FEATURES = 128;
 constexpr int EPI_WARP = 4;
 constexpr int THREADS = 352;                     // warps 0, 1: weight copies, MMA issuer; 4..7: epilogue; 2, 3, 8..10: quantisers
-constexpr int W_BYTES = FEATURES * 128, X_BYTES = ROWS * 128;
+constexpr int X_BYTES = ROWS * 128;
 constexpr int TMEM_COLS = 128;
 constexpr int ACC_STRIDE = 32, SFW_COL = 64, SFX_COL = 96;
 
 template <bool MXF4> struct Cfg {
-    static constexpr int K_STEP = MXF4 ? 256 : 128, SF_STEPS = MXF4 ? 2 : 1;
+    using Tile = WeightTile<MXF4>;
+    static constexpr int K_STEP = Tile::K_STEP, SF_STEPS = Tile::SF_STEPS;
     static constexpr int STAGES = MXF4 ? 4 : 5;
     // a warp that took a stage more than one turn of the ring ahead would mistake the phase its barrier is in
     static constexpr int QUANT_WARPS = STAGES;
     static_assert(QUANT_WARPS <= STAGES && EPI_WARP + 2 + QUANT_WARPS <= THREADS / 32, "quantising warps");
-    static constexpr int STAGE_BYTES = W_BYTES + X_BYTES + SF_STEPS * 1024;          // scales: 512 bytes of either operand per 128 elements of K
+    // a stage: row codes | a block of the weights, its scales behind its codes | scales of the rows, 512 bytes per 128 elements of K
+    static constexpr int W = X_BYTES, SFW = W + Tile::CODES, SFX = W + Tile::BYTES;
+    static constexpr int STAGE_BYTES = SFX + SF_STEPS * 512;
     static constexpr int SLOTS = 4 * 2048, EXCHANGE = 3 * 2048;                      // 32 features x 16 rows per epilogue warp, and per part received
     static constexpr int FIXED_BYTES = 1024 + STAGES * STAGE_BYTES + 256 + SLOTS + EXCHANGE;
     static int smem_bytes(int groups) { return FIXED_BYTES + 2 * (groups + 1) * 4; }  // the group table comes last
@@ -75,7 +78,7 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity,
 // DT: type of x, out, bias and extra; F, OUT: element format of the rows and what the tensor cores read of it
 template <int DT, class F, int OUT>
 __global__ void __launch_bounds__(THREADS, 2)
-decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ Params p, const __grid_constant__ Source src, int split) {
+decode_kernel(const __grid_constant__ Params p, const __grid_constant__ Source src, int split) {
     constexpr bool MXF4 = OUT == 5;
     using C = Cfg<MXF4>;
     constexpr int STAGES = C::STAGES;
@@ -109,7 +112,6 @@ decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == 0 && elect_one()) prefetch_map(map_w);
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -124,7 +126,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(~0u, *tmem_slot, 0);
 
-    const int KT_all = (p.K + C::K_STEP - 1) / C::K_STEP, KT128 = (p.K + 127) / 128;
+    const int KT_all = (p.K + C::K_STEP - 1) / C::K_STEP;
     const int k_begin = rank * KT_all / split, KT = (rank + 1) * KT_all / split - k_begin;     // this CTA's steps of K, one at least
     const int ftiles = (p.N + FEATURES - 1) / FEATURES;
     const int u_begin = blockIdx.x / split, u_step = gridDim.x / split;
@@ -137,8 +139,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         uint32_t issued = 0;
         for (int u = u_begin; u < walk.total && ok; u += u_step) {
             const Unit t = walk.at(u, FEATURES);
-            const uint8_t* sf = p.w_sf + (size_t)uniform(t.g) * p.w_sf_group + (size_t)uniform(t.ftile >> 1) * KT128 * 1024 + uniform(t.ftile & 1) * 512;
-            const int w_row = uniform(t.g * p.N + t.f0);
+            const uint8_t* w = p.w + (size_t)uniform(t.g) * p.w_group + (size_t)uniform(t.ftile) * KT_all * C::Tile::BYTES;
             for (int kt = k_begin; kt < k_begin + KT; ++kt, ++issued, at.step()) {
                 ok = mbar_wait(empty_bar(at.s), at.phase ^ 1u, p.status, ST_PRODUCER_TIMEOUT);      // (a fresh barrier's phase before counts as complete)
                 if (!ok) break;
@@ -148,11 +149,8 @@ decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
                 if (issued == 0) dependency_wait();
                 if (issued == 1) mbar_wait(rows_bar, 0, p.status, ST_PRODUCER_TIMEOUT);
                 if (elect_one()) {
-                    mbar_expect_tx(full, W_BYTES + C::SF_STEPS * 512u);
-                    tma_load_2d(st, &map_w, kt * C::K_STEP, w_row, full);
-#pragma unroll
-                    for (int c = 0; c < C::SF_STEPS; ++c)
-                        bulk_load(st + W_BYTES + X_BYTES + c * 1024, sf + (size_t)(kt * C::SF_STEPS + c) * 1024, 512, full);
+                    mbar_expect_tx(full, C::Tile::BYTES);
+                    bulk_load(st + C::W, w + (size_t)kt * C::Tile::BYTES, C::Tile::BYTES, full);
                 }
                 __syncwarp();
             }
@@ -168,12 +166,12 @@ decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         constexpr uint32_t SF_COLS = C::SF_STEPS * 8;
         const uint32_t idesc = p.idesc | ((uint32_t)(ROWS >> 3) << 17);
         auto copy_scales = [&](int s, uint32_t into) {
-            const uint32_t sf = ring + s * C::STAGE_BYTES + W_BYTES + X_BYTES, sfw = tmem + SFW_COL + into, sfx = tmem + SFX_COL + into;
+            const uint32_t from = ring + s * C::STAGE_BYTES, sfw = tmem + SFW_COL + into, sfx = tmem + SFX_COL + into;
             if (elect_one()) {
 #pragma unroll
                 for (int c = 0; c < C::SF_STEPS; ++c) {
-                    tmem_cp_32x128b(sfw + 8 * c, smem_desc(sf + c * 1024, 0, 128, LAYOUT_NONE));
-                    tmem_cp_32x128b(sfx + 8 * c, smem_desc(sf + c * 1024 + 512, 0, 128, LAYOUT_NONE));
+                    tmem_cp_32x128b(sfw + 8 * c, smem_desc(from + C::SFW + c * 512, 0, 128, LAYOUT_NONE));
+                    tmem_cp_32x128b(sfx + 8 * c, smem_desc(from + C::SFX + c * 512, 0, 128, LAYOUT_NONE));
                 }
             }
             __syncwarp();
@@ -199,7 +197,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
                     copy_scales(at.s, set ^ SF_COLS);
                     copied = true;
                 }
-                const uint64_t w_desc = smem_desc(st, 16, 1024, LAYOUT_SW128), x_desc = smem_desc(st + W_BYTES, 16, 1024, LAYOUT_SW128);
+                const uint64_t w_desc = smem_desc(st + C::W, 16, 1024, LAYOUT_SW128), x_desc = smem_desc(st, 16, 1024, LAYOUT_SW128);
                 const uint32_t sfw = tmem + SFW_COL + set, sfx = tmem + SFX_COL + set;
                 if (elect_one()) {
 #pragma unroll
@@ -293,11 +291,11 @@ decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
                     if (r < rows) {
                         // 8 of the row's 128 bytes: 16-byte unit j lies at j ^ (r % 8)
                         const uint32_t j = (lane & 15) >> 1;
-                        *reinterpret_cast<uint2*>(st + W_BYTES + r * 128 + ((j ^ (r & 7)) << 4) + (lane & 1) * 8) = make_uint2(codes[0], codes[1]);
+                        *reinterpret_cast<uint2*>(st + r * 128 + ((j ^ (r & 7)) << 4) + (lane & 1) * 8) = make_uint2(codes[0], codes[1]);
                         if (lane % (32 / E) == 0) {
                             // scale of row r and block b at r * 16 + b; blocks behind K are 2^0 (their codes are zero)
                             const int blk = kl / 32;
-                            st[W_BYTES + X_BYTES + (blk >> 2) * 1024 + 512 + r * 16 + (blk & 3)] = (uint8_t)(k < p.K ? sbyte : 127u);
+                            st[C::SFX + (blk >> 2) * 512 + r * 16 + (blk & 3)] = (uint8_t)(k < p.K ? sbyte : 127u);
                         }
                     }
                 }
@@ -402,13 +400,11 @@ decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
 }
 
 template <int DT, class F, int OUT>
-static int launch(const Params& p, const Source& src, const uint8_t* w_codes, int split, cudaStream_t st) {
+static int launch(const Params& p, const Source& src, int split, cudaStream_t st) {
     using C = Cfg<OUT == 5>;
     static bool attr_done[MAX_DEVICES] = {false};
     cudaError_t e = raise_smem_limit(decode_kernel<DT, F, OUT>, C::smem_bytes(MAX_GROUPS), attr_done);
     if (e != cudaSuccess) { set_last_cuda_error(e); return MXQ_ELAUNCH; }
-    CUtensorMap mw;
-    if (!make_map(&mw, w_codes, (int64_t)p.rows.groups * p.N, p.K, FEATURES, OUT == 5)) return MXQ_ELAUNCH;
     const int64_t units = most_units(p.rows, p.N, FEATURES), room = 2 * sm_count();
     cudaLaunchConfig_t cfg = {};
     // a cluster works on one unit; without clusters the CTAs stay and walk over theirs
@@ -424,7 +420,7 @@ static int launch(const Params& p, const Source& src, const uint8_t* w_codes, in
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = split > 1 ? 2 : 1;
-    e = cudaLaunchKernelEx(&cfg, decode_kernel<DT, F, OUT>, mw, p, src, split);
+    e = cudaLaunchKernelEx(&cfg, decode_kernel<DT, F, OUT>, p, src, split);
     if (e != cudaSuccess) { set_last_cuda_error(e); return MXQ_ELAUNCH; }
     return check_launch();
 }
@@ -434,7 +430,7 @@ static int launch(const Params& p, const Source& src, const uint8_t* w_codes, in
 int decode_rows() { return decode::ROWS; }
 
 int launch_decode(const Params& p, int dt, const void* x, const void* row_index, int index64, int64_t rows_in, int eb, int fb, bool nibbles,
-                  const uint8_t* w_codes, cudaStream_t st) {
+                  cudaStream_t st) {
     // CTAs that share a unit: as many as the SMs hold (two each), the steps of K allow, and 4 at most (a lane quadrant each)
     const int64_t units = most_units(p.rows, p.N, decode::FEATURES);
     const int steps = (p.K + (nibbles ? 255 : 127)) / (nibbles ? 256 : 128);
@@ -445,9 +441,9 @@ int launch_decode(const Params& p, int dt, const void* x, const void* row_index,
     with_row_format(eb, fb, nibbles, [&](auto fmt, auto out) {
         using F = decltype(fmt);
         constexpr int OUT = decltype(out)::value;
-        if (dt == MXQ_F32) rc = decode::launch<MXQ_F32, F, OUT>(p, src, w_codes, split, st);
-        else if (dt == MXQ_BF16) rc = decode::launch<MXQ_BF16, F, OUT>(p, src, w_codes, split, st);
-        else rc = decode::launch<MXQ_F16, F, OUT>(p, src, w_codes, split, st);
+        if (dt == MXQ_F32) rc = decode::launch<MXQ_F32, F, OUT>(p, src, split, st);
+        else if (dt == MXQ_BF16) rc = decode::launch<MXQ_BF16, F, OUT>(p, src, split, st);
+        else rc = decode::launch<MXQ_F16, F, OUT>(p, src, split, st);
     });
     return rc;
 }

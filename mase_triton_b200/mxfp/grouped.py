@@ -20,18 +20,17 @@ _INDEX_DTYPES = (torch.int32, torch.int64)
 
 @dataclass
 class PackedExperts:
-    """Weights ``[groups, N, K]`` as the kernel reads them: hardware codes (bytes, or nibbles when ``hw_format`` is 5)
-    and scale chunks of every group."""
+    """Weights ``[groups, N, K]`` as the kernels read them: blocks of 128 features and 128 elements of K (256 for packed
+    4-bit codes, ``hw_format`` 5), the codes of a block and its scales one after the other."""
 
-    codes: Tensor
-    sf: Tensor
+    blocks: Tensor
     hw_format: int
     groups: int
     N: int
     K: int
 
     def __post_init__(self):
-        self.device_index, self.codes_ptr, self.sf_ptr = self.codes.get_device(), self.codes.data_ptr(), self.sf.data_ptr()
+        self.device_index, self.pointer = self.blocks.get_device(), self.blocks.data_ptr()
 
 
 def check_formats(x_meta: MXFPMeta | None, w_meta: MXFPMeta | None, K: int) -> None:
@@ -60,14 +59,13 @@ def pack_experts(w_scales: Tensor, w_elements: Tensor, groups: int, N: int, K: i
     w_scales, w_elements = w_scales.contiguous(), w_elements.contiguous()
     if w_elements.data_ptr() % 16 != 0:
         w_elements = w_elements.clone()
-    codes = torch.empty((groups, N, K // 2 if nibbles else K), dtype=torch.uint8, device=dev)
-    sf = torch.empty((groups * L.mxq_mx_sf_bytes(N, K, 0, 0),), dtype=torch.uint8, device=dev)
+    blocks = torch.empty(L.mxq_mx_packed_experts_bytes(groups, N, K, int(nibbles)), dtype=torch.uint8, device=dev)
     fmt = ctypes.c_int(0)
     with torch.cuda.device(dev):
         rc = L.mxq_mx_pack_experts(w_scales.data_ptr(), w_elements.data_ptr(), groups, N, K, w_meta.element_exp_bits, w_meta.element_frac_bits,
-                                   int(nibbles), codes.data_ptr(), sf.data_ptr(), ctypes.addressof(fmt), _lib.stream_ptr(dev))
+                                   int(nibbles), blocks.data_ptr(), ctypes.addressof(fmt), _lib.stream_ptr(dev))
     _lib.check(rc, "mxq_mx_pack_experts")
-    return PackedExperts(codes, sf, fmt.value, groups, N, K)
+    return PackedExperts(blocks, fmt.value, groups, N, K)
 
 
 def epilogue_operand(multiplier: Tensor | None, residual: Tensor | None) -> tuple[Tensor | None, int]:
@@ -120,7 +118,7 @@ def grouped_linear(x: Tensor, x_meta: MXFPMeta, w: PackedExperts, offsets: Tenso
     if not supported(x_meta) or (w.hw_format == 5 and not is_e2m1(x_meta)):
         raise ValueError(f"the weight was packed for another activation format than {x_meta}")
     if w.device_index != dev:
-        raise ValueError(f"the weight is on {w.codes.device}, the input on {x.device}")
+        raise ValueError(f"the weight is on {w.blocks.device}, the input on {x.device}")
     x = x.contiguous()
     tokens = rows = x.shape[0]
     offsets_ptr = index_ptr = bias_ptr = extra_ptr = None
@@ -167,8 +165,8 @@ def grouped_linear(x: Tensor, x_meta: MXFPMeta, w: PackedExperts, offsets: Tenso
     nbytes = L.mxq_mx_grouped_scratch_bytes(x_ptr, round_id, tokens, rows, K, groups)
     # of this call alone: two captured graphs, or two streams, never share it
     scratch = None if nbytes == 0 else torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-    args = (x_ptr, dtype_id, tokens, rows, K, x_meta.element_exp_bits, x_meta.element_frac_bits, round_id, index_ptr, index64, w.codes_ptr, w.sf_ptr, w.hw_format,
-            groups, N, offsets_ptr, offsets64, out.data_ptr(), bias_ptr, act, extra_ptr, extra_mode, zero_rest,
+    args = (x_ptr, dtype_id, tokens, rows, K, x_meta.element_exp_bits, x_meta.element_frac_bits, round_id, index_ptr, index64, w.pointer, w.hw_format, groups,
+            N, offsets_ptr, offsets64, out.data_ptr(), bias_ptr, act, extra_ptr, extra_mode, zero_rest,
             None if scratch is None else scratch.data_ptr(), nbytes, status, _lib.raw_stream(dev))
     if torch.cuda.current_device() == dev:
         rc = L.mxq_mx_grouped_linear(*args)

@@ -122,10 +122,10 @@ def fake(*shape, dtype=torch.bfloat16):
     (dict(out=torch.zeros(N, 2, dtype=torch.bfloat16).t()), "contiguous"),
     (dict(row_index=torch.zeros(5, dtype=torch.int32), out=torch.zeros(2, N, dtype=torch.bfloat16)), "out"),
     (dict(x_meta=MXFPMeta(16, 8, 4, 3, True, "rn")), "format"),
-    (dict(w=GR.PackedExperts(torch.zeros(1), torch.zeros(1), 5, E, N, K)), "format"),
+    (dict(w=GR.PackedExperts(torch.zeros(1), 5, E, N, K)), "format"),
 ])
 def test_grouped_refusals(change, match):
-    w = GR.PackedExperts(torch.zeros(1, dtype=torch.uint8), torch.zeros(1, dtype=torch.uint8), 0, E, N, K)
+    w = GR.PackedExperts(torch.zeros(1, dtype=torch.uint8), 0, E, N, K)
     call = dict(x=fake(2, K), x_meta=MXFP8_E4M3_fn, w=w, offsets=torch.zeros(E + 1, dtype=torch.int32)) | change
     with pytest.raises(ValueError, match=match):
         GR.grouped_linear(**call)
@@ -146,11 +146,11 @@ def test_c_entry_refuses_before_it_launches():
     L = _lib.load()
     buf = torch.zeros(1 << 16, dtype=torch.uint8)
     p = (buf.data_ptr() + 255) // 256 * 256
-    good = dict(x=p, x_dtype=1, rows_in=2, rows=2, K=64, eb=4, fb=3, rm=0, row_index=None, index64=0, w_codes=p, w_sf=p, fmt=0, groups=1, N=8, offsets=None,
+    good = dict(x=p, x_dtype=1, rows_in=2, rows=2, K=64, eb=4, fb=3, rm=0, row_index=None, index64=0, w=p, fmt=0, groups=1, N=8, offsets=None,
                 offsets64=0, out=p, bias=None, act=0, extra=None, mode=0, zero=0, scratch=p, nbytes=1 << 16, status=None, stream=None)
     assert L.mxq_mx_grouped_linear(*(good | dict(rows=0, rows_in=0)).values()) == 0
     for bad in (dict(K=48), dict(K=0), dict(N=0), dict(groups=0), dict(groups=2), dict(rows=3), dict(rows=-1), dict(x_dtype=3), dict(act=5), dict(act=-1), dict(mode=3),
-                dict(mode=1), dict(x=None), dict(w_codes=None), dict(w_sf=p + 8), dict(out=None), dict(scratch=None, rm=1), dict(scratch=p + 16), dict(fmt=3), dict(fmt=5),
+                dict(mode=1), dict(x=None), dict(w=None), dict(w=p + 8), dict(out=None), dict(scratch=None, rm=1), dict(scratch=p + 16), dict(fmt=3), dict(fmt=5),
                 dict(eb=3, fb=3)):
         assert L.mxq_mx_grouped_linear(*(good | bad).values()) == -1, bad
     for bad in (dict(groups=L.mxq_mx_max_groups() + 1, offsets=p), dict(nbytes=64, rm=1), dict(rows=1 << 31, rows_in=1 << 31)):
