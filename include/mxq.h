@@ -379,7 +379,8 @@ int mxq_mx_max_groups(void);
  * `extra` may be the same buffer as `out`.  K % 32 == 0, w_packed / w_hw_format from mxq_mx_pack_experts.
  * `status` as for mxq_mx_gemm.
  */
-int64_t mxq_mx_grouped_scratch_bytes(const void* x, int x_round_mode, int64_t rows_in, int64_t rows, int64_t K, int64_t groups);
+int64_t mxq_mx_grouped_scratch_bytes(const void* x, int x_round_mode, int64_t rows_in, int64_t rows, int64_t K,
+                                     int64_t groups, int64_t N);
 int mxq_mx_grouped_linear(const void* x, int x_dtype, int64_t rows_in, int64_t rows, int64_t K, int x_exp_bits,
                           int x_frac_bits, int x_round_mode, const void* row_index, int index64,
                           const uint8_t* w_packed, int w_hw_format, int64_t groups, int64_t N, const void* offsets,

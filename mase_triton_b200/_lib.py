@@ -50,7 +50,7 @@ SIGNATURES = {
     "mxq_version": [],
 }
 _I64_FUNCS = {"mxq_mx_sf_bytes": [_i64, _i64, _i, _i], "mxq_packed_bytes": [_i64, _i], "mxq_mx_linear_scratch_bytes": [_i64, _i64],
-              "mxq_mx_linear_static_capacity": [], "mxq_mx_packed_experts_bytes": [_i64, _i64, _i64, _i], "mxq_mx_grouped_scratch_bytes": [_p, _i, _i64, _i64, _i64, _i64]}
+              "mxq_mx_linear_static_capacity": [], "mxq_mx_packed_experts_bytes": [_i64, _i64, _i64, _i], "mxq_mx_grouped_scratch_bytes": [_p, _i, _i64, _i64, _i64, _i64, _i64]}
 _STRING_FUNCS = {"mxq_status_string": [_i], "mxq_last_cuda_error": []}
 
 _lib = None

@@ -19,6 +19,8 @@
 //   weights: blocks of 128 features x one step of K, see WeightTile in mxq_grouped.cuh;
 //   rows:    codes [rows, K], scales [tile slot][ceil(K / 128)][chunks][512] bytes.  With tiles of at most `width` rows, tile t of a
 //            group that begins at row f has slot f / width + group + t: no two tiles share one, and no sum over the groups before is needed.
+#include <algorithm>
+
 #include "mxq_grouped.cuh"
 
 namespace mxq {
@@ -28,42 +30,38 @@ constexpr int EPI_WARPS = 8;                     // two per TMEM lane quadrant
 constexpr int FIRST_EPI_WARP = 4;                // warps 0, 1, 3: weight copies, MMA issuer, row copies
 constexpr int THREADS = (FIRST_EPI_WARP + EPI_WARPS) * 32;
 
-// MH: 128-feature halves of a tile; BT: widest row tile; MXF4: both operands packed E2M1 nibbles (256 elements of K per 128 bytes)
-template <int MH_, int BT_, int STAGES_, bool MXF4_> struct Cfg {
-    static constexpr int MH = MH_, BT = BT_, STAGES = STAGES_;
+// A tile is 128 features x at most BT rows; MXF4: both operands packed E2M1 nibbles (256 elements of K per 128 bytes).
+template <int BT_, int STAGES_, bool MXF4_> struct Cfg {
+    static constexpr int BT = BT_, STAGES = STAGES_;
     static constexpr bool MXF4 = MXF4_;
-    static constexpr int FEATURES = 128 * MH;
-    static constexpr int K_STEP = MXF4 ? 256 : 128;                 // elements of K per stage
-    static constexpr int SF_STEPS = MXF4 ? 2 : 1;                   // 128-element steps of scales per stage
+    static constexpr int FEATURES = 128;
     using Tile = WeightTile<MXF4>;
-    static constexpr int W_BYTES = FEATURES * 128, X_BYTES = BT * 128;
-    static constexpr int X_CHUNKS = BT > 128 ? 2 : 1;
-    // a stage: weight codes | row codes | scales: [MH][SF_STEPS][512] of the weights, [SF_STEPS][X_CHUNKS][512] of the rows
-    static constexpr int SFW = W_BYTES + X_BYTES, SFX = SFW + MH * SF_STEPS * 512;
-    static constexpr int STAGE_BYTES = SFX + SF_STEPS * X_CHUNKS * 512;
-    // Two accumulators of BT columns.  MH = 2: the two halves of one tile.  MH = 1: two tiles in turn, so that one is read
-    // while the next is computed.  The scales take the columns behind them, two sets in turn.
-    static constexpr int ACC_STRIDE = MH == 2 ? 256 : BT;
-    static constexpr int SF_SETS = 2, SF_COLS = SF_STEPS * 8;
-    static constexpr int SFW_COL = MH == 2 ? BT : 2 * ACC_STRIDE, SFX_COL = MH == 2 ? ACC_STRIDE + BT : SFW_COL + SF_SETS * SF_COLS;
-    static_assert(MH == 1 || BT + SF_SETS * SF_COLS <= ACC_STRIDE, "tensor memory");
-    static_assert(SFX_COL + SF_SETS * SF_COLS <= 512, "tensor memory");
-    static_assert(STAGE_BYTES % 1024 == 0, "the 128-byte swizzle repeats every 1024 bytes");
+    static constexpr int K_STEP = Tile::K_STEP, SF_STEPS = Tile::SF_STEPS;          // elements of K and 128-element steps of scales per stage
+    static constexpr int X_BYTES = BT * 128, X_CHUNKS = BT > 128 ? 2 : 1;
+    // a stage: weight codes | row codes | scales: [SF_STEPS][512] of the weights, [SF_STEPS][X_CHUNKS][512] of the rows
+    static constexpr int X = Tile::CODES, SFW = X + X_BYTES, SFX = SFW + SF_STEPS * 512;
+    static constexpr int STAGE_BYTES = (SFX + SF_STEPS * X_CHUNKS * 512 + 1023) / 1024 * 1024;      // the 128-byte swizzle repeats every 1024 bytes
+    // Two accumulators of BT columns, tiles in turn: one is read while the next is computed.  Behind them two sets of scale columns.
+    static constexpr int ACC_STRIDE = BT > 128 ? 256 : BT;
+    static constexpr int SF_COLS = SF_STEPS * 8;
+    static constexpr int SFW_COL = BT > 128 ? BT : 2 * ACC_STRIDE, SFX_COL = BT > 128 ? ACC_STRIDE + BT : SFW_COL + 2 * SF_COLS;
+    static_assert(BT <= 128 || BT + 2 * SF_COLS <= ACC_STRIDE, "tensor memory");
+    static_assert(SFX_COL + 2 * SF_COLS <= 512, "tensor memory");
     // behind the ring: barriers, the group table, the epilogue's 2 KiB per warp
     static constexpr int TABLE_END = (256 + 2 * (MAX_GROUPS + 1) * 4 + 15) / 16 * 16;
     static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + TABLE_END + EPI_WARPS * 2048;
     static_assert(SMEM_BYTES <= 232448, "more shared memory than a CTA can have");
 };
-using Wide = Cfg<2, 240, 3, false>;
-using WideFp4 = Cfg<2, 224, 3, true>;
-using Narrow = Cfg<1, 128, 6, false>;
-using NarrowFp4 = Cfg<1, 128, 5, true>;
+using Narrow = Cfg<128, 6, false>;
+using NarrowFp4 = Cfg<128, 5, true>;
+using Tall = Cfg<240, 4, false>;
+using TallFp4 = Cfg<224, 4, true>;
 
 template <class C, int DT>
 __global__ void __launch_bounds__(THREADS, 1)
 grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constant__ CUtensorMap map_x16,
                const __grid_constant__ Params p) {
-    constexpr int MH = C::MH, STAGES = C::STAGES;
+    constexpr int STAGES = C::STAGES;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t ring = (raw + 1023u) & ~1023u;
@@ -99,7 +97,6 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constan
     const int KT = (p.K + C::K_STEP - 1) / C::K_STEP, KT128 = (p.K + 127) / 128;
     const int ftiles = (p.N + C::FEATURES - 1) / C::FEATURES;
     Walk walk(tiles, first, p.rows.groups, ftiles);
-    auto halves_of = [&](const Unit& t) { return MH == 2 && p.N - t.f0 > 128 ? 2 : 1; };
 
     // The kernel before this one quantises the rows.  It lets this one start when everything before it has completed, so that
     // all but its own output may be read at once: the weights are on their way while the rows are quantised.
@@ -114,9 +111,9 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constan
         uint32_t issued = 0;
         for (int u = blockIdx.x; u < walk.total && ok; u += gridDim.x) {
             const Unit t = walk.at(u, C::FEATURES);
-            const int halves = uniform(halves_of(t)), row = uniform(t.row);
+            const int row = uniform(t.row);
             const uint32_t n = uniform(t.padded());
-            const uint8_t* w = p.w + (size_t)uniform(t.g) * p.w_group + (size_t)uniform(t.ftile * MH) * KT * C::Tile::BYTES;
+            const uint8_t* w = p.w + (size_t)uniform(t.g) * p.w_group + (size_t)uniform(t.ftile) * KT * C::Tile::BYTES;
             const uint8_t* x_sf = p.x_sf + (size_t)uniform(t.begin / p.rows.width + t.g + t.tile) * KT128 * (C::X_CHUNKS * 512);
             const uint32_t x_chunks = n > 128 ? 2 : 1;
             for (int kt = 0; kt < KT; ++kt, ++issued, at.step()) {
@@ -125,17 +122,15 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constan
                 const uint32_t st = ring + at.s * C::STAGE_BYTES, full = full_bar(at.s);
                 if (elect_one()) {
                     if (warp == 0) {
-                        mbar_expect_tx(full, (uint32_t)halves * C::Tile::BYTES);
-                        for (int h = 0; h < halves; ++h) {
-                            const uint8_t* block = w + ((size_t)h * KT + kt) * C::Tile::BYTES;
-                            bulk_load(st + h * 16384, block, C::Tile::CODES, full);
-                            bulk_load(st + C::SFW + h * C::SF_STEPS * 512, block + C::Tile::CODES, C::SF_STEPS * 512, full);
-                        }
+                        const uint8_t* block = w + (size_t)kt * C::Tile::BYTES;
+                        mbar_expect_tx(full, C::Tile::BYTES);
+                        bulk_load(st, block, C::Tile::CODES, full);
+                        bulk_load(st + C::SFW, block + C::Tile::CODES, C::SF_STEPS * 512, full);
                     } else {
                         mbar_expect_tx(full, n * 128u + C::SF_STEPS * x_chunks * 512u);
                         uint32_t r = 0;
-                        for (; r + 64 <= n; r += 64) tma_load_2d(st + C::W_BYTES + r * 128, &map_x64, kt * C::K_STEP, row + r, full);
-                        for (; r < n; r += 16) tma_load_2d(st + C::W_BYTES + r * 128, &map_x16, kt * C::K_STEP, row + r, full);
+                        for (; r + 64 <= n; r += 64) tma_load_2d(st + C::X + r * 128, &map_x64, kt * C::K_STEP, row + r, full);
+                        for (; r < n; r += 16) tma_load_2d(st + C::X + r * 128, &map_x16, kt * C::K_STEP, row + r, full);
 #pragma unroll
                         for (int c = 0; c < C::SF_STEPS; ++c)
                             bulk_load(st + C::SFX + c * C::X_CHUNKS * 512, x_sf + (size_t)(kt * C::SF_STEPS + c) * (C::X_CHUNKS * 512),
@@ -152,21 +147,20 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constan
         // ---------------- MMA issuer ----------------
         // One thread's issue rate is what a narrow tile's products run at, so everything here is uniform over the warp (the
         // instructions take their operands from uniform registers) and the thread is elected.  The scales of a stage are copied
-        // to tensor memory before the last products of the stage in front of it, into the other set of columns: behind
-        // them the copies would hold up the tensor pipe (256 x 240: 1330 -> 1060 cycles per 128 of K).
+        // to tensor memory before the products of the stage in front of it, into the other set of columns: right in front of their own
+        // products the copies hold up the tensor pipe (256 x 240 x 128: 1330 -> 1060 cycles).
         uint32_t count = 0, set = 0;
         bool ok = true, copied = false;
         RingAt<STAGES> at;
         int u = blockIdx.x;
         Unit next = u < walk.total ? walk.at(u, C::FEATURES) : Unit{};
-        auto copy_scales = [&](int s, uint32_t into, int halves, uint32_t n) {
+        auto copy_scales = [&](int s, uint32_t into, uint32_t n) {
             const uint32_t from = ring + s * C::STAGE_BYTES, sfw = tmem + C::SFW_COL + into, sfx = tmem + C::SFX_COL + into;
             if (elect_one()) {
 #pragma unroll
                 for (int c = 0; c < C::SF_STEPS; ++c) {
                     const uint32_t w = from + C::SFW + c * 512, x = from + C::SFX + c * C::X_CHUNKS * 512;
                     tmem_cp_32x128b(sfw + 8 * c, smem_desc(w, 0, 128, LAYOUT_NONE));
-                    if (MH == 2 && halves == 2) tmem_cp_32x128b(sfw + 8 * c + 4, smem_desc(w + C::SF_STEPS * 512, 0, 128, LAYOUT_NONE));
                     tmem_cp_32x128b(sfx + 8 * c, smem_desc(x, 0, 128, LAYOUT_NONE));
                     if (C::X_CHUNKS == 2 && n > 128) tmem_cp_32x128b(sfx + 8 * c + 4, smem_desc(x + 512, 0, 128, LAYOUT_NONE));
                 }
@@ -174,59 +168,47 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constan
             __syncwarp();
         };
         for (; u < walk.total && ok; u += gridDim.x, ++count) {
-            const int halves = uniform(halves_of(next));
             const uint32_t n = uniform(next.padded());
             const bool more = u + (int)gridDim.x < walk.total;
             if (more) next = walk.at(u + gridDim.x, C::FEATURES);
-            const int next_halves = uniform(halves_of(next));
             const uint32_t next_n = uniform(next.padded());
-            const uint32_t idesc_n = p.idesc | ((n >> 3) << 17);
-            const int buf = MH == 1 ? (int)(count & 1u) : 0;
-            for (int kt = 0; kt < KT; ++kt, set ^= C::SF_COLS) {
+            const uint32_t idesc = p.idesc | ((n >> 3) << 17);
+            const int buf = (int)(count & 1u);
+            // the first product into an accumulator overwrites it: the epilogue must have read what it held
+            if (count >= 2) ok = mbar_wait(accum_empty(buf), ((count >> 1) - 1) & 1, p.status, ST_MMA_TIMEOUT);
+            tc_fence_after();
+            const uint32_t d = tmem + buf * C::ACC_STRIDE;
+            for (int kt = 0; kt < KT && ok; ++kt, set ^= C::SF_COLS) {
                 const uint32_t st = ring + at.s * C::STAGE_BYTES, empty = empty_bar(at.s);
                 if (!copied) {
                     ok = mbar_wait(full_bar(at.s), at.phase, p.status, ST_MMA_TIMEOUT);
                     tc_fence_after();
                     if (!ok) break;
-                    copy_scales(at.s, set, halves, n);
+                    copy_scales(at.s, set, n);
                 }
                 copied = false;
-                auto products = [&](int h, int a, bool last) {
-                    const uint64_t w_desc = smem_desc(st + h * 16384, 16, 1024, LAYOUT_SW128), x_desc = smem_desc(st + C::W_BYTES, 16, 1024, LAYOUT_SW128);
-                    const uint32_t d = tmem + a * C::ACC_STRIDE, sfw = tmem + C::SFW_COL + set + 4 * h, sfx = tmem + C::SFX_COL + set;
-                    if (elect_one()) {
-#pragma unroll
-                        for (uint32_t k = 0; k < 4; ++k) {
-                            const uint32_t acc = (kt > 0 || k > 0) ? 1u : 0u;
-                            if constexpr (C::MXF4) {
-                                const uint32_t id = (k & 1u) * 2u;                 // 64 elements: scale bytes (0, 1) or (2, 3) of step k / 2
-                                mma_mxf4(d, w_desc + 2 * k, x_desc + 2 * k, idesc_n | (id << 29) | (id << 4), sfw + 8 * (k >> 1), sfx + 8 * (k >> 1), acc);
-                            } else {
-                                mma_mxf8f6f4(d, w_desc + 2 * k, x_desc + 2 * k, idesc_n | (k << 29) | (k << 4), sfw, sfx, acc);
-                            }
-                        }
-                        if (last) mma_commit(empty);                               // frees the stage once these products have read it
-                    }
-                    __syncwarp();
-                };
-                // the first product into an accumulator overwrites it: the epilogue must have read what it held
-                auto free_accumulator = [&](int a, uint32_t uses) {
-                    if (kt == 0 && uses > 0) { ok = mbar_wait(accum_empty(a), (uses - 1) & 1, p.status, ST_MMA_TIMEOUT); tc_fence_after(); }
-                    return ok;
-                };
                 at.step();
-                if (MH == 2 && free_accumulator(0, count)) products(0, 0, halves == 1);
-                if (ok && (kt + 1 < KT || more) && mbar_test_wait(full_bar(at.s), at.phase)) {
+                if ((kt + 1 < KT || more) && mbar_test_wait(full_bar(at.s), at.phase)) {
                     tc_fence_after();
-                    copy_scales(at.s, set ^ C::SF_COLS, kt + 1 < KT ? halves : next_halves, kt + 1 < KT ? n : next_n);
+                    copy_scales(at.s, set ^ C::SF_COLS, kt + 1 < KT ? n : next_n);
                     copied = true;
                 }
-                if constexpr (MH == 2) {
-                    if (halves == 2 && ok && free_accumulator(1, count)) products(1, 1, true);
-                } else {
-                    if (ok && free_accumulator(buf, count >> 1)) products(0, buf, true);
+                const uint64_t w_desc = smem_desc(st, 16, 1024, LAYOUT_SW128), x_desc = smem_desc(st + C::X, 16, 1024, LAYOUT_SW128);
+                const uint32_t sfw = tmem + C::SFW_COL + set, sfx = tmem + C::SFX_COL + set;
+                if (elect_one()) {
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k) {
+                        const uint32_t acc = (kt > 0 || k > 0) ? 1u : 0u;
+                        if constexpr (C::MXF4) {
+                            const uint32_t id = (k & 1u) * 2u;                     // 64 elements: scale bytes (0, 1) or (2, 3) of step k / 2
+                            mma_mxf4(d, w_desc + 2 * k, x_desc + 2 * k, idesc | (id << 29) | (id << 4), sfw + 8 * (k >> 1), sfx + 8 * (k >> 1), acc);
+                        } else {
+                            mma_mxf8f6f4(d, w_desc + 2 * k, x_desc + 2 * k, idesc | (k << 29) | (k << 4), sfw, sfx, acc);
+                        }
+                    }
+                    mma_commit(empty);                                             // frees the stage once these products have read it
                 }
-                if (!ok) break;
+                __syncwarp();
             }
             if (elect_one()) mma_commit(accum_full(buf));
             __syncwarp();
@@ -253,15 +235,14 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constan
         uint32_t count = 0;
         for (int u = blockIdx.x; u < walk.total && ok; u += gridDim.x, ++count) {
             const Unit t = walk.at(u, C::FEATURES);
-            const int halves = halves_of(t);
-            const int buf = MH == 1 ? (int)(count & 1u) : 0;
+            const int buf = (int)(count & 1u), f = t.f0 + ef;
             const int chunks = (t.rows + 15) >> 4;
             Four<T> e[4];
-            auto request = [&](int h, int c) {
+            auto request = [&](int c) {
                 if (p.extra_mode == X_NONE) return;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int r = c * 16 + i * 4 + er, f = t.f0 + h * 128 + ef;
+                    const int r = c * 16 + i * 4 + er;
                     if (r < t.rows) load_four(extra + (size_t)(t.row + r) * p.N + f, p.N - f, p.vector, e[i]);
                 }
             };
@@ -272,48 +253,34 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constan
                     asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char*>(extra + (size_t)(t.row + i / lines) * p.N + t.f0) +
                                                                   min(i % lines * 128, bytes - 1)));
             }
-            if (side < chunks) request(0, side);
-            ok = mbar_wait(accum_full(buf), MH == 1 ? (count >> 1) & 1 : count & 1, p.status, ST_EPILOGUE_TIMEOUT);
+            float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (p.bias != nullptr) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) if (f + i < p.N) bias[i] = widen(reinterpret_cast<const T*>(p.bias)[(size_t)t.g * p.N + f + i]);
+            }
+            if (side < chunks) request(side);
+            ok = mbar_wait(accum_full(buf), (count >> 1) & 1, p.status, ST_EPILOGUE_TIMEOUT);
             tc_fence_after();
             if (!ok) break;
-            for (int h = 0; h < MH; ++h) {
-                const int a = MH == 1 ? buf : h;
-                const int f = t.f0 + h * 128 + ef;
-                const bool reads = h < halves && side < chunks;
-                float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                if (reads && p.bias != nullptr) {
+            for (int c = side; c < chunks; c += 2) {
+                uint32_t r[32];
+                tmem_ld_32x32b_x16(tmem + ((uint32_t)(q * 32) << 16) + buf * C::ACC_STRIDE + c * 16, r);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) if (f + i < p.N) bias[i] = widen(reinterpret_cast<const T*>(p.bias)[(size_t)t.g * p.N + f + i]);
-                }
-                if (reads) {
-                    for (int c = side; c < chunks; c += 2) {
-                        uint32_t r[32];
-                        tmem_ld_32x32b_x16(tmem + ((uint32_t)(q * 32) << 16) + a * C::ACC_STRIDE + c * 16, r);
-                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                        if (c + 2 >= chunks) {                               // the last read of this accumulator: hand it back
-                            tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(accum_empty(a));
-                        }
+                for (int j = 0; j < 16; ++j) slot[j * 32 + lane] = __uint_as_float(r[j]);
+                __syncwarp();
+                Four<T> now[4];
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) slot[j * 32 + lane] = __uint_as_float(r[j]);
-                        __syncwarp();
-                        Four<T> now[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) now[i].w = e[i].w;
-                        if (c + 2 < chunks) request(h, c + 2);
-                        else if (h + 1 < halves) request(h + 1, side);
-                        T* at = out + (size_t)(t.row + c * 16 + er) * p.N + f;
-                        const int rows = (t.rows - c * 16 - er + 3) >> 2, left = p.N - f;
-                        finish_any(p.act, slot, lane, bias, now, p.extra_mode, at, p.N, rows, left, p.vector);
-                        __syncwarp();
-                    }
-                } else {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(accum_empty(a));
-                }
+                for (int i = 0; i < 4; ++i) now[i].w = e[i].w;
+                if (c + 2 < chunks) request(c + 2);
+                T* at = out + (size_t)(t.row + c * 16 + er) * p.N + f;
+                const int rows = (t.rows - c * 16 - er + 3) >> 2, left = p.N - f;
+                finish_any(p.act, slot, lane, bias, now, p.extra_mode, at, p.N, rows, left, p.vector);
+                __syncwarp();
             }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(accum_empty(buf));
         }
         if (p.zero_rest) zero_rows_outside(out, first[0], first[p.rows.groups], p.rows.rows, p.N, threadIdx.x - FIRST_EPI_WARP * 32, EPI_WARPS * 32);
     }
@@ -540,17 +507,32 @@ static bool valid_mx_preset(int eb, int fb) {
 }
 static int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 
-// Kernel and tile shape of a call, from the sizes that the host knows.
+// Kernel and tile width of a call, from the sizes that the host knows.
+enum Shape { DECODE, NARROW, TALL };
 struct Plan {
-    bool decode;                 // a few rows per group: mxq_grouped_decode.cu, where x and its format allow
-    bool narrow;                 // 128 features, up to 128 rows (else 256, and 240 or 224)
-    int width;
-    int chunks() const { return narrow ? 1 : 2; }
+    Shape shape;                 // the kernel for few rows, where x and its format allow; tiles of up to 128 rows; up to 240 (224 of E2M1 pairs)
+    int width;                   // rows per tile at most
+    int chunks() const { return shape <= NARROW ? 1 : 2; }
     int64_t sf_bytes(int64_t rows, int64_t groups, int64_t K) const { return (rows / width + groups + 1) * ((K + 127) / 128) * chunks() * 512; }
 };
-static Plan make_plan(int64_t rows, int64_t groups, bool fp4) {
-    const bool narrow = rows / groups <= 128;
-    return Plan{groups == 1 ? rows <= decode_rows() : rows / groups <= decode_rows() / 2, narrow, narrow ? Narrow::BT : fp4 ? WideFp4::BT : Wide::BT};
+// The width whose tiles take the fewest estimated cycles of the whole GPU: rounds of tiles x steps of K x the larger of what one thread
+// issues (some 400 cycles) and what L2 gives all SMs together (13.4 TB/s measured: 47.6 KB of a 240-row step in 534 ns on 148 SMs, 33.3 KB
+// of a 128-row step in 364 ns).  Measured widths this picks between, microseconds: 8192 rows, 14336 x 4096: 596 (128 rows), 486 (240);
+// 192 rows, 4096 x 4096: 21.1 (64), 20.0 (128), 22.9 (240); 2048 rows, 2048 x 2048: 33.7 (64), 26.1 (128), 24.9 (240).
+// (Tiles of 256 x 240 have fewer bytes per product, but fill tensor memory: their epilogue overlaps nothing, 544.)
+static Plan make_plan(int64_t rows, int64_t groups, int64_t N, int64_t K, bool fp4) {
+    if (groups == 1 ? rows <= decode_rows() : rows / groups <= decode_rows() / 2) return Plan{DECODE, Narrow::BT};
+    const int64_t sms = sm_count(), each = (rows + groups - 1) / groups, ftiles = (N + 127) / 128, steps = (K + (fp4 ? 255 : 127)) / (fp4 ? 256 : 128);
+    Plan best{NARROW, 0};
+    double least = 0.0;
+    for (int width = 48; width <= (fp4 ? TallFp4::BT : Tall::BT); width += 16) {
+        const int64_t per_group = (each + width - 1) / width, units = per_group * groups * ftiles;
+        const double used = (double)(((each + per_group - 1) / per_group + 15) / 16 * 16), busy = units < sms ? (double)units / sms : 1.0;
+        const double step = (17.0 + 0.128 * used) * 11.05 * busy;                     // ns
+        const double cost = (double)((units + sms - 1) / sms * steps) * (step > 215.0 ? step : 215.0);
+        if (best.width == 0 || cost < 0.98 * least) { best = Plan{width <= Narrow::BT ? NARROW : TALL, width}; least = cost; }
+    }
+    return best;
 }
 
 }  // namespace grouped
@@ -585,14 +567,16 @@ extern "C" int mxq_mx_pack_experts(const uint8_t* scales, const uint8_t* element
 
 // the decode kernel quantises by itself: no operand in memory
 static bool takes_decode(const grouped::Plan& plan, const void* x, int round_mode) {
-    return plan.decode && round_mode == MXQ_RN && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+    return plan.shape == grouped::DECODE && round_mode == MXQ_RN && reinterpret_cast<uintptr_t>(x) % 16 == 0;
 }
 
-extern "C" int64_t mxq_mx_grouped_scratch_bytes(const void* x, int round_mode, int64_t rows_in, int64_t rows, int64_t K, int64_t groups) {
-    if (rows_in < 0 || rows < 0 || groups <= 0 || K <= 0 || K % 32 != 0) return MXQ_EINVAL;
-    const grouped::Plan plan = grouped::make_plan(rows, groups, true);
+extern "C" int64_t mxq_mx_grouped_scratch_bytes(const void* x, int round_mode, int64_t rows_in, int64_t rows, int64_t K, int64_t groups, int64_t N) {
+    if (rows_in < 0 || rows < 0 || groups <= 0 || N <= 0 || K <= 0 || K % 32 != 0) return MXQ_EINVAL;
+    const grouped::Plan plan = grouped::make_plan(rows, groups, N, K, false);
     if (rows == 0 || takes_decode(plan, x, round_mode)) return 0;
-    return grouped::align256(rows * K) + grouped::align256(plan.sf_bytes(rows, groups, K)) + grouped::align256(rows_in * K) + grouped::align256(rows_in * K / 32);
+    // (whichever way the weight is packed)
+    const int64_t sf = std::max(plan.sf_bytes(rows, groups, K), grouped::make_plan(rows, groups, N, K, true).sf_bytes(rows, groups, K));
+    return grouped::align256(rows * K) + grouped::align256(sf) + grouped::align256(rows_in * K) + grouped::align256(rows_in * K / 32);
 }
 
 extern "C" int mxq_mx_grouped_linear(const void* x, int x_dtype, int64_t rows_in, int64_t rows, int64_t K, int x_exp_bits, int x_frac_bits,
@@ -609,7 +593,7 @@ extern "C" int mxq_mx_grouped_linear(const void* x, int x_dtype, int64_t rows_in
     if (rows == 0) return MXQ_OK;
     if ((!x && rows_in > 0) || !w_packed || !out || (extra_mode != MXQ_EXTRA_NONE && !extra)) return MXQ_EINVAL;
     if (reinterpret_cast<uintptr_t>(w_packed) % 16 != 0 || reinterpret_cast<uintptr_t>(scratch) % 256 != 0) return MXQ_EINVAL;
-    const int64_t needed = mxq_mx_grouped_scratch_bytes(x, x_round_mode, rows_in, rows, K, groups);
+    const int64_t needed = mxq_mx_grouped_scratch_bytes(x, x_round_mode, rows_in, rows, K, groups, N);
     if (needed > 0 && !scratch) return MXQ_EINVAL;
     if (scratch_bytes < needed) return MXQ_ESIZE;
     // both operands E2M1 and the weight kept as nibbles: the 4-bit kind
@@ -620,7 +604,7 @@ extern "C" int mxq_mx_grouped_linear(const void* x, int x_dtype, int64_t rows_in
     if (!grouped::valid_mx_preset(x_exp_bits, x_frac_bits) || x_round_mode < MXQ_RN || x_round_mode > MXQ_RZ) return MXQ_EINVAL;
     const int x_fmt = x_exp_bits == 5 ? 1 : 0;
 
-    const grouped::Plan plan = grouped::make_plan(rows, groups, fp4);
+    const grouped::Plan plan = grouped::make_plan(rows, groups, N, K, fp4);
     grouped::Params p{};
     p.w = w_packed;
     p.w_group = fp4 ? grouped::WeightTile<true>::group_bytes(N, K) : grouped::WeightTile<false>::group_bytes(N, K);
@@ -658,6 +642,7 @@ extern "C" int mxq_mx_grouped_linear(const void* x, int x_dtype, int64_t rows_in
         rc = check_launch();
     }
     if (rc != MXQ_OK) return rc;
-    if (fp4) return plan.narrow ? grouped::launch_dt<grouped::NarrowFp4>(p, x_dtype, codes, st) : grouped::launch_dt<grouped::WideFp4>(p, x_dtype, codes, st);
-    return plan.narrow ? grouped::launch_dt<grouped::Narrow>(p, x_dtype, codes, st) : grouped::launch_dt<grouped::Wide>(p, x_dtype, codes, st);
+    using namespace grouped;
+    if (plan.shape == TALL) return fp4 ? launch_dt<TallFp4>(p, x_dtype, codes, st) : launch_dt<Tall>(p, x_dtype, codes, st);
+    return fp4 ? launch_dt<NarrowFp4>(p, x_dtype, codes, st) : launch_dt<Narrow>(p, x_dtype, codes, st);
 }

@@ -162,7 +162,7 @@ def grouped_linear(x: Tensor, x_meta: MXFPMeta, w: PackedExperts, offsets: Tenso
     status = status_address(dev)
     L = _lib.load()
     x_ptr, round_id = x.data_ptr(), _lib.ROUND_ID[x_meta.round_mode]
-    nbytes = L.mxq_mx_grouped_scratch_bytes(x_ptr, round_id, tokens, rows, K, groups)
+    nbytes = L.mxq_mx_grouped_scratch_bytes(x_ptr, round_id, tokens, rows, K, groups, N)
     # of this call alone: two captured graphs, or two streams, never share it
     scratch = None if nbytes == 0 else torch.empty(nbytes, dtype=torch.uint8, device=x.device)
     args = (x_ptr, dtype_id, tokens, rows, K, x_meta.element_exp_bits, x_meta.element_frac_bits, round_id, index_ptr, index64, w.pointer, w.hw_format, groups,

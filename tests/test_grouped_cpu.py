@@ -155,7 +155,7 @@ def test_c_entry_refuses_before_it_launches():
         assert L.mxq_mx_grouped_linear(*(good | bad).values()) == -1, bad
     for bad in (dict(groups=L.mxq_mx_max_groups() + 1, offsets=p), dict(nbytes=64, rm=1), dict(rows=1 << 31, rows_in=1 << 31)):
         assert L.mxq_mx_grouped_linear(*(good | bad).values()) == -3, bad
-    assert L.mxq_mx_grouped_scratch_bytes(p, 0, 2, 2, 48, 1) == -1 and L.mxq_mx_grouped_scratch_bytes(p, 0, 2, 2, 64, 1) == 0
-    assert L.mxq_mx_grouped_scratch_bytes(p + 2, 0, 2, 2, 64, 1) > 0 and L.mxq_mx_grouped_scratch_bytes(p, 1, 2, 2, 64, 1) > 0
-    assert L.mxq_mx_grouped_scratch_bytes(p, 0, 500, 500, 64, 1) > 0
+    assert L.mxq_mx_grouped_scratch_bytes(p, 0, 2, 2, 48, 1, 8) == -1 and L.mxq_mx_grouped_scratch_bytes(p, 0, 2, 2, 64, 1, 8) == 0
+    assert L.mxq_mx_grouped_scratch_bytes(p + 2, 0, 2, 2, 64, 1, 8) > 0 and L.mxq_mx_grouped_scratch_bytes(p, 1, 2, 2, 64, 1, 8) > 0
+    assert L.mxq_mx_grouped_scratch_bytes(p, 0, 500, 500, 64, 1, 8) > 0
     assert SimpleNamespace(**good).K == 64
