@@ -30,14 +30,16 @@ constexpr int EPI_WARPS = 8;                     // two per TMEM lane quadrant
 constexpr int FIRST_EPI_WARP = 4;                // warps 0, 1, 3: weight copies, MMA issuer, row copies
 constexpr int THREADS = (FIRST_EPI_WARP + EPI_WARPS) * 32;
 
-// A tile is 128 features x at most BT rows; MXF4: both operands packed E2M1 nibbles (256 elements of K per 128 bytes).
-template <int BT_, int STAGES_, bool MXF4_> struct Cfg {
-    static constexpr int BT = BT_, STAGES = STAGES_;
+// A CTA's tile is 128 features x at most BT rows; MXF4: both operands packed E2M1 nibbles (256 elements of K per 128 bytes).
+// CTAS = 2: a pair of CTAs on two neighbouring SMs takes 256 features and the same rows, each brings its own weights and half of the
+// rows: what tensor tiles read from L2 bounds a large product, and a pair reads two thirds (32 KB a step and SM instead of 48).
+template <int BT_, int STAGES_, bool MXF4_, int CTAS_ = 1> struct Cfg {
+    static constexpr int BT = BT_, STAGES = STAGES_, CTAS = CTAS_;
     static constexpr bool MXF4 = MXF4_;
-    static constexpr int FEATURES = 128;
+    static constexpr int FEATURES = 128 * CTAS;                     // of a unit of work
     using Tile = WeightTile<MXF4>;
     static constexpr int K_STEP = Tile::K_STEP, SF_STEPS = Tile::SF_STEPS;          // elements of K and 128-element steps of scales per stage
-    static constexpr int X_BYTES = BT * 128, X_CHUNKS = BT > 128 ? 2 : 1;
+    static constexpr int X_BYTES = BT / CTAS * 128, X_CHUNKS = BT > 128 ? 2 : 1;
     // a stage: weight codes | row codes | scales: [SF_STEPS][512] of the weights, [SF_STEPS][X_CHUNKS][512] of the rows
     static constexpr int X = Tile::CODES, SFW = X + X_BYTES, SFX = SFW + SF_STEPS * 512;
     static constexpr int STAGE_BYTES = (SFX + SF_STEPS * X_CHUNKS * 512 + 1023) / 1024 * 1024;      // the 128-byte swizzle repeats every 1024 bytes
@@ -56,41 +58,42 @@ using Narrow = Cfg<128, 6, false>;
 using NarrowFp4 = Cfg<128, 5, true>;
 using Tall = Cfg<240, 4, false>;
 using TallFp4 = Cfg<224, 4, true>;
+using Pair = Cfg<240, 6, false, 2>;
+using PairFp4 = Cfg<224, 6, true, 2>;
 
 template <class C, int DT>
 __global__ void __launch_bounds__(THREADS, 1)
-grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constant__ CUtensorMap map_x16,
+grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constant__ CUtensorMap map_x16, const __grid_constant__ CUtensorMap map_x8,
                const __grid_constant__ Params p) {
-    constexpr int STAGES = C::STAGES;
+    constexpr int STAGES = C::STAGES, CTAS = C::CTAS;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t ring = (raw + 1023u) & ~1023u;
     uint8_t* ring_ptr = smem_raw + (ring - raw);
-    const uint32_t bars = ring + STAGES * C::STAGE_BYTES;            // full[S], empty[S], accum_full[2], accum_empty[2], drain, tmem slot
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ring_ptr + STAGES * C::STAGE_BYTES + 8 * (2 * STAGES + 5));
+    const uint32_t bars = ring + STAGES * C::STAGE_BYTES;            // full[S], empty[S], peer_full[S], accum_full[2], accum_empty[2], drain, tmem slot
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ring_ptr + STAGES * C::STAGE_BYTES + 8 * (3 * STAGES + 5));
     int* tiles = reinterpret_cast<int*>(ring_ptr + STAGES * C::STAGE_BYTES + 256);
     int* first = tiles + MAX_GROUPS + 1;
     auto full_bar = [&](int s) { return bars + 8u * s; };
     auto empty_bar = [&](int s) { return bars + 8u * (STAGES + s); };
-    auto accum_full = [&](int a) { return bars + 8u * (2 * STAGES + a); };
-    auto accum_empty = [&](int a) { return bars + 8u * (2 * STAGES + 2 + a); };
-    const uint32_t drain_bar = bars + 8u * (2 * STAGES + 4);
+    auto peer_full = [&](int s) { return bars + 8u * (2 * STAGES + s); };            // in the leader: the other CTA's part of the stage is there
+    auto accum_full = [&](int a) { return bars + 8u * (3 * STAGES + a); };
+    auto accum_empty = [&](int a) { return bars + 8u * (3 * STAGES + 2 + a); };
+    const uint32_t drain_bar = bars + 8u * (3 * STAGES + 4);
 
     const int warp = __shfl_sync(~0u, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) { mbar_init(full_bar(s), 2); mbar_init(empty_bar(s), 1); }      // full: weight copies, row copies
-        for (int a = 0; a < 2; ++a) { mbar_init(accum_full(a), 1); mbar_init(accum_empty(a), EPI_WARPS); }
+        for (int s = 0; s < STAGES; ++s) { mbar_init(full_bar(s), 2); mbar_init(empty_bar(s), 1); mbar_init(peer_full(s), 1); }      // full: weight copies, row copies
+        for (int a = 0; a < 2; ++a) { mbar_init(accum_full(a), 1); mbar_init(accum_empty(a), EPI_WARPS * CTAS); }
         mbar_init(drain_bar, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == 0 && elect_one()) { prefetch_map(map_x16); prefetch_map(map_x64); }
-    if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
+    if (warp == 0 && elect_one()) { prefetch_map(map_x16); prefetch_map(map_x64); if (CTAS == 2) prefetch_map(map_x8); }
+    if (warp == 1) tc_alloc<CTAS>(smem_u32(tmem_slot), 512);
     tc_fence_before();
     build_table(p.rows, tiles, first);
+    if (CTAS > 1) cluster_barrier();                                // both CTAs' barriers and tensor memory exist
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(~0u, *tmem_slot, 0);
 
@@ -98,6 +101,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constan
     const int ftiles = (p.N + C::FEATURES - 1) / C::FEATURES;
     Walk walk(tiles, first, p.rows.groups, ftiles);
 
+    const int rank = CTAS == 2 ? (int)(blockIdx.x & 1u) : 0, u_begin = blockIdx.x / CTAS, u_step = gridDim.x / CTAS;
     // The kernel before this one quantises the rows.  It lets this one start when everything before it has completed, so that
     // all but its own output may be read at once: the weights are on their way while the rows are quantised.
     // (The kernel behind this one may come up too; it waits for this one's end before it touches memory.)
@@ -109,11 +113,13 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constan
         bool ok = true;
         RingAt<STAGES> at;
         uint32_t issued = 0;
-        for (int u = blockIdx.x; u < walk.total && ok; u += gridDim.x) {
+        for (int u = u_begin; u < walk.total && ok; u += u_step) {
             const Unit t = walk.at(u, C::FEATURES);
-            const int row = uniform(t.row);
-            const uint32_t n = uniform(t.padded());
-            const uint8_t* w = p.w + (size_t)uniform(t.g) * p.w_group + (size_t)uniform(t.ftile) * KT * C::Tile::BYTES;
+            const uint32_t n = uniform(t.padded()), mine = n / CTAS;                             // rows that this CTA brings
+            const int row = uniform(t.row) + rank * (int)mine;
+            // (features in tiles of 128; the second CTA of a pair whose first one has the last of them reads that again and stores nothing)
+            const int ftile = min(uniform(t.ftile) * CTAS + rank, (p.N + 127) / 128 - 1);
+            const uint8_t* w = p.w + (size_t)uniform(t.g) * p.w_group + (size_t)ftile * KT * C::Tile::BYTES;
             const uint8_t* x_sf = p.x_sf + (size_t)uniform(t.begin / p.rows.width + t.g + t.tile) * KT128 * (C::X_CHUNKS * 512);
             const uint32_t x_chunks = n > 128 ? 2 : 1;
             for (int kt = 0; kt < KT; ++kt, ++issued, at.step()) {
@@ -127,10 +133,11 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constan
                         bulk_load(st, block, C::Tile::CODES, full);
                         bulk_load(st + C::SFW, block + C::Tile::CODES, C::SF_STEPS * 512, full);
                     } else {
-                        mbar_expect_tx(full, n * 128u + C::SF_STEPS * x_chunks * 512u);
+                        mbar_expect_tx(full, mine * 128u + C::SF_STEPS * x_chunks * 512u);
                         uint32_t r = 0;
-                        for (; r + 64 <= n; r += 64) tma_load_2d(st + C::X + r * 128, &map_x64, kt * C::K_STEP, row + r, full);
-                        for (; r < n; r += 16) tma_load_2d(st + C::X + r * 128, &map_x16, kt * C::K_STEP, row + r, full);
+                        for (; r + 64 <= mine; r += 64) tma_load_2d(st + C::X + r * 128, &map_x64, kt * C::K_STEP, row + r, full);
+                        for (; r + 16 <= mine; r += 16) tma_load_2d(st + C::X + r * 128, &map_x16, kt * C::K_STEP, row + r, full);
+                        if (CTAS == 2 && r < mine) tma_load_2d(st + C::X + r * 128, &map_x8, kt * C::K_STEP, row + r, full);
 #pragma unroll
                         for (int c = 0; c < C::SF_STEPS; ++c)
                             bulk_load(st + C::SFX + c * C::X_CHUNKS * 512, x_sf + (size_t)(kt * C::SF_STEPS + c) * (C::X_CHUNKS * 512),
@@ -143,6 +150,16 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constan
         // every copy this warp started must have landed before the CTA gives its shared memory back (returns at once in a run that went well)
         for (uint32_t j = issued > (uint32_t)STAGES ? issued - STAGES : 0u; j < issued; ++j)
             mbar_wait(full_bar(j % STAGES), (j / STAGES) & 1, p.status, ST_PRODUCER_TIMEOUT);
+    } else if (warp == 1 && CTAS == 2 && rank == 1) {
+        // ---------------- second CTA of a pair: tell the leader that this CTA's part of a stage is there ----------------
+        bool ok = true;
+        RingAt<STAGES> at;
+        for (int u = u_begin; u < walk.total && ok; u += u_step)
+            for (int kt = 0; kt < KT && ok; ++kt, at.step()) {
+                ok = mbar_wait(full_bar(at.s), at.phase, p.status, ST_MMA_TIMEOUT);
+                if (ok && elect_one()) arrive_at(peer_full(at.s), 0);
+                __syncwarp();
+            }
     } else if (warp == 1) {
         // ---------------- MMA issuer ----------------
         // One thread's issue rate is what a narrow tile's products run at, so everything here is uniform over the warp (the
@@ -152,7 +169,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constan
         uint32_t count = 0, set = 0;
         bool ok = true, copied = false;
         RingAt<STAGES> at;
-        int u = blockIdx.x;
+        int u = u_begin;
         Unit next = u < walk.total ? walk.at(u, C::FEATURES) : Unit{};
         auto copy_scales = [&](int s, uint32_t into, uint32_t n) {
             const uint32_t from = ring + s * C::STAGE_BYTES, sfw = tmem + C::SFW_COL + into, sfx = tmem + C::SFX_COL + into;
@@ -160,35 +177,39 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constan
 #pragma unroll
                 for (int c = 0; c < C::SF_STEPS; ++c) {
                     const uint32_t w = from + C::SFW + c * 512, x = from + C::SFX + c * C::X_CHUNKS * 512;
-                    tmem_cp_32x128b(sfw + 8 * c, smem_desc(w, 0, 128, LAYOUT_NONE));
-                    tmem_cp_32x128b(sfx + 8 * c, smem_desc(x, 0, 128, LAYOUT_NONE));
-                    if (C::X_CHUNKS == 2 && n > 128) tmem_cp_32x128b(sfx + 8 * c + 4, smem_desc(x + 512, 0, 128, LAYOUT_NONE));
+                    tc_copy_scales<CTAS>(sfw + 8 * c, smem_desc(w, 0, 128, LAYOUT_NONE));
+                    tc_copy_scales<CTAS>(sfx + 8 * c, smem_desc(x, 0, 128, LAYOUT_NONE));
+                    if (C::X_CHUNKS == 2 && n > 128) tc_copy_scales<CTAS>(sfx + 8 * c + 4, smem_desc(x + 512, 0, 128, LAYOUT_NONE));
                 }
             }
             __syncwarp();
         };
-        for (; u < walk.total && ok; u += gridDim.x, ++count) {
+        for (; u < walk.total && ok; u += u_step, ++count) {
             const uint32_t n = uniform(next.padded());
-            const bool more = u + (int)gridDim.x < walk.total;
-            if (more) next = walk.at(u + gridDim.x, C::FEATURES);
+            const bool more = u + u_step < walk.total;
+            if (more) next = walk.at(u + u_step, C::FEATURES);
             const uint32_t next_n = uniform(next.padded());
             const uint32_t idesc = p.idesc | ((n >> 3) << 17);
             const int buf = (int)(count & 1u);
             // the first product into an accumulator overwrites it: the epilogue must have read what it held
-            if (count >= 2) ok = mbar_wait(accum_empty(buf), ((count >> 1) - 1) & 1, p.status, ST_MMA_TIMEOUT);
+            if (count >= 2)
+                ok = CTAS == 2 ? mbar_wait_cluster(accum_empty(buf), ((count >> 1) - 1) & 1, p.status, ST_MMA_TIMEOUT)
+                               : mbar_wait(accum_empty(buf), ((count >> 1) - 1) & 1, p.status, ST_MMA_TIMEOUT);
             tc_fence_after();
             const uint32_t d = tmem + buf * C::ACC_STRIDE;
             for (int kt = 0; kt < KT && ok; ++kt, set ^= C::SF_COLS) {
                 const uint32_t st = ring + at.s * C::STAGE_BYTES, empty = empty_bar(at.s);
                 if (!copied) {
                     ok = mbar_wait(full_bar(at.s), at.phase, p.status, ST_MMA_TIMEOUT);
+                    if (CTAS == 2 && ok) ok = mbar_wait_cluster(peer_full(at.s), at.phase, p.status, ST_MMA_TIMEOUT);
                     tc_fence_after();
                     if (!ok) break;
                     copy_scales(at.s, set, n);
                 }
                 copied = false;
                 at.step();
-                if ((kt + 1 < KT || more) && mbar_test_wait(full_bar(at.s), at.phase)) {
+                if ((kt + 1 < KT || more) && mbar_test_wait(full_bar(at.s), at.phase) &&
+                    (CTAS == 1 || mbar_test_wait_cluster(peer_full(at.s), at.phase))) {
                     tc_fence_after();
                     copy_scales(at.s, set ^ C::SF_COLS, kt + 1 < KT ? n : next_n);
                     copied = true;
@@ -199,23 +220,20 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constan
 #pragma unroll
                     for (uint32_t k = 0; k < 4; ++k) {
                         const uint32_t acc = (kt > 0 || k > 0) ? 1u : 0u;
-                        if constexpr (C::MXF4) {
-                            const uint32_t id = (k & 1u) * 2u;                     // 64 elements: scale bytes (0, 1) or (2, 3) of step k / 2
-                            mma_mxf4(d, w_desc + 2 * k, x_desc + 2 * k, idesc | (id << 29) | (id << 4), sfw + 8 * (k >> 1), sfx + 8 * (k >> 1), acc);
-                        } else {
-                            mma_mxf8f6f4(d, w_desc + 2 * k, x_desc + 2 * k, idesc | (k << 29) | (k << 4), sfw, sfx, acc);
-                        }
+                        // scale byte k of a column; 64 elements of 4-bit pairs: bytes (0, 1) or (2, 3) of step k / 2
+                            const uint32_t id = C::MXF4 ? (k & 1u) * 2u : k, step = C::MXF4 ? 8 * (k >> 1) : 0u;
+                            tc_mma<CTAS, C::MXF4>(d, w_desc + 2 * k, x_desc + 2 * k, idesc | (id << 29) | (id << 4), sfw + step, sfx + step, acc);
                     }
-                    mma_commit(empty);                                             // frees the stage once these products have read it
+                    tc_commit<CTAS>(empty);                                             // frees the stage once these products have read it
                 }
                 __syncwarp();
             }
-            if (elect_one()) mma_commit(accum_full(buf));
+            if (elect_one()) tc_commit<CTAS>(accum_full(buf));
             __syncwarp();
         }
         if (!ok) {
             // unwinding after a wait that ran out: the MMAs already issued must finish before tensor memory is freed
-            if (elect_one()) mma_commit(drain_bar);
+            if (elect_one()) tc_commit<CTAS>(drain_bar);
             __syncwarp();
             mbar_wait(drain_bar, 0, nullptr, 0);
         }
@@ -233,9 +251,9 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constan
         const T* extra = reinterpret_cast<const T*>(p.extra);
         bool ok = true;
         uint32_t count = 0;
-        for (int u = blockIdx.x; u < walk.total && ok; u += gridDim.x, ++count) {
+        for (int u = u_begin; u < walk.total && ok; u += u_step, ++count) {
             const Unit t = walk.at(u, C::FEATURES);
-            const int buf = (int)(count & 1u), f = t.f0 + ef;
+            const int buf = (int)(count & 1u), f0 = t.f0 + rank * 128, f = f0 + ef;
             const int chunks = (t.rows + 15) >> 4;
             Four<T> e[4];
             auto request = [&](int c) {
@@ -246,11 +264,11 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constan
                     if (r < t.rows) load_four(extra + (size_t)(t.row + r) * p.N + f, p.N - f, p.vector, e[i]);
                 }
             };
-            if (p.extra_mode != X_NONE) {
+            if (p.extra_mode != X_NONE && f0 < p.N) {
                 // the whole tile of the second operand on its way to L2 while the products are formed: 128-byte lines, rows dealt to the threads
-                const int bytes = min(C::FEATURES, p.N - t.f0) * (int)sizeof(T), lines = (bytes + 127) >> 7;
+                const int bytes = min(128, p.N - f0) * (int)sizeof(T), lines = (bytes + 127) >> 7;
                 for (int i = threadIdx.x - FIRST_EPI_WARP * 32; i < t.rows * lines; i += EPI_WARPS * 32)
-                    asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char*>(extra + (size_t)(t.row + i / lines) * p.N + t.f0) +
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char*>(extra + (size_t)(t.row + i / lines) * p.N + f0) +
                                                                   min(i % lines * 128, bytes - 1)));
             }
             float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -280,15 +298,16 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constan
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(accum_empty(buf));
+            if (lane == 0) { if (rank == 0) mbar_arrive(accum_empty(buf)); else arrive_at(accum_empty(buf), 0); }
         }
         if (p.zero_rest) zero_rows_outside(out, first[0], first[p.rows.groups], p.rows.rows, p.N, threadIdx.x - FIRST_EPI_WARP * 32, EPI_WARPS * 32);
     }
     tc_fence_before();
     __syncthreads();
+    if (CTAS > 1) cluster_barrier();                                // neither CTA leaves while the other reads its memory or arrives on its barriers
     if (warp == 1) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+        tc_dealloc<CTAS>(tmem, 512);
     }
 }
 
@@ -474,7 +493,7 @@ static int quantize_rows(const void* x, int x_dtype, const void* row_index, int 
     with_kind(x_dtype, [&](auto kin) {
         using KIn = decltype(kin);
         with_row_format(eb, fb, o.nibbles, [&](auto fmt, auto out) {
-            rc = launch_after(quantize_rows_kernel<KIn, decltype(fmt), decltype(out)::value>, (unsigned)(rows * segments), (unsigned)block, 0, st, x, row_index,
+            rc = launch_after(quantize_rows_kernel<KIn, decltype(fmt), decltype(out)::value>, (unsigned)(rows * segments), (unsigned)block, 0, 1, st, x, row_index,
                               index64, rows_in, g, o, (int)segments, early);
         });
     });
@@ -486,12 +505,13 @@ static int launch(const Params& p, const uint8_t* x_codes, cudaStream_t st) {
     static bool attr_done[MAX_DEVICES] = {false};
     const cudaError_t e = raise_smem_limit(grouped_kernel<C, DT>, C::SMEM_BYTES, attr_done);
     if (e != cudaSuccess) { set_last_cuda_error(e); return MXQ_ELAUNCH; }
-    CUtensorMap mx64, mx16;
+    CUtensorMap mx64, mx16, mx8;
     const Groups& g = p.rows;
-    if (!make_map(&mx64, x_codes, g.rows, p.K, 64, C::MXF4) || !make_map(&mx16, x_codes, g.rows, p.K, 16, C::MXF4)) return MXQ_ELAUNCH;
+    if (!make_map(&mx64, x_codes, g.rows, p.K, 64, C::MXF4) || !make_map(&mx16, x_codes, g.rows, p.K, 16, C::MXF4) ||
+        !make_map(&mx8, x_codes, g.rows, p.K, 8, C::MXF4)) return MXQ_ELAUNCH;
     const int64_t units = most_units(g, p.N, C::FEATURES);
-    const int grid = (int)(units < sm_count() ? units : sm_count());
-    return launch_after(grouped_kernel<C, DT>, (unsigned)grid, THREADS, C::SMEM_BYTES, st, mx64, mx16, p);
+    const int64_t room = sm_count() / C::CTAS;
+    return launch_after(grouped_kernel<C, DT>, (unsigned)((units < room ? units : room) * C::CTAS), THREADS, C::SMEM_BYTES, C::CTAS, st, mx64, mx16, mx8, p);
 }
 
 template <class C>
@@ -508,7 +528,7 @@ static bool valid_mx_preset(int eb, int fb) {
 static int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 
 // Kernel and tile width of a call, from the sizes that the host knows.
-enum Shape { DECODE, NARROW, TALL };
+enum Shape { DECODE, NARROW, TALL, PAIR };
 struct Plan {
     Shape shape;                 // the kernel for few rows, where x and its format allow; tiles of up to 128 rows; up to 240 (224 of E2M1 pairs)
     int width;                   // rows per tile at most
@@ -643,6 +663,10 @@ extern "C" int mxq_mx_grouped_linear(const void* x, int x_dtype, int64_t rows_in
     }
     if (rc != MXQ_OK) return rc;
     using namespace grouped;
+    if (plan.shape == PAIR) {
+        p.idesc += (uint32_t)(128 >> 4) << 24;           // 256 features per instruction
+        return fp4 ? launch_dt<PairFp4>(p, x_dtype, codes, st) : launch_dt<Pair>(p, x_dtype, codes, st);
+    }
     if (plan.shape == TALL) return fp4 ? launch_dt<TallFp4>(p, x_dtype, codes, st) : launch_dt<Tall>(p, x_dtype, codes, st);
     return fp4 ? launch_dt<NarrowFp4>(p, x_dtype, codes, st) : launch_dt<Narrow>(p, x_dtype, codes, st);
 }

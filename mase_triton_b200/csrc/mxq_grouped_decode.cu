@@ -50,30 +50,7 @@ struct Source {
     int64_t rows_in;
 };
 
-__device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-    return r;
-}
-__device__ __forceinline__ void cluster_barrier() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 __device__ __forceinline__ void dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-// bounded wait for a phase that other CTAs of the cluster complete
-__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, int* status, int code) {
-    for (uint32_t i = 0; i < SPIN_LIMIT; ++i) {
-        uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-        if (ok) return true;
-        if (i > 64) __nanosleep(32);
-    }
-    if (status) *reinterpret_cast<volatile int*>(status) = code;
-    return false;
-}
 
 // DT: type of x, out, bias and extra; F, OUT: element format of the rows and what the tensor cores read of it
 template <int DT, class F, int OUT>
@@ -363,8 +340,7 @@ decode_kernel(const __grid_constant__ Params p, const __grid_constant__ Source s
                         asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to + j * 128), "r"(v[j]) : "memory");
                     asm volatile("fence.acq_rel.cluster;" ::: "memory");
                     __syncwarp();
-                    if (lane == 0)
-                        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(map_to_rank(parts_bar, (uint32_t)owner)) : "memory");
+                    if (lane == 0) arrive_at(parts_bar, owner);
                     continue;
                 }
                 ok = mbar_wait_cluster(parts_bar, 0, p.status, ST_EPILOGUE_TIMEOUT);
@@ -403,26 +379,12 @@ template <int DT, class F, int OUT>
 static int launch(const Params& p, const Source& src, int split, cudaStream_t st) {
     using C = Cfg<OUT == 5>;
     static bool attr_done[MAX_DEVICES] = {false};
-    cudaError_t e = raise_smem_limit(decode_kernel<DT, F, OUT>, C::smem_bytes(MAX_GROUPS), attr_done);
+    const cudaError_t e = raise_smem_limit(decode_kernel<DT, F, OUT>, C::smem_bytes(MAX_GROUPS), attr_done);
     if (e != cudaSuccess) { set_last_cuda_error(e); return MXQ_ELAUNCH; }
     const int64_t units = most_units(p.rows, p.N, FEATURES), room = 2 * sm_count();
-    cudaLaunchConfig_t cfg = {};
     // a cluster works on one unit; without clusters the CTAs stay and walk over theirs
-    cfg.gridDim = dim3((unsigned)(split > 1 ? units * split : units < room ? units : room));
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = (size_t)C::smem_bytes(p.rows.groups);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned)split;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = split > 1 ? 2 : 1;
-    e = cudaLaunchKernelEx(&cfg, decode_kernel<DT, F, OUT>, p, src, split);
-    if (e != cudaSuccess) { set_last_cuda_error(e); return MXQ_ELAUNCH; }
-    return check_launch();
+    return launch_after(decode_kernel<DT, F, OUT>, (unsigned)(split > 1 ? units * split : units < room ? units : room), THREADS, C::smem_bytes(p.rows.groups),
+                        (unsigned)split, st, p, src, split);
 }
 
 }  // namespace decode
