@@ -157,7 +157,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constan
         for (int u = u_begin; u < walk.total && ok; u += u_step)
             for (int kt = 0; kt < KT && ok; ++kt, at.step()) {
                 ok = mbar_wait(full_bar(at.s), at.phase, p.status, ST_MMA_TIMEOUT);
-                if (ok && elect_one()) arrive_at(peer_full(at.s), 0);
+                if (ok && elect_one()) signal_rank(peer_full(at.s), 0);
                 __syncwarp();
             }
     } else if (warp == 1) {
@@ -192,16 +192,14 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constan
             const uint32_t idesc = p.idesc | ((n >> 3) << 17);
             const int buf = (int)(count & 1u);
             // the first product into an accumulator overwrites it: the epilogue must have read what it held
-            if (count >= 2)
-                ok = CTAS == 2 ? mbar_wait_cluster(accum_empty(buf), ((count >> 1) - 1) & 1, p.status, ST_MMA_TIMEOUT)
-                               : mbar_wait(accum_empty(buf), ((count >> 1) - 1) & 1, p.status, ST_MMA_TIMEOUT);
+            if (count >= 2) ok = mbar_wait(accum_empty(buf), ((count >> 1) - 1) & 1, p.status, ST_MMA_TIMEOUT);
             tc_fence_after();
             const uint32_t d = tmem + buf * C::ACC_STRIDE;
             for (int kt = 0; kt < KT && ok; ++kt, set ^= C::SF_COLS) {
                 const uint32_t st = ring + at.s * C::STAGE_BYTES, empty = empty_bar(at.s);
                 if (!copied) {
                     ok = mbar_wait(full_bar(at.s), at.phase, p.status, ST_MMA_TIMEOUT);
-                    if (CTAS == 2 && ok) ok = mbar_wait_cluster(peer_full(at.s), at.phase, p.status, ST_MMA_TIMEOUT);
+                    if (CTAS == 2 && ok) ok = mbar_wait(peer_full(at.s), at.phase, p.status, ST_MMA_TIMEOUT);
                     tc_fence_after();
                     if (!ok) break;
                     copy_scales(at.s, set, n);
@@ -209,7 +207,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constan
                 copied = false;
                 at.step();
                 if ((kt + 1 < KT || more) && mbar_test_wait(full_bar(at.s), at.phase) &&
-                    (CTAS == 1 || mbar_test_wait_cluster(peer_full(at.s), at.phase))) {
+                    (CTAS == 1 || mbar_test_wait(peer_full(at.s), at.phase))) {
                     tc_fence_after();
                     copy_scales(at.s, set ^ C::SF_COLS, kt + 1 < KT ? n : next_n);
                     copied = true;
@@ -298,7 +296,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constan
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) { if (rank == 0) mbar_arrive(accum_empty(buf)); else arrive_at(accum_empty(buf), 0); }
+            if (lane == 0) { if (rank == 0) mbar_arrive(accum_empty(buf)); else signal_rank(accum_empty(buf), 0); }
         }
         if (p.zero_rest) zero_rows_outside(out, first[0], first[p.rows.groups], p.rows.rows, p.N, threadIdx.x - FIRST_EPI_WARP * 32, EPI_WARPS * 32);
     }
@@ -530,28 +528,31 @@ static int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 // Kernel and tile width of a call, from the sizes that the host knows.
 enum Shape { DECODE, NARROW, TALL, PAIR };
 struct Plan {
-    Shape shape;                 // the kernel for few rows, where x and its format allow; tiles of up to 128 rows; up to 240 (224 of E2M1 pairs)
+    Shape shape;                 // the kernel for few rows, where x and its format allow; tiles of up to 128 rows; up to 240 (224 of E2M1 pairs); these on a pair of CTAs
     int width;                   // rows per tile at most
     int chunks() const { return shape <= NARROW ? 1 : 2; }
     int64_t sf_bytes(int64_t rows, int64_t groups, int64_t K) const { return (rows / width + groups + 1) * ((K + 127) / 128) * chunks() * 512; }
 };
-// The width whose tiles take the fewest estimated cycles of the whole GPU: rounds of tiles x steps of K x the larger of what one thread
-// issues (some 400 cycles) and what L2 gives all SMs together (13.4 TB/s measured: 47.6 KB of a 240-row step in 534 ns on 148 SMs, 33.3 KB
-// of a 128-row step in 364 ns).  Measured widths this picks between, microseconds: 8192 rows, 14336 x 4096: 596 (128 rows), 486 (240);
-// 192 rows, 4096 x 4096: 21.1 (64), 20.0 (128), 22.9 (240); 2048 rows, 2048 x 2048: 33.7 (64), 26.1 (128), 24.9 (240).
-// (Tiles of 256 x 240 have fewer bytes per product, but fill tensor memory: their epilogue overlaps nothing, 544.)
+// The tiles that take the fewest estimated nanoseconds of the whole GPU: rounds of tiles x steps of K x what a step takes.  That is
+// what one thread issues (215) at least; else, for one CTA, what L2 gives all SMs together (13.4 TB/s measured: 47.6 KB of a 240-row step in
+// 534 ns on 148 SMs, 33.3 KB of a 128-row step in 364), for a pair the products and a fixed part (347 at 128 rows, 483 at 224; under the power
+// cap, which large products run into).  Measured, microseconds, one CTA / pair: 8192 rows, 14336 x 4096: 570 / 570 (128 rows), 525 / 477 (192),
+// 482 / 458 (224); 192 rows, 4096 x 4096: 20.6 / 20.0 (64), 19.4 / 19.9 (128); 2048 rows, 2048 x 2048: 25.9 (128), 24.8 (240), 29.8 (pair, 240).
+// (One CTA with 256 x 240 has the pair's bytes, but fills tensor memory: its epilogue overlaps nothing, 544.)
 static Plan make_plan(int64_t rows, int64_t groups, int64_t N, int64_t K, bool fp4) {
     if (groups == 1 ? rows <= decode_rows() : rows / groups <= decode_rows() / 2) return Plan{DECODE, Narrow::BT};
     const int64_t sms = sm_count(), each = (rows + groups - 1) / groups, ftiles = (N + 127) / 128, steps = (K + (fp4 ? 255 : 127)) / (fp4 ? 256 : 128);
     Plan best{NARROW, 0};
     double least = 0.0;
-    for (int width = 48; width <= (fp4 ? TallFp4::BT : Tall::BT); width += 16) {
-        const int64_t per_group = (each + width - 1) / width, units = per_group * groups * ftiles;
-        const double used = (double)(((each + per_group - 1) / per_group + 15) / 16 * 16), busy = units < sms ? (double)units / sms : 1.0;
-        const double step = (17.0 + 0.128 * used) * 11.05 * busy;                     // ns
-        const double cost = (double)((units + sms - 1) / sms * steps) * (step > 215.0 ? step : 215.0);
-        if (best.width == 0 || cost < 0.98 * least) { best = Plan{width <= Narrow::BT ? NARROW : TALL, width}; least = cost; }
-    }
+    for (int ctas = 1; ctas <= 2; ++ctas)
+        for (int width = ctas == 1 ? 48 : 160; width <= (fp4 ? TallFp4::BT : Tall::BT); width += 16) {
+            const int64_t per_group = (each + width - 1) / width, units = per_group * groups * ((ftiles + ctas - 1) / ctas), places = sms / ctas;
+            if (ctas == 2 && units < 4 * places) continue;                // a few rounds: the coarser tiles' last one costs more than they save
+            const double used = (double)(((each + per_group - 1) / per_group + 15) / 16 * 16), busy = units < places ? (double)units / places : 1.0;
+            const double step = ctas == 1 ? (17.0 + 0.128 * used) * 11.05 * busy : 160.0 + 1.4 * used;
+            const double cost = (double)((units + places - 1) / places * steps) * (step > 215.0 ? step : 215.0);
+            if (best.width == 0 || cost < 0.98 * least) { best = Plan{ctas == 2 ? PAIR : width <= Narrow::BT ? NARROW : TALL, width}; least = cost; }
+        }
     return best;
 }
 
