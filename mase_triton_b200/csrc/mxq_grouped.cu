@@ -425,10 +425,10 @@ __global__ void __launch_bounds__(256) pack_rows_kernel(const uint8_t* __restric
     *sf_at = (uint8_t)((any_bad && scale < 255u) ? scale + 1u : scale);
 }
 
-// One pass from x to the operand (built-in round-to-nearest formats, 16-byte aligned rows): 8 elements per lane and access.  One
-// CTA per row segment: the row's group and place are looked up once.
-// Bound by memory (x read once, gathered rows mostly from L2) and integer issue about equally.
-constexpr int QUANT_ACCESSES = 2;                // accesses of 8 elements per lane
+// One pass from x to the operand (built-in round-to-nearest formats, 16-byte aligned rows).  One CTA per row segment: the row's group and
+// place are looked up once.  A lane has four accesses of 8 elements; of the four lanes of a block, lane i derives the header of
+// access i and stores its scale.  Bound by memory (x read once, gathered rows mostly from L2) and integer issue about equally.
+constexpr int QUANT_ACCESSES = 4;                // accesses of 8 elements per lane = lanes of a block
 template <class KIn, class F, int OUT>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restrict__ x, const void* __restrict__ row_index, int index64, int64_t rows_in,
                                                             const Groups g, const RowOperand o_, int segments, int early) {
@@ -458,21 +458,35 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restri
     }
     const Place place = find_row(g, row, s_two);
     if (place.slot < 0) return;
+    const int lane = threadIdx.x & 31, sub = lane & 3;
+    uint32_t hi[QUANT_ACCESSES], lo[QUANT_ACCESSES];
 #pragma unroll
     for (int a = 0; a < QUANT_ACCESSES; ++a) {
-        const int k = first + a * (int)blockDim.x * 8;
+        part_range<KIn, 8>(raw[a], hi[a], lo[a]);
+        hi[a] = part_reduce<KIn, 8>(hi[a]);
+    }
+    uint32_t mine = hi[0];
+#pragma unroll
+    for (int a = 1; a < QUANT_ACCESSES; ++a) mine = sub == a ? hi[a] : mine;
+    const uint2 header = part_header<KIn, F>(mine);
+    uint32_t scale = 0u;
+#pragma unroll
+    for (int a = 0; a < QUANT_ACCESSES; ++a) {
+        const int k = first + a * (int)blockDim.x * 8, from_lane = (lane & ~3) + a;
         uint32_t o[OUT == 5 ? 1 : 2];
-        const uint32_t sbyte = quantise_part<KIn, F, OUT, 8>(raw[a], o);
+        const uint2 of_block = make_uint2(__shfl_sync(~0u, header.x, from_lane), __shfl_sync(~0u, header.y, from_lane));
+        const uint32_t sbyte = part_encode<KIn, F, OUT, 8>(raw[a], lo[a], of_block, o);
+        scale = sub == a ? sbyte : scale;
         if (k < K) {
             if constexpr (OUT == 5) *reinterpret_cast<uint32_t*>(o_.codes + ((int64_t)row * K + k) / 2) = o[0];
             else *reinterpret_cast<uint2*>(o_.codes + (int64_t)row * K + k) = make_uint2(o[0], o[1]);
-            if ((threadIdx.x & 3) == 0) {
-                const int kb = k >> 5;
-                uint8_t* at = o_.sf + place.at(kb, (K + 127) / 128, o_.chunks);
-                *at = (uint8_t)sbyte;
-                if (k + 32 == K) for (int i = 1; i < 4 - (kb & 3); ++i) at[i] = 127;     // K blocks that only fill up the last 128 elements
-            }
         }
+    }
+    const int kb = (first + sub * (int)blockDim.x * 8) >> 5;                     // the block of access `sub`
+    if (kb * 32 < K) {
+        uint8_t* at = o_.sf + place.at(kb, (K + 127) / 128, o_.chunks);
+        *at = (uint8_t)scale;
+        if (kb * 32 + 32 == K) for (int i = 1; i < 4 - (kb & 3); ++i) at[i] = 127;     // K blocks that only fill up the last 128 elements
     }
     if (!early) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }

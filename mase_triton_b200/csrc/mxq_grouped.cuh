@@ -157,52 +157,76 @@ template <class F> __device__ __forceinline__ uint32_t widen_codes4(uint32_t w) 
     }
 }
 
-// E (8 or 16) elements of a 32-element block per lane, as they lie in memory (the 32 / E lanes of the block are neighbours) -> the
-// tensor cores' codes, and the block's scale byte as the result.  The lanes agree on the block's maximum by shuffles and every lane
-// derives the scale; bf16 inputs take the packed quantisers, the 8-bit element formats their short form where no element of the warp lies
-// below its block's normal range (so lanes without a row should hold ones, not zeros).  A block with a code that the hardware reads
-// as Inf / NaN becomes (scale + 1, elements / 2).  All lanes of the warp take part.
-// OUT: 0 = E4M3 bytes, 1 = E5M2 bytes, 5 = E2M1 nibbles.
-template <class KIn, class F, int OUT, int E>
-__device__ __forceinline__ uint32_t quantise_part(const uint32_t (&raw)[E * KIn::size / 4], uint32_t (&codes)[OUT == 5 ? E / 8 : E / 4]) {
-    const F f{};
-    constexpr int LANES = 32 / E;
-    uint32_t o[E / 4], sbyte;
-    bool special;
+// Quantising E (8 or 16) elements of a 32-element block per lane, as they lie in memory (the 32 / E lanes of the block are neighbours),
+// in four steps, so that a kernel with several blocks per lane can derive each block's header on one lane only.
+// Range of the lane's magnitudes: bf16 -- packed pairs of the largest and the smallest, else fp32 bits.
+template <class KIn, int E> __device__ __forceinline__ void part_range(const uint32_t (&raw)[E * KIn::size / 4], uint32_t& hi, uint32_t& lo) {
     if constexpr (std::is_same<KIn, KBF16>::value) {
-        uint32_t mx2, mn2;
-        Pack<16> p[E / 8];
 #pragma unroll
         for (int i = 0; i < E / 8; ++i) {
-            uint32_t hi, lo;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) p[i].w[j] = raw[4 * i + j];
-            bf16_abs_range(p[i], hi, lo);
-            mx2 = i == 0 ? hi : bf2_bits(__hmax2_nan(bf2(mx2), bf2(hi)));
-            mn2 = i == 0 ? lo : bf2_bits(__hmin2(bf2(mn2), bf2(lo)));
+            const Pack<16> p{{raw[4 * i], raw[4 * i + 1], raw[4 * i + 2], raw[4 * i + 3]}};
+            uint32_t h, l;
+            bf16_abs_range(p, h, l);
+            hi = i == 0 ? h : bf2_bits(__hmax2_nan(bf2(hi), bf2(h)));
+            lo = i == 0 ? l : bf2_bits(__hmin2(bf2(lo), bf2(l)));
         }
-#pragma unroll
-        for (int d = 1; d < LANES; d <<= 1) mx2 = bf2_bits(__hmax2_nan(bf2(mx2), bf2(__shfl_xor_sync(~0u, mx2, d))));
-        const uint32_t header = block_header_bf16(bf16x2_max_bits(mx2), f), word = bf16_block_word<F>(header);
-#pragma unroll
-        for (int i = 0; i < E / 8; ++i) bf16_quantise_access<F, false>(p[i], word, mn2, header, 0u, o + 2 * i);
-        sbyte = (header >> 8) & 0xFFu;
-        special = header & 1u;
     } else {
-        uint32_t b[E], amax = 0, amin = ~0u;
+        hi = 0u;
+        lo = ~0u;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-            if constexpr (KIn::size == 4) b[i] = raw[i];
-            else b[i] = KIn::to_bits(i & 1 ? raw[i >> 1] >> 16 : raw[i >> 1] & 0xFFFFu);
-            amax = max(amax, b[i] & 0x7FFFFFFFu);
-            amin = min(amin, b[i] & 0x7FFFFFFFu);
+            const uint32_t m = (KIn::size == 4 ? raw[i * KIn::size / 4] : KIn::to_bits(i & 1 ? raw[i >> 1] >> 16 : raw[i >> 1] & 0xFFFFu)) & 0x7FFFFFFFu;
+            hi = max(hi, m);
+            lo = min(lo, m);
         }
+    }
+}
+// the block's largest magnitude, on all its lanes
+template <class KIn, int E> __device__ __forceinline__ uint32_t part_reduce(uint32_t hi) {
 #pragma unroll
-        for (int d = 1; d < LANES; d <<= 1) amax = max(amax, __shfl_xor_sync(~0u, amax, d));
-        const uint32_t header = block_header(amax, f);
-        const float inv = __uint_as_float(header & 0x7F800000u);
+    for (int d = 1; d < 32 / E; d <<= 1) {
+        const uint32_t other = __shfl_xor_sync(~0u, hi, d);
+        if constexpr (std::is_same<KIn, KBF16>::value) hi = bf2_bits(__hmax2_nan(bf2(hi), bf2(other)));
+        else hi = max(hi, other);
+    }
+    return hi;
+}
+// the block's header (2^-se, scale byte, whether it holds Inf / NaN) and a second word: what the packed bf16 quantisers share, else the
+// bound of the short form
+template <class KIn, class F> __device__ __forceinline__ uint2 part_header(uint32_t hi) {
+    const F f{};
+    if constexpr (std::is_same<KIn, KBF16>::value) {
+        const uint32_t header = block_header_bf16(bf16x2_max_bits(hi), f);
+        return make_uint2(header, bf16_block_word<F>(header));
+    } else {
+        const uint32_t header = block_header(hi, f);
+        uint32_t bound = 0u;
+        if constexpr (PkFmt<F>::RARE_SUBRANGE) bound = short_form_limit_bits<F>(header);
+        return make_uint2(header, bound);
+    }
+}
+// The tensor cores' codes, and the block's scale byte as the result.  bf16 inputs take the packed quantisers, the 8-bit element formats
+// their short form where no element of the warp lies below its block's normal range (so lanes without a row should hold
+// ones, not zeros).  A block with a code that the hardware reads as Inf / NaN becomes (scale + 1, elements / 2).
+// OUT: 0 = E4M3 bytes, 1 = E5M2 bytes, 5 = E2M1 nibbles.
+template <class KIn, class F, int OUT, int E>
+__device__ __forceinline__ uint32_t part_encode(const uint32_t (&raw)[E * KIn::size / 4], uint32_t lo, uint2 header, uint32_t (&codes)[OUT == 5 ? E / 8 : E / 4]) {
+    const F f{};
+    uint32_t o[E / 4], sbyte = (header.x >> 8) & 0xFFu;
+    const bool special = header.x & 1u;
+    if constexpr (std::is_same<KIn, KBF16>::value) {
+#pragma unroll
+        for (int i = 0; i < E / 8; ++i) {
+            const Pack<16> p{{raw[4 * i], raw[4 * i + 1], raw[4 * i + 2], raw[4 * i + 3]}};
+            bf16_quantise_access<F, false>(p, header.y, lo, header.x, 0u, o + 2 * i);
+        }
+    } else {
+        uint32_t b[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) b[i] = KIn::size == 4 ? raw[i * KIn::size / 4] : KIn::to_bits(i & 1 ? raw[i >> 1] >> 16 : raw[i >> 1] & 0xFFFFu);
+        const float inv = __uint_as_float(header.x & 0x7F800000u);
         bool short_form = false;
-        if constexpr (PkFmt<F>::RARE_SUBRANGE) short_form = !__any_sync(~0u, amin < short_form_limit_bits<F>(header));
+        if constexpr (PkFmt<F>::RARE_SUBRANGE) short_form = !__any_sync(~0u, lo < header.y);
         if (short_form) {
             if constexpr (PkFmt<F>::RARE_SUBRANGE) {
 #pragma unroll
@@ -218,8 +242,6 @@ __device__ __forceinline__ uint32_t quantise_part(const uint32_t (&raw)[E * KIn:
 #pragma unroll
             for (int i = 0; i < E / 4; ++i) o[i] = pack4_codes(mag + 4 * i, qb + 4 * i, f);
         }
-        sbyte = (header >> 8) & 0xFFu;
-        special = header & 1u;
     }
     if constexpr (F{}.eb() >= 4) {
         // carry out of the magnitude byte: a code the hardware reads as Inf / NaN
@@ -228,7 +250,7 @@ __device__ __forceinline__ uint32_t quantise_part(const uint32_t (&raw)[E * KIn:
 #pragma unroll
         for (int i = 0; i < E / 4; ++i) bad |= ((o[i] & 0x7F7F7F7Fu) + probe) & 0x80808080u;
 #pragma unroll
-        for (int d = 1; d < LANES; d <<= 1) bad |= __shfl_xor_sync(~0u, bad, d);
+        for (int d = 1; d < 32 / E; d <<= 1) bad |= __shfl_xor_sync(~0u, bad, d);
         if (bad != 0u) {
 #pragma unroll
             for (int i = 0; i < E / 4; ++i) o[i] = halve_codes4<F{}.fb()>(o[i]);
@@ -250,6 +272,13 @@ __device__ __forceinline__ uint32_t quantise_part(const uint32_t (&raw)[E * KIn:
         }
     }
     return special ? 255u : sbyte;                                       // 255 is NaN to the tensor cores, whatever the codes
+}
+// all four steps; all lanes of the warp take part
+template <class KIn, class F, int OUT, int E>
+__device__ __forceinline__ uint32_t quantise_part(const uint32_t (&raw)[E * KIn::size / 4], uint32_t (&codes)[OUT == 5 ? E / 8 : E / 4]) {
+    uint32_t hi, lo;
+    part_range<KIn, E>(raw, hi, lo);
+    return part_encode<KIn, F, OUT, E>(raw, lo, part_header<KIn, F>(part_reduce<KIn, E>(hi)), codes);
 }
 
 // fn(F, the operand's format) for a built-in round-to-nearest format; `nibbles`: E2M1 stays packed in four bits
