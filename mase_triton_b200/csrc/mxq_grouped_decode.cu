@@ -338,8 +338,7 @@ decode_kernel(const __grid_constant__ Params p, const __grid_constant__ Source s
 #pragma unroll
                     for (int j = 0; j < 16; ++j)
                         asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to + j * 128), "r"(v[j]) : "memory");
-                    asm volatile("fence.acq_rel.cluster;" ::: "memory");
-                    __syncwarp();
+                    __syncwarp();                                                        // the warp's stores, then their release by one lane
                     if (lane == 0) arrive_at(parts_bar, owner);
                     continue;
                 }

@@ -31,6 +31,16 @@ class PackedExperts:
 
     def __post_init__(self):
         self.device_index, self.pointer = self.blocks.get_device(), self.blocks.data_ptr()
+        self._row_formats: dict[MXFPMeta, tuple[int, int, int]] = {}
+
+    def row_format(self, x_meta: MXFPMeta) -> tuple[int, int, int]:
+        """Exponent bits, fraction bits and rounding mode of an activation format that goes with these weights."""
+        known = self._row_formats.get(x_meta)
+        if known is None:
+            if not supported(x_meta) or (self.hw_format == 5 and not is_e2m1(x_meta)):
+                raise ValueError(f"the weight was packed for another activation format than {x_meta}")
+            known = self._row_formats[x_meta] = (x_meta.element_exp_bits, x_meta.element_frac_bits, _lib.ROUND_ID[x_meta.round_mode])
+        return known
 
 
 def check_formats(x_meta: MXFPMeta | None, w_meta: MXFPMeta | None, K: int) -> None:
@@ -115,8 +125,7 @@ def grouped_linear(x: Tensor, x_meta: MXFPMeta, w: PackedExperts, offsets: Tenso
         raise ValueError(f"input dtype {dtype}: one of {[str(d) for d in _lib.DTYPE_ID]}")
     if x.ndim != 2 or x.shape[1] != K:
         raise ValueError(f"input of shape {tuple(x.shape)}: expected [tokens, {K}]")
-    if not supported(x_meta) or (w.hw_format == 5 and not is_e2m1(x_meta)):
-        raise ValueError(f"the weight was packed for another activation format than {x_meta}")
+    exp_bits, frac_bits, round_id = w.row_format(x_meta)
     if w.device_index != dev:
         raise ValueError(f"the weight is on {w.blocks.device}, the input on {x.device}")
     x = x.contiguous()
@@ -161,11 +170,11 @@ def grouped_linear(x: Tensor, x_meta: MXFPMeta, w: PackedExperts, offsets: Tenso
         return out
     status = status_address(dev)
     L = _lib.load()
-    x_ptr, round_id = x.data_ptr(), _lib.ROUND_ID[x_meta.round_mode]
+    x_ptr = x.data_ptr()
     nbytes = L.mxq_mx_grouped_scratch_bytes(x_ptr, round_id, tokens, rows, K, groups, N)
     # of this call alone: two captured graphs, or two streams, never share it
-    scratch = None if nbytes == 0 else torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-    args = (x_ptr, dtype_id, tokens, rows, K, x_meta.element_exp_bits, x_meta.element_frac_bits, round_id, index_ptr, index64, w.pointer, w.hw_format, groups,
+    scratch = None if nbytes == 0 else x.new_empty(nbytes // x.element_size())           # (a multiple of 256 bytes)
+    args = (x_ptr, dtype_id, tokens, rows, K, exp_bits, frac_bits, round_id, index_ptr, index64, w.pointer, w.hw_format, groups,
             N, offsets_ptr, offsets64, out.data_ptr(), bias_ptr, act, extra_ptr, extra_mode, zero_rest,
             None if scratch is None else scratch.data_ptr(), nbytes, status, _lib.raw_stream(dev))
     if torch.cuda.current_device() == dev:

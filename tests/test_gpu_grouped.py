@@ -203,6 +203,33 @@ def test_grouped_formats(lib, counts, pair):
     check(got, *grouped_expected(dequant(x, x_meta), wq, b, first, counts, "silu", m, None, torch.bfloat16, torch.zeros_like(m)))
 
 
+@pytest.mark.parametrize("pair", [(MXFP8_E4M3_fn, OCP_MXFP6_E2M3, 160), (MXFP8_E5M2_fn, MXFP8_E4M3_fn, 640), (OCP_MXFP4_E2M1, OCP_MXFP4_E2M1, 1280)],
+                         ids=lambda p: f"{p[0].tag}-{p[1].tag}-{p[2]}")
+@pytest.mark.parametrize("N", [8192, 7873])
+def test_many_tiles(lib, pair, N):
+    """Sizes with several rounds of tiles on every SM: the widest tiles, and those of pairs of CTAs, whole and with the last of
+    the features and rows missing; a row's result is that of the kernel for few rows within what their orders of summation differ."""
+    x_meta, w_meta, K = pair
+    layer, wq, b = linear_layer(N, K, x_meta, w_meta, bias=True)
+    x, m = rand(2500, K), rand(2500, N, seed=1)
+    y = layer(x, activation="silu", multiplier=m)
+    check(y, *expected(dequant(x, x_meta), wq, b, "silu", m, None, torch.bfloat16))
+    counts = [1200, 0, 1, 2000, 700, 16]
+    grouped, wq, b, x = grouped_case(counts, N // 4, K, x_meta, w_meta)
+    r = rand(sum(counts), N // 4, seed=2)
+    first = [sum(counts[:i]) for i in range(len(counts))]
+    check(grouped(x, offsets_of(counts), residual=r), *grouped_expected(dequant(x, x_meta), wq, b, first, counts, None, None, r, torch.bfloat16, torch.zeros_like(r)))
+    G.check_status(DEV)
+
+
+@pytest.mark.parametrize("M,N,K", [(300, 1024, 1024), (1000, 2048, 512), (2000, 640, 2080)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_middle_sizes(lib, M, N, K, dtype):
+    layer, wq, b = linear_layer(N, K, MXFP8_E4M3_fn, MXFP8_E4M3_fn, dtype, bias=True)
+    x, r = rand(M, K, dtype=dtype), rand(M, N, dtype=dtype, seed=1)
+    check(layer(x, activation="gelu_tanh", residual=r), *expected(dequant(x, MXFP8_E4M3_fn), wq, b, "gelu_tanh", None, r, dtype))
+
+
 @pytest.mark.parametrize("start,pad", [(0, 37), (5, 0), (300, 131)])
 def test_rows_outside_the_groups(lib, start, pad):
     counts = [20, 0, 150, 3]
