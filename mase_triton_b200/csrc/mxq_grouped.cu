@@ -26,7 +26,7 @@
 namespace mxq {
 namespace grouped {
 
-constexpr int EPI_WARPS = 8;                     // two per TMEM lane quadrant
+constexpr int EPI_SIDES = 3, EPI_WARPS = 4 * EPI_SIDES;          // epilogue warps: three per TMEM lane quadrant
 constexpr int FIRST_EPI_WARP = 4;                // warps 0, 1, 3: weight copies, MMA issuer, row copies
 constexpr int THREADS = (FIRST_EPI_WARP + EPI_WARPS) * 32;
 
@@ -54,12 +54,12 @@ template <int BT_, int STAGES_, bool MXF4_, int CTAS_ = 1> struct Cfg {
     static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + TABLE_END + EPI_WARPS * 2048;
     static_assert(SMEM_BYTES <= 232448, "more shared memory than a CTA can have");
 };
-using Narrow = Cfg<128, 6, false>;
+using Narrow = Cfg<128, 5, false>;
 using NarrowFp4 = Cfg<128, 5, true>;
 using Tall = Cfg<240, 4, false>;
 using TallFp4 = Cfg<224, 4, true>;
-using Pair = Cfg<240, 6, false, 2>;
-using PairFp4 = Cfg<224, 6, true, 2>;
+using Pair = Cfg<240, 5, false, 2>;
+using PairFp4 = Cfg<224, 5, true, 2>;
 
 template <class C, int DT>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -219,8 +219,8 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constan
                     for (uint32_t k = 0; k < 4; ++k) {
                         const uint32_t acc = (kt > 0 || k > 0) ? 1u : 0u;
                         // scale byte k of a column; 64 elements of 4-bit pairs: bytes (0, 1) or (2, 3) of step k / 2
-                            const uint32_t id = C::MXF4 ? (k & 1u) * 2u : k, step = C::MXF4 ? 8 * (k >> 1) : 0u;
-                            tc_mma<CTAS, C::MXF4>(d, w_desc + 2 * k, x_desc + 2 * k, idesc | (id << 29) | (id << 4), sfw + step, sfx + step, acc);
+                        const uint32_t id = C::MXF4 ? (k & 1u) * 2u : k, step = C::MXF4 ? 8 * (k >> 1) : 0u;
+                        tc_mma<CTAS, C::MXF4>(d, w_desc + 2 * k, x_desc + 2 * k, idesc | (id << 29) | (id << 4), sfw + step, sfx + step, acc);
                     }
                     tc_commit<CTAS>(empty);                                             // frees the stage once these products have read it
                 }
@@ -242,7 +242,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constan
         // (fp32: 128-byte) segments.  The second operand of the next 16 rows is requested before the current ones are worked on, that of a
         // tile's first ones before the accumulator is complete.
         typedef typename Elem<DT>::T T;
-        const int q = warp & 3, side = (warp - FIRST_EPI_WARP) >> 2;      // lane quadrant; the two warps of one take 16-row chunks in turn
+        const int q = warp & 3, side = (warp - FIRST_EPI_WARP) >> 2;      // lane quadrant; the warps of one take 16-row chunks in turn
         const int er = lane >> 3, ef = q * 32 + (lane & 7) * 4;           // this lane's row (of every four) and first feature
         float* slot = reinterpret_cast<float*>(ring_ptr + STAGES * C::STAGE_BYTES + C::TABLE_END) + (warp - FIRST_EPI_WARP) * 512;
         T* out = reinterpret_cast<T*>(p.out);
@@ -278,7 +278,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constan
             ok = mbar_wait(accum_full(buf), (count >> 1) & 1, p.status, ST_EPILOGUE_TIMEOUT);
             tc_fence_after();
             if (!ok) break;
-            for (int c = side; c < chunks; c += 2) {
+            for (int c = side; c < chunks; c += EPI_SIDES) {
                 uint32_t r[32];
                 tmem_ld_32x32b_x16(tmem + ((uint32_t)(q * 32) << 16) + buf * C::ACC_STRIDE + c * 16, r);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -288,7 +288,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constan
                 Four<T> now[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) now[i].w = e[i].w;
-                if (c + 2 < chunks) request(c + 2);
+                if (c + EPI_SIDES < chunks) request(c + EPI_SIDES);
                 T* at = out + (size_t)(t.row + c * 16 + er) * p.N + f;
                 const int rows = (t.rows - c * 16 - er + 3) >> 2, left = p.N - f;
                 finish_any(p.act, slot, lane, bias, now, p.extra_mode, at, p.N, rows, left, p.vector);
@@ -430,10 +430,11 @@ __global__ void __launch_bounds__(256) pack_rows_kernel(const uint8_t* __restric
 // access i and stores its scale.  Bound by memory (x read once, gathered rows mostly from L2) and integer issue about equally.
 constexpr int QUANT_ACCESSES = 4;                // accesses of 8 elements per lane = lanes of a block
 template <class KIn, class F, int OUT>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restrict__ x, const void* __restrict__ row_index, int index64, int64_t rows_in,
-                                                            const Groups g, const RowOperand o_, int segments, int early) {
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const void* x, const void* row_index, int index64, int64_t rows_in, const Groups g,
+                                                            const RowOperand o_, int segments, int early) {
     __shared__ int s_two[2];
     // everything before this kernel has completed; then the product may start: until it waits for this kernel it only reads what is older
+    // (what an earlier kernel may still be writing when this one starts is not loaded as read-only data: such loads could move in front)
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (early) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     constexpr int BYTES = 8 * KIn::size;
@@ -452,7 +453,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restri
         const int k = first + a * (int)blockDim.x * 8;
 #pragma unroll
         for (int i = 0; i < BYTES / 16; ++i) {
-            const uint4 v = there && k < K ? __ldg(reinterpret_cast<const uint4*>(from + (int64_t)k * KIn::size) + i) : make_uint4(fill, fill, fill, fill);
+            const uint4 v = there && k < K ? __ldcg(reinterpret_cast<const uint4*>(from + (int64_t)k * KIn::size) + i) : make_uint4(fill, fill, fill, fill);
             raw[a][4 * i] = v.x; raw[a][4 * i + 1] = v.y; raw[a][4 * i + 2] = v.z; raw[a][4 * i + 3] = v.w;
         }
     }
@@ -499,8 +500,8 @@ static int quantize_rows(const void* x, int x_dtype, const void* row_index, int 
     const int block = lanes >= 256 ? 256 : (int)((lanes + 31) / 32 * 32);
     const int64_t segments = (K / 8 + (int64_t)block * QUANT_ACCESSES - 1) / ((int64_t)block * QUANT_ACCESSES);
     if (rm != MXQ_RN || reinterpret_cast<uintptr_t>(x) % 16 != 0 || rows * segments > (1ll << 31) - 1) return MXQ_ESIZE;
-    // a grid of one wave lets the product's CTAs come up beside it; a longer one keeps the SMs' registers to itself until its end
-    const int early = rows * segments <= 2 * sm_count();
+    // a short grid lets the product's CTAs come up beside it (777 rows: 15.1 -> 14.4 us the call); a long one keeps the SMs' registers to itself until its end
+    const int early = rows * segments <= 32 * sm_count();
     int rc = MXQ_ESIZE;
     with_kind(x_dtype, [&](auto kin) {
         using KIn = decltype(kin);

@@ -141,6 +141,7 @@ decode_kernel(const __grid_constant__ Params p, const __grid_constant__ Source s
         bool ok = true, copied = false;
         RingAt<STAGES> at;
         constexpr uint32_t SF_COLS = C::SF_STEPS * 8;
+        dependency_wait();                                           // not in a bounded wait while the kernel before this one runs
         const uint32_t idesc = p.idesc | ((uint32_t)(ROWS >> 3) << 17);
         auto copy_scales = [&](int s, uint32_t into) {
             const uint32_t from = ring + s * C::STAGE_BYTES, sfw = tmem + SFW_COL + into, sfx = tmem + SFX_COL + into;
@@ -244,7 +245,7 @@ decode_kernel(const __grid_constant__ Params p, const __grid_constant__ Source s
                     const uint32_t fill = from[i0 + i] == -2 ? one_bits<KIn>() : 0u;
                     uint4 q = make_uint4(fill, fill, fill, fill);
                     if (from[i0 + i] >= 0 && k < p.K)
-                        q = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(src.x) + (int64_t)from[i0 + i] * p.K + k) + j / 4);
+                        q = __ldcg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(src.x) + (int64_t)from[i0 + i] * p.K + k) + j / 4);
                     w[i][j] = q.x; w[i][j + 1] = q.y; w[i][j + 2] = q.z; w[i][j + 3] = q.w;
                 }
         };
