@@ -23,8 +23,7 @@ class PTQLinearBase(nn.Module):
     in_features: int
     out_features: int
 
-    # the quantised weight as the products with an epilogue read it (mxfp.grouped), and the versions of the codes it was
-    # built from; built on first use
+    # the quantised weight as the products with an epilogue read it, and what it was built from (mxfp.grouped.kept_weight)
     _row_weight = None
 
     def __getstate__(self):

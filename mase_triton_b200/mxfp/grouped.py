@@ -51,11 +51,15 @@ def check_formats(x_meta: MXFPMeta | None, w_meta: MXFPMeta | None, K: int) -> N
         raise ValueError(f"in_features has to be a positive multiple of 32: got {K}")
 
 
-def pack_experts(w_scales: Tensor, w_elements: Tensor, groups: int, N: int, K: int, w_meta: MXFPMeta, x_meta: MXFPMeta) -> PackedExperts:
+def pack_experts(w_scales: Tensor, w_elements: Tensor, groups: int, N: int, K: int, w_meta: MXFPMeta, x_meta: MXFPMeta,
+                 into: PackedExperts | None = None) -> PackedExperts:
     """Reference ``(scales, elements)`` of a ``[groups, N, K]`` weight with blocks along K, for activations of ``x_meta``
-    (an MXFP4 pair with K a multiple of 256 keeps packed nibbles and runs on the 4-bit x 4-bit tensor-core kind)."""
+    (an MXFP4 pair with K a multiple of 256 keeps packed nibbles and runs on the 4-bit x 4-bit tensor-core kind).
+    ``into``: an earlier result whose memory is taken again where it fits."""
     _lib.require_cuda(w_elements, "pack_experts")
     check_formats(x_meta, w_meta, K)
+    if groups <= 0 or N <= 0:
+        raise ValueError(f"a weight of shape [{groups}, {N}, {K}] has no entries")
     if w_elements.dtype != torch.uint8 or w_scales.dtype != torch.uint8:
         raise ValueError(f"weight codes and scales have to be uint8: got {w_elements.dtype} and {w_scales.dtype}")
     if w_elements.numel() != groups * N * K or w_scales.numel() != groups * N * K // 32:
@@ -69,13 +73,34 @@ def pack_experts(w_scales: Tensor, w_elements: Tensor, groups: int, N: int, K: i
     w_scales, w_elements = w_scales.contiguous(), w_elements.contiguous()
     if w_elements.data_ptr() % 16 != 0:
         w_elements = w_elements.clone()
-    blocks = torch.empty(L.mxq_mx_packed_experts_bytes(groups, N, K, int(nibbles)), dtype=torch.uint8, device=dev)
+    nbytes = L.mxq_mx_packed_experts_bytes(groups, N, K, int(nibbles))
+    blocks = into.blocks if into is not None and into.blocks.numel() == nbytes and into.blocks.device == dev else \
+        torch.empty(nbytes, dtype=torch.uint8, device=dev)
     fmt = ctypes.c_int(0)
     with torch.cuda.device(dev):
         rc = L.mxq_mx_pack_experts(w_scales.data_ptr(), w_elements.data_ptr(), groups, N, K, w_meta.element_exp_bits, w_meta.element_frac_bits,
                                    int(nibbles), blocks.data_ptr(), ctypes.addressof(fmt), _lib.stream_ptr(dev))
     _lib.check(rc, "mxq_mx_pack_experts")
     return PackedExperts(blocks, fmt.value, groups, N, K)
+
+
+def kept_weight(layer, groups: int, N: int, K: int) -> PackedExperts:
+    """The packed weight of a layer (``w_scales``, ``w_elements``, ``w_tensor_meta``, ``x_mxfp_meta``), kept with it until its code tensors
+    are written, replaced or moved.  It is packed anew into the same memory, so that a captured graph finds it there, and before
+    this returns it is complete for every stream.  While a graph is captured nothing is kept: packing is then part of the graph."""
+    w_scales, w_elements, kept = layer.w_scales, layer.w_elements, layer._row_weight
+    state = (w_elements._version, w_scales._version, w_elements.data_ptr(), w_scales.data_ptr())
+    if kept is not None and kept[0] is w_elements and kept[1] is w_scales and kept[2] is layer.w_tensor_meta and kept[3] is layer.x_mxfp_meta and kept[4] == state:
+        return kept[5]
+    _lib.require_cuda(w_elements, "pack_experts")
+    with torch.cuda.device(w_elements.device):
+        capturing = torch.cuda.is_current_stream_capturing()
+        packed = pack_experts(w_scales.data, w_elements.data, groups, N, K, layer.w_tensor_meta.meta, layer.x_mxfp_meta,
+                              None if kept is None or capturing else kept[5])
+        if not capturing:
+            torch.cuda.current_stream().synchronize()
+            layer._row_weight = (w_elements, w_scales, layer.w_tensor_meta, layer.x_mxfp_meta, state, packed)
+    return packed
 
 
 def epilogue_operand(multiplier: Tensor | None, residual: Tensor | None) -> tuple[Tensor | None, int]:
@@ -164,6 +189,10 @@ def grouped_linear(x: Tensor, x_meta: MXFPMeta, w: PackedExperts, offsets: Tenso
             raise _operand_error(out, "out", (rows, N), x)
         if not out.is_contiguous():
             raise ValueError("out has to be contiguous")
+        begin, end = out.data_ptr(), out.data_ptr() + out.nbytes
+        for t, name in ((x, "input"), (offsets, "offsets"), (row_index, "row_index"), (bias, "bias"), (extra, "multiplier or residual")):
+            if t is not None and t.data_ptr() < end and begin < t.data_ptr() + t.nbytes and not (t is extra and t.data_ptr() == begin):
+                raise ValueError(f"out overlaps the {name}, which other rows of the result are still computed from")
         if not out.is_inference():
             torch.autograd.graph.increment_version(out)
     if rows == 0:

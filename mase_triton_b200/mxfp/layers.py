@@ -111,16 +111,10 @@ class MXFPLinearPTQ(PTQLinearBase):
         return _gemm.PackedOperand(self._tc_codes, self._tc_sf, self._tc_info[1], n, k, _gemm.OPERAND_B, self._tc_info[2])
 
     def row_weight(self):
-        """The quantised weight as the product with an epilogue reads it (``mxfp.grouped``), kept with the module and rebuilt when
-        the code tensors were written or moved."""
-        w_scales, w_elements = self.w_scales, self.w_elements
-        if self._row_weight is None or self._row_weight[:2] != (w_elements._version, w_scales._version):
-            from . import grouped as _grouped
+        """The quantised weight as the product with an epilogue reads it; see ``mxfp.grouped.kept_weight``."""
+        from . import grouped as _grouped
 
-            n, k = self.w_tensor_meta.shape
-            self._row_weight = (w_elements._version, w_scales._version,
-                                _grouped.pack_experts(w_scales.data, w_elements.data, 1, n, k, self.w_tensor_meta.meta, self.x_mxfp_meta))
-        return self._row_weight[2]
+        return _grouped.kept_weight(self, 1, self.out_features, self.in_features)
 
     def export_packed(self) -> dict:
         """A ``torch.save``-able dict holding this layer with its element codes bit-packed to their true width
@@ -275,15 +269,10 @@ class MXFPGroupedLinearPTQ(PTQLinearBase):
         return cls(w_scales, w_elements, w_tensor_meta, bias, x_mxfp_meta)
 
     def row_weight(self):
-        """The weights as the kernel reads them, kept with the module and rebuilt when the code tensors were written or moved."""
-        w_scales, w_elements = self.w_scales, self.w_elements
-        if self._row_weight is None or self._row_weight[:2] != (w_elements._version, w_scales._version):
-            from . import grouped as _grouped
+        """The weights as the kernel reads them; see ``mxfp.grouped.kept_weight``."""
+        from . import grouped as _grouped
 
-            self._row_weight = (w_elements._version, w_scales._version,
-                                _grouped.pack_experts(w_scales.data, w_elements.data, self.groups, self.out_features, self.in_features,
-                                                      self.w_tensor_meta.meta, self.x_mxfp_meta))
-        return self._row_weight[2]
+        return _grouped.kept_weight(self, self.groups, self.out_features, self.in_features)
 
     def forward(self, input: Tensor, offsets: Tensor, activation: str | None = None, multiplier: Tensor | None = None,
                 residual: Tensor | None = None, row_index: Tensor | None = None, out: Tensor | None = None) -> Tensor:

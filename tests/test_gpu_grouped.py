@@ -506,6 +506,103 @@ def test_layer_follows_its_codes(lib):
     assert torch.equal(stacked(x, offsets_of(counts), residual=r)[5:], one(x[5:], residual=r[5:]))
 
 
+def test_replaced_code_tensors(lib):
+    """A new Parameter counts its versions anew: what the layer has packed is told apart by more than those."""
+    counts = [5, 6]
+    off = offsets_of(counts)
+    layer, _, _, x = grouped_case(counts, 64, 64, MXFP8_E4M3_fn, MXFP8_E4M3_fn, bias=False)
+    other = MXFPGroupedLinearPTQ.from_weight(rand(2, 64, 64, seed=31), None, MXFP8_E4M3_fn, MXFP8_E4M3_fn)
+    want = other(x, off)
+    assert not torch.equal(layer(x, off), want)
+    layer.load_state_dict(other.state_dict(), assign=True)
+    assert torch.equal(layer(x, off), want)
+    layer.w_elements = torch.nn.Parameter(torch.zeros_like(other.w_elements), requires_grad=False)
+    assert not layer(x, off).any()
+    layer.w_elements.data = other.w_elements.data.clone()
+    assert torch.equal(layer(x, off), want)
+
+
+def test_first_call_on_another_stream(lib):
+    """What a layer packs in its first call is complete for every stream, whatever the first one is busy with."""
+    layer, _, _, x = grouped_case([5, 200], 256, 512, MXFP8_E4M3_fn, MXFP8_E4M3_fn)
+    off = offsets_of([5, 200])
+    want = layer(x, off)
+    layer._row_weight = None
+    busy = torch.cuda.Stream()
+    busy.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(busy):
+        big = torch.ones(1 << 28, device=DEV)
+        for _ in range(20):
+            big.mul_(1.0)
+        one = layer(x, off)
+    two = layer(x, off)
+    torch.cuda.synchronize()
+    assert torch.equal(one, want) and torch.equal(two, want)
+
+
+def test_first_call_inside_a_capture(lib):
+    """A graph that packs the weight does so in every replay; the layer keeps nothing that only a replay fills."""
+    counts = [5, 6]
+    off = offsets_of(counts)
+    layer, _, _, x = grouped_case(counts, 64, 64, MXFP8_E4M3_fn, MXFP8_E4M3_fn, bias=False)
+    want = MX.mxfp_grouped_linear(x, MXFP8_E4M3_fn, layer.w_scales, layer.w_elements, layer.w_tensor_meta, off)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = layer(x, off)
+    assert torch.equal(layer(x, off), want)
+    graph.replay()
+    assert torch.equal(got, want)
+    with torch.no_grad():
+        layer.w_elements.zero_()
+    graph.replay()
+    assert not got.any()
+
+
+def test_a_captured_graph_finds_the_weights_packed_anew(lib):
+    counts = [5, 6]
+    off = offsets_of(counts)
+    layer, _, _, x = grouped_case(counts, 64, 64, MXFP8_E4M3_fn, MXFP8_E4M3_fn, bias=False)
+    other = MXFPGroupedLinearPTQ.from_weight(rand(2, 64, 64, seed=31), None, MXFP8_E4M3_fn, MXFP8_E4M3_fn)
+    layer(x, off)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = layer(x, off)
+    layer.load_state_dict(other.state_dict())
+    want = layer(x, off)
+    assert torch.equal(want, other(x, off))
+    graph.replay()
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("M", [3, 200])
+def test_calls_in_a_row_read_what_the_one_before_wrote(lib, M):
+    """Kernels that may start before the one in front of them has ended: each call's input is the last one's output, in place and
+    through an odd width (no wide accesses), many times over."""
+    square, wq, _ = linear_layer(256, 256, MXFP8_E4M3_fn, MXFP8_E4M3_fn)
+    x = rand(M, 256, seed=4)
+    want, got = x.clone(), x.clone()
+    for _ in range(30):
+        want = square(want, residual=want)
+        torch.cuda.synchronize()
+        want = want / 4
+    for _ in range(30):
+        got = square(got, residual=got).div_(4)
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    y = x.clone()
+    square(y, activation="relu")
+    with torch.cuda.graph(graph):
+        z = y
+        for _ in range(12):
+            z = square(z, activation="silu", residual=z)
+    graph.replay()
+    v = x.clone()
+    for _ in range(12):
+        v = square(v, activation="silu", residual=v)
+        torch.cuda.synchronize()
+    assert torch.equal(z, v)
+
+
 def test_long_axis_and_many_rows(lib):
     """More row tiles than CTAs, offsets of the output past 2^31 bytes, a long K."""
     layer, wq, b, x = grouped_case([9000, 0, 20000, 1], 40, 2048, MXFP8_E4M3_fn, MXFP8_E4M3_fn)

@@ -131,10 +131,25 @@ def test_grouped_refusals(change, match):
         GR.grouped_linear(**call)
 
 
+@pytest.mark.parametrize("name", ["x", "multiplier", "residual", "row_index", "bias", "offsets"])
+def test_out_may_not_overlap_what_is_read(name):
+    """``out`` shares its last row with an operand; only the residual or multiplier itself may be ``out``."""
+    room = torch.zeros(4096, dtype=torch.bfloat16)
+    out = room[:2 * N].view(2, N)
+    at = room[N:]
+    operand = {"x": lambda: at[:2 * K].view(2, K).as_subclass(FakeCuda), "row_index": lambda: at[:4].view(torch.int32),
+               "offsets": lambda: at[:2 * (E + 1)].view(torch.int32), "bias": lambda: at[:E * N].view(E, N)}.get(name, lambda: at[:2 * N].view(2, N))()
+    w = GR.PackedExperts(torch.zeros(1, dtype=torch.uint8), 0, E, N, K)
+    call = dict(x=fake(2, K), x_meta=MXFP8_E4M3_fn, w=w, offsets=torch.zeros(E + 1, dtype=torch.int32), out=out) | {name: operand}
+    with pytest.raises(ValueError, match="overlaps the .*" + ("input" if name == "x" else name)):
+        GR.grouped_linear(**call)
+
+
 def test_pack_refusals():
     s, e, _ = codes()
     e = e.as_subclass(FakeCuda)
-    for bad in (dict(groups=2), dict(K=K * 2), dict(w_elements=e.to(torch.int8)), dict(w_scales=s.int()), dict(w_scales=s[:-1])):
+    for bad in (dict(groups=2), dict(K=K * 2), dict(w_elements=e.to(torch.int8)), dict(w_scales=s.int()), dict(w_scales=s[:-1]),
+                dict(groups=0, w_scales=s[:0], w_elements=e[:0]), dict(N=0, w_scales=s[:0], w_elements=e[:0])):
         with pytest.raises(ValueError):
             GR.pack_experts(**(dict(w_scales=s, w_elements=e, groups=E, N=N, K=K, w_meta=MXFP8_E4M3_fn, x_meta=MXFP8_E4M3_fn) | bad))
     with pytest.raises(_lib.MXQError, match="CUDA"):
