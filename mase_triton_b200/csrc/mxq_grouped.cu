@@ -26,16 +26,17 @@
 namespace mxq {
 namespace grouped {
 
-constexpr int EPI_SIDES = 3, EPI_WARPS = 4 * EPI_SIDES;          // epilogue warps: three per TMEM lane quadrant
 constexpr int FIRST_EPI_WARP = 4;                // warps 0, 1, 3: weight copies, MMA issuer, row copies
-constexpr int THREADS = (FIRST_EPI_WARP + EPI_WARPS) * 32;
 
+// Three epilogue warps per lane quadrant (EPI_SIDES) keep up with tall tiles (8192 rows, 32 experts of 2048 x 2048 in four bits: 70.8 -> 65.3 us
+// against two); narrow ones take two, and the shared memory as one more stage (192 x 4096 x 4096: 19.7 -> 19.1).
 // A CTA's tile is 128 features x at most BT rows; MXF4: both operands packed E2M1 nibbles (256 elements of K per 128 bytes).
 // CTAS = 2: a pair of CTAs on two neighbouring SMs takes 256 features and the same rows, each brings its own weights and half of the
 // rows: what tensor tiles read from L2 bounds a large product, and a pair reads two thirds (32 KB a step and SM instead of 48).
-template <int BT_, int STAGES_, bool MXF4_, int CTAS_ = 1> struct Cfg {
+template <int BT_, int STAGES_, bool MXF4_, int CTAS_, int EPI_SIDES_> struct Cfg {
     static constexpr int BT = BT_, STAGES = STAGES_, CTAS = CTAS_;
     static constexpr bool MXF4 = MXF4_;
+    static constexpr int EPI_SIDES = EPI_SIDES_, EPI_WARPS = 4 * EPI_SIDES, THREADS = (FIRST_EPI_WARP + EPI_WARPS) * 32;
     static constexpr int FEATURES = 128 * CTAS;                     // of a unit of work
     using Tile = WeightTile<MXF4>;
     static constexpr int K_STEP = Tile::K_STEP, SF_STEPS = Tile::SF_STEPS;          // elements of K and 128-element steps of scales per stage
@@ -54,18 +55,18 @@ template <int BT_, int STAGES_, bool MXF4_, int CTAS_ = 1> struct Cfg {
     static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + TABLE_END + EPI_WARPS * 2048;
     static_assert(SMEM_BYTES <= 232448, "more shared memory than a CTA can have");
 };
-using Narrow = Cfg<128, 5, false>;
-using NarrowFp4 = Cfg<128, 5, true>;
-using Tall = Cfg<240, 4, false>;
-using TallFp4 = Cfg<224, 4, true>;
-using Pair = Cfg<240, 5, false, 2>;
-using PairFp4 = Cfg<224, 5, true, 2>;
+using Narrow = Cfg<128, 6, false, 1, 2>;
+using NarrowFp4 = Cfg<128, 5, true, 1, 2>;
+using Tall = Cfg<240, 4, false, 1, 3>;
+using TallFp4 = Cfg<224, 4, true, 1, 3>;
+using Pair = Cfg<240, 5, false, 2, 3>;
+using PairFp4 = Cfg<224, 5, true, 2, 3>;
 
 template <class C, int DT>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(C::THREADS, 1)
 grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constant__ CUtensorMap map_x16, const __grid_constant__ CUtensorMap map_x8,
                const __grid_constant__ Params p) {
-    constexpr int STAGES = C::STAGES, CTAS = C::CTAS;
+    constexpr int STAGES = C::STAGES, CTAS = C::CTAS, EPI_SIDES = C::EPI_SIDES, EPI_WARPS = C::EPI_WARPS;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t ring = (raw + 1023u) & ~1023u;
@@ -521,10 +522,11 @@ static int launch(const Params& p, const uint8_t* x_codes, cudaStream_t st) {
     CUtensorMap mx64, mx16, mx8;
     const Groups& g = p.rows;
     if (!make_map(&mx64, x_codes, g.rows, p.K, 64, C::MXF4) || !make_map(&mx16, x_codes, g.rows, p.K, 16, C::MXF4) ||
-        !make_map(&mx8, x_codes, g.rows, p.K, 8, C::MXF4)) return MXQ_ELAUNCH;
+        (C::CTAS == 2 && !make_map(&mx8, x_codes, g.rows, p.K, 8, C::MXF4))) return MXQ_ELAUNCH;
+    if (C::CTAS == 1) mx8 = mx16;                                    // half of a 16-row step is a pair's only
     const int64_t units = most_units(g, p.N, C::FEATURES);
     const int64_t room = sm_count() / C::CTAS;
-    return launch_after(grouped_kernel<C, DT>, (unsigned)((units < room ? units : room) * C::CTAS), THREADS, C::SMEM_BYTES, C::CTAS, st, mx64, mx16, mx8, p);
+    return launch_after(grouped_kernel<C, DT>, (unsigned)((units < room ? units : room) * C::CTAS), C::THREADS, C::SMEM_BYTES, C::CTAS, st, mx64, mx16, mx8, p);
 }
 
 template <class C>
