@@ -376,17 +376,27 @@ int mxq_mx_max_groups(void);
  *   zero_rest : rows of out outside every group are set to zero; otherwise they are left as they are.
  *   scratch   : 256-byte aligned, at least mxq_mx_grouped_scratch_bytes(...) bytes, of this call alone; that is 0, and scratch may
  *               be NULL, for a few rows per group on 16 bytes (one kernel that keeps the quantised rows on the chip).
- * `extra` may be the same buffer as `out`.  K % 32 == 0, w_packed / w_hw_format from mxq_mx_pack_experts.
+ * `extra` may be the same buffer as `out`; no other operand may overlap it.  K % 32 == 0, w_packed / w_hw_format from mxq_mx_pack_experts.
  * `status` as for mxq_mx_gemm.
  */
 int64_t mxq_mx_grouped_scratch_bytes(const void* x, int x_round_mode, int64_t rows_in, int64_t rows, int64_t K,
                                      int64_t groups, int64_t N);
-int mxq_mx_grouped_linear(const void* x, int x_dtype, int64_t rows_in, int64_t rows, int64_t K, int x_exp_bits,
-                          int x_frac_bits, int x_round_mode, const void* row_index, int index64,
-                          const uint8_t* w_packed, int w_hw_format, int64_t groups, int64_t N, const void* offsets,
-                          int offsets64, void* out, const void* bias, int activation,
-                          const void* extra, int extra_mode, int zero_rest, void* scratch, int64_t scratch_bytes,
-                          int* status, void* stream);
+typedef struct mxq_grouped_linear_args {
+    const void* x;
+    const void* row_index;
+    const uint8_t* w_packed;
+    const void* offsets;
+    void* out;
+    const void* bias;
+    const void* extra;
+    void* scratch;
+    int* status;
+    void* stream;
+    int64_t rows_in, rows, K, groups, N, scratch_bytes;
+    int x_dtype, x_exp_bits, x_frac_bits, x_round_mode;
+    int index64, offsets64, w_hw_format, activation, extra_mode, zero_rest;
+} mxq_grouped_linear_args;
+int mxq_mx_grouped_linear(const mxq_grouped_linear_args* args);
 
 #ifdef __cplusplus
 }

@@ -40,7 +40,7 @@ SIGNATURES = {
     "mxq_mx_linear": [_p, _i, _i64, _i64, _i, _i, _p, _p, _i, _i, _i64, _p, _i, _p, _p, _i64, _p, _p],
     "mxq_mx_linear_static": [_p, _i, _i64, _i64, _i, _i, _p, _p, _i, _i, _i64, _p, _i, _p, _p, _p],
     "mxq_mx_pack_experts": [_p, _p, _i64, _i64, _i64, _i, _i, _i, _p, _p, _p],
-    "mxq_mx_grouped_linear": [_p, _i, _i64, _i64, _i64, _i, _i, _i, _p, _i, _p, _i, _i64, _i64, _p, _i, _p, _p, _i, _p, _i, _i, _p, _i64, _p, _p],
+    "mxq_mx_grouped_linear": [ctypes.c_char_p],
     "mxq_mx_max_groups": [],
     "mxq_dense_linear": [_p, _p, _i, _p, _p, _i64, _i64, _i64, _p, _p],
     "mxq_mxfp_weight_linear": [_p, _i, _p, _p, _i, _i, _p, _p, _i64, _i64, _i64, _p, _p],
@@ -101,6 +101,10 @@ def stream_ptr(device: torch.device) -> int:
 
 # the current stream's handle by device index; torch.cuda.current_stream builds a Stream object for it (1.3 us)
 raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+# the current device's index (torch.cuda.current_device checks for lazy initialisation first)
+current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def fmt_args(meta) -> tuple[int, int, int, int]:

@@ -617,10 +617,10 @@ extern "C" int64_t mxq_mx_grouped_scratch_bytes(const void* x, int round_mode, i
     return grouped::align256(rows * K) + grouped::align256(sf) + grouped::align256(rows_in * K) + grouped::align256(rows_in * K / 32);
 }
 
-extern "C" int mxq_mx_grouped_linear(const void* x, int x_dtype, int64_t rows_in, int64_t rows, int64_t K, int x_exp_bits, int x_frac_bits,
-                                     int x_round_mode, const void* row_index, int index64, const uint8_t* w_packed, int w_hw_format, int64_t groups, int64_t N, const void* offsets, int offsets64, void* out, const void* bias,
-                                     int activation, const void* extra, int extra_mode, int zero_rest, void* scratch, int64_t scratch_bytes,
-                                     int* status, void* stream) {
+extern "C" int mxq_mx_grouped_linear(const mxq_grouped_linear_args* args) {
+    if (!args) return MXQ_EINVAL;
+    const auto [x, row_index, w_packed, offsets, out, bias, extra, scratch, status, stream, rows_in, rows, K, groups, N, scratch_bytes, x_dtype, x_exp_bits, x_frac_bits,
+                x_round_mode, index64, offsets64, w_hw_format, activation, extra_mode, zero_rest] = *args;
     if (rows < 0 || rows_in < 0 || groups <= 0 || N <= 0 || K <= 0 || K % 32 != 0) return MXQ_EINVAL;
     if (x_dtype != MXQ_F32 && x_dtype != MXQ_BF16 && x_dtype != MXQ_F16) return MXQ_EINVAL;
     if (activation < MXQ_ACT_NONE || activation > MXQ_ACT_SILU || extra_mode < MXQ_EXTRA_NONE || extra_mode > MXQ_EXTRA_ADD) return MXQ_EINVAL;

@@ -105,8 +105,8 @@ def linear_with_epilogue(x: Tensor, x_meta: MXFPMeta, w: "_grouped.PackedExperts
                 raise ValueError(f"{name} has to have the result's shape {(*lead, w.N)}: got {tuple(t.shape)}")
         flat = [None if t is None else t.reshape(-1, w.N) for t in (multiplier, residual)]
         return linear_with_epilogue(x.reshape(-1, x.shape[-1]), x_meta, w, bias, activation, *flat).reshape(*lead, w.N)
-    if bias is not None:
-        bias = (bias if bias.dtype == x.dtype else bias.to(x.dtype)).view(1, -1)
+    if bias is not None and bias.dtype != x.dtype:
+        bias = bias.to(x.dtype)
     return _grouped.grouped_linear(x, x_meta, w, None, bias, activation, multiplier, residual)
 
 

@@ -5,6 +5,7 @@ activation, or one for each group of rows (experts).  The reference has neither 
 from __future__ import annotations
 
 import ctypes
+import struct
 from dataclasses import dataclass
 
 import torch
@@ -16,6 +17,8 @@ from .meta import MXFPMeta
 
 EXTRA_NONE, EXTRA_MULTIPLY, EXTRA_ADD = 0, 1, 2
 _INDEX_DTYPES = (torch.int32, torch.int64)
+# mxq_grouped_linear_args: one packed argument costs the host 1 us, 26 separate ones cost it 2.5
+_ARGS = struct.Struct("@10P6q10i")
 
 
 @dataclass
@@ -31,15 +34,29 @@ class PackedExperts:
 
     def __post_init__(self):
         self.device_index, self.pointer = self.blocks.get_device(), self.blocks.data_ptr()
-        self._row_formats: dict[MXFPMeta, tuple[int, int, int]] = {}
+        self._row_format: tuple[MXFPMeta | None, tuple[int, int, int]] = (None, (0, 0, 0))
+        self._scratch_bytes: dict[tuple[int, int, int, bool], int] = {}
 
     def row_format(self, x_meta: MXFPMeta) -> tuple[int, int, int]:
         """Exponent bits, fraction bits and rounding mode of an activation format that goes with these weights."""
-        known = self._row_formats.get(x_meta)
-        if known is None:
+        known, row_format = self._row_format
+        if known is not x_meta:
             if not supported(x_meta) or (self.hw_format == 5 and not is_e2m1(x_meta)):
                 raise ValueError(f"the weight was packed for another activation format than {x_meta}")
-            known = self._row_formats[x_meta] = (x_meta.element_exp_bits, x_meta.element_frac_bits, _lib.ROUND_ID[x_meta.round_mode])
+            row_format = (x_meta.element_exp_bits, x_meta.element_frac_bits, _lib.ROUND_ID[x_meta.round_mode])
+            self._row_format = (x_meta, row_format)
+        return row_format
+
+    def scratch_bytes(self, x_ptr: int, round_id: int, tokens: int, rows: int) -> int:
+        """Workspace of a call (asked of the library once per size)."""
+        key = (tokens, rows, round_id, x_ptr % 16 == 0)
+        known = self._scratch_bytes.get(key)
+        if known is None:
+            with torch.cuda.device(self.device_index):
+                known = _lib.load().mxq_mx_grouped_scratch_bytes(x_ptr, round_id, tokens, rows, self.K, self.groups, self.N)
+            if len(self._scratch_bytes) >= 4096:
+                self._scratch_bytes.clear()
+            self._scratch_bytes[key] = known
         return known
 
 
@@ -88,7 +105,8 @@ def kept_weight(layer, groups: int, N: int, K: int) -> PackedExperts:
     """The packed weight of a layer (``w_scales``, ``w_elements``, ``w_tensor_meta``, ``x_mxfp_meta``), kept with it until its code tensors
     are written, replaced or moved.  It is packed anew into the same memory, so that a captured graph finds it there, and before
     this returns it is complete for every stream.  While a graph is captured nothing is kept: packing is then part of the graph."""
-    w_scales, w_elements, kept = layer.w_scales, layer.w_elements, layer._row_weight
+    params, kept = layer._parameters, layer._row_weight
+    w_scales, w_elements = params["w_scales"], params["w_elements"]
     state = (w_elements._version, w_scales._version, w_elements.data_ptr(), w_scales.data_ptr())
     if kept is not None and kept[0] is w_elements and kept[1] is w_scales and kept[2] is layer.w_tensor_meta and kept[3] is layer.x_mxfp_meta and kept[4] == state:
         return kept[5]
@@ -155,8 +173,7 @@ def grouped_linear(x: Tensor, x_meta: MXFPMeta, w: PackedExperts, offsets: Tenso
         raise ValueError(f"the weight is on {w.blocks.device}, the input on {x.device}")
     x = x.contiguous()
     tokens = rows = x.shape[0]
-    offsets_ptr = index_ptr = bias_ptr = extra_ptr = None
-    offsets64 = index64 = 0
+    offsets_ptr = index_ptr = bias_ptr = extra_ptr = offsets64 = index64 = 0
     if offsets is not None:
         if _bad_index(offsets, "offsets", groups + 1, dev):
             raise _index_error(offsets, "offsets", groups + 1, x)
@@ -171,7 +188,7 @@ def grouped_linear(x: Tensor, x_meta: MXFPMeta, w: PackedExperts, offsets: Tenso
         rows = row_index.shape[0]
         index_ptr, index64 = row_index.data_ptr(), int(row_index.dtype == torch.int64)
     if bias is not None:
-        if bias.dtype != dtype or bias.shape != (groups, N) or bias.get_device() != dev:
+        if bias.dtype != dtype or bias.get_device() != dev or (bias.shape != (groups, N) and (offsets is not None or bias.shape != (N,))):
             raise _operand_error(bias, "bias", (groups, N), x)
         bias = bias.contiguous()
         bias_ptr = bias.data_ptr()
@@ -198,19 +215,19 @@ def grouped_linear(x: Tensor, x_meta: MXFPMeta, w: PackedExperts, offsets: Tenso
     if rows == 0:
         return out
     status = status_address(dev)
-    L = _lib.load()
     x_ptr = x.data_ptr()
-    nbytes = L.mxq_mx_grouped_scratch_bytes(x_ptr, round_id, tokens, rows, K, groups, N)
+    nbytes = w.scratch_bytes(x_ptr, round_id, tokens, rows)
     # of this call alone: two captured graphs, or two streams, never share it
     scratch = None if nbytes == 0 else x.new_empty(nbytes // x.element_size())           # (a multiple of 256 bytes)
-    args = (x_ptr, dtype_id, tokens, rows, K, exp_bits, frac_bits, round_id, index_ptr, index64, w.pointer, w.hw_format, groups,
-            N, offsets_ptr, offsets64, out.data_ptr(), bias_ptr, act, extra_ptr, extra_mode, zero_rest,
-            None if scratch is None else scratch.data_ptr(), nbytes, status, _lib.raw_stream(dev))
-    if torch.cuda.current_device() == dev:
-        rc = L.mxq_mx_grouped_linear(*args)
+    args = _ARGS.pack(x_ptr, index_ptr, w.pointer, offsets_ptr, out.data_ptr(), bias_ptr, extra_ptr, 0 if scratch is None else scratch.data_ptr(), status,
+                      _lib.raw_stream(dev), tokens, rows, K, groups, N, nbytes, dtype_id, exp_bits, frac_bits, round_id, index64, offsets64, w.hw_format, act,
+                      extra_mode, zero_rest)
+    run = _lib.load().mxq_mx_grouped_linear
+    if _lib.current_device() == dev:
+        rc = run(args)
     else:
         with torch.cuda.device(dev):
-            rc = L.mxq_mx_grouped_linear(*args)
+            rc = run(args)
     if rc != 0:
         _lib.check(rc, "mxq_mx_grouped_linear")
     return out

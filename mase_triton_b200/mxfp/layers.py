@@ -16,6 +16,7 @@ from torch import Tensor, nn
 from .._linear_common import parse_layer_type
 from .._ptq_base import PTQLinearBase
 from . import functional as MXFP_F
+from . import grouped as _grouped
 from .meta import MXFPMeta, MXFPTensorMeta
 
 LayerType = Literal["XWB", "XWBq", "XWqB", "XWqBq", "XqWB", "XqWBq", "XqWqB", "XqWqBq"]
@@ -112,8 +113,6 @@ class MXFPLinearPTQ(PTQLinearBase):
 
     def row_weight(self):
         """The quantised weight as the product with an epilogue reads it; see ``mxfp.grouped.kept_weight``."""
-        from . import grouped as _grouped
-
         return _grouped.kept_weight(self, 1, self.out_features, self.in_features)
 
     def export_packed(self) -> dict:
@@ -234,8 +233,6 @@ class MXFPGroupedLinearPTQ(PTQLinearBase):
 
     def __init__(self, w_scales: Tensor, w_elements: Tensor, w_tensor_meta: MXFPTensorMeta, bias: Tensor | None, x_mxfp_meta: MXFPMeta):
         super().__init__()
-        from . import grouped as _grouped
-
         self.groups, self.out_features, self.in_features = MXFP_F.grouped.expert_shape(w_tensor_meta)
         _grouped.check_formats(x_mxfp_meta, w_tensor_meta.meta, self.in_features)
         if bias is not None and tuple(bias.shape) != (self.groups, self.out_features):
@@ -270,15 +267,11 @@ class MXFPGroupedLinearPTQ(PTQLinearBase):
 
     def row_weight(self):
         """The weights as the kernel reads them; see ``mxfp.grouped.kept_weight``."""
-        from . import grouped as _grouped
-
         return _grouped.kept_weight(self, self.groups, self.out_features, self.in_features)
 
     def forward(self, input: Tensor, offsets: Tensor, activation: str | None = None, multiplier: Tensor | None = None,
                 residual: Tensor | None = None, row_index: Tensor | None = None, out: Tensor | None = None) -> Tensor:
         """``mxfp_grouped_linear`` with this layer's weights."""
-        from . import grouped as _grouped
-
         bias = self.bias
         if bias is not None and bias.dtype != input.dtype:
             bias = bias.to(input.dtype)

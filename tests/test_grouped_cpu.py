@@ -3,7 +3,6 @@
 from __future__ import annotations
 
 import math
-from types import SimpleNamespace
 
 import pytest
 import torch
@@ -161,16 +160,19 @@ def test_c_entry_refuses_before_it_launches():
     L = _lib.load()
     buf = torch.zeros(1 << 16, dtype=torch.uint8)
     p = (buf.data_ptr() + 255) // 256 * 256
-    good = dict(x=p, x_dtype=1, rows_in=2, rows=2, K=64, eb=4, fb=3, rm=0, row_index=None, index64=0, w=p, fmt=0, groups=1, N=8, offsets=None,
-                offsets64=0, out=p, bias=None, act=0, extra=None, mode=0, zero=0, scratch=p, nbytes=1 << 16, status=None, stream=None)
-    assert L.mxq_mx_grouped_linear(*(good | dict(rows=0, rows_in=0)).values()) == 0
+    good = dict(x=p, row_index=0, w=p, offsets=0, out=p, bias=0, extra=0, scratch=p, status=0, stream=0, rows_in=2, rows=2, K=64, groups=1, N=8, nbytes=1 << 16,
+                x_dtype=1, eb=4, fb=3, rm=0, index64=0, offsets64=0, fmt=0, act=0, mode=0, zero=0)
+
+    def entry(**change):
+        return L.mxq_mx_grouped_linear(GR._ARGS.pack(*(good | change).values()))
+
+    assert entry(rows=0, rows_in=0) == 0 and L.mxq_mx_grouped_linear(None) == -1
     for bad in (dict(K=48), dict(K=0), dict(N=0), dict(groups=0), dict(groups=2), dict(rows=3), dict(rows=-1), dict(x_dtype=3), dict(act=5), dict(act=-1), dict(mode=3),
-                dict(mode=1), dict(x=None), dict(w=None), dict(w=p + 8), dict(out=None), dict(scratch=None, rm=1), dict(scratch=p + 16), dict(fmt=3), dict(fmt=5),
+                dict(mode=1), dict(x=0), dict(w=0), dict(w=p + 8), dict(out=0), dict(scratch=0, rm=1), dict(scratch=p + 16), dict(fmt=3), dict(fmt=5),
                 dict(eb=3, fb=3)):
-        assert L.mxq_mx_grouped_linear(*(good | bad).values()) == -1, bad
+        assert entry(**bad) == -1, bad
     for bad in (dict(groups=L.mxq_mx_max_groups() + 1, offsets=p), dict(nbytes=64, rm=1), dict(rows=1 << 31, rows_in=1 << 31)):
-        assert L.mxq_mx_grouped_linear(*(good | bad).values()) == -3, bad
+        assert entry(**bad) == -3, bad
     assert L.mxq_mx_grouped_scratch_bytes(p, 0, 2, 2, 48, 1, 8) == -1 and L.mxq_mx_grouped_scratch_bytes(p, 0, 2, 2, 64, 1, 8) == 0
     assert L.mxq_mx_grouped_scratch_bytes(p + 2, 0, 2, 2, 64, 1, 8) > 0 and L.mxq_mx_grouped_scratch_bytes(p, 1, 2, 2, 64, 1, 8) > 0
     assert L.mxq_mx_grouped_scratch_bytes(p, 0, 500, 500, 64, 1, 8) > 0
-    assert SimpleNamespace(**good).K == 64
