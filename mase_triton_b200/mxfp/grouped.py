@@ -107,7 +107,10 @@ def kept_weight(layer, groups: int, N: int, K: int) -> PackedExperts:
     this returns it is complete for every stream.  While a graph is captured nothing is kept: packing is then part of the graph."""
     params, kept = layer._parameters, layer._row_weight
     w_scales, w_elements = params["w_scales"], params["w_elements"]
-    state = (w_elements._version, w_scales._version, w_elements.data_ptr(), w_scales.data_ptr())
+    try:
+        state = (w_elements._version, w_scales._version, w_elements.data_ptr(), w_scales.data_ptr())
+    except RuntimeError:                                             # inference tensors count no versions: packed in every call
+        return pack_experts(w_scales.data, w_elements.data, groups, N, K, layer.w_tensor_meta.meta, layer.x_mxfp_meta)
     if kept is not None and kept[0] is w_elements and kept[1] is w_scales and kept[2] is layer.w_tensor_meta and kept[3] is layer.x_mxfp_meta and kept[4] == state:
         return kept[5]
     _lib.require_cuda(w_elements, "pack_experts")

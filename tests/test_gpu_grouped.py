@@ -522,6 +522,29 @@ def test_replaced_code_tensors(lib):
     assert torch.equal(layer(x, off), want)
 
 
+def test_code_tensors_made_in_inference_mode(lib):
+    """Such tensors count no versions; what a layer computes follows them all the same."""
+    off = offsets_of([5, 6])
+    layer, _, _, x = grouped_case([5, 6], 64, 64, MXFP8_E4M3_fn, MXFP8_E4M3_fn, bias=False)
+    with torch.inference_mode():
+        want = layer(x, off)
+        layer.load_state_dict({k: v.clone() for k, v in layer.state_dict().items()}, assign=True)
+        assert torch.equal(layer(x, off), want)
+        layer.w_elements.zero_()
+        assert not layer(x, off).any()
+
+
+@pytest.mark.parametrize("rows", [3, 300])
+@pytest.mark.parametrize("mode", ["rn", "rz"])
+def test_no_tokens_at_all(lib, rows, mode):
+    """Every row index lies outside an empty x: rows of zeros, the bias is left."""
+    meta = MXFPMeta(32, 8, 4, 3, True, mode)
+    layer, _, b, _ = grouped_case([rows], 72, 96, meta, MXFP8_E4M3_fn)
+    got = layer(torch.empty(0, 96, dtype=torch.bfloat16, device=DEV), offsets_of([rows]), activation="relu",
+                row_index=torch.zeros(rows, dtype=torch.int32, device=DEV))
+    assert torch.equal(got, torch.relu(b).expand(rows, 72))
+
+
 def test_first_call_on_another_stream(lib):
     """What a layer packs in its first call is complete for every stream, whatever the first one is busy with."""
     layer, _, _, x = grouped_case([5, 200], 256, 512, MXFP8_E4M3_fn, MXFP8_E4M3_fn)
