@@ -19,6 +19,9 @@
 //   weights: blocks of 128 features x one step of K, see WeightTile in mxq_grouped.cuh;
 //   rows:    codes [rows, K], scales [tile slot][ceil(K / 128)][chunks][512] bytes.  With tiles of at most `width` rows, tile t of a
 //            group that begins at row f has slot f / width + group + t: no two tiles share one, and no sum over the groups before is needed.
+//
+// Measured (replays in a row, quantiser included): 8192 rows, 4096 -> 14336, E4M3, silu and multiplier: 441 us, 2.2 PFLOP/s under the power cap;
+// 192 rows, 4096 -> 4096: 19.1 us, of which the products are 32 steps at the issue rate; 8192 rows over 32 experts, 2048 -> 2048, E2M1: 65 us.
 #include <algorithm>
 
 #include "mxq_grouped.cuh"
@@ -428,7 +431,9 @@ __global__ void __launch_bounds__(256) pack_rows_kernel(const uint8_t* __restric
 
 // One pass from x to the operand (built-in round-to-nearest formats, 16-byte aligned rows).  One CTA per row segment: the row's group and
 // place are looked up once.  A lane has four accesses of 8 elements; of the four lanes of a block, lane i derives the header of
-// access i and stores its scale.  Bound by memory (x read once, gathered rows mostly from L2) and integer issue about equally.
+// access i and stores its scale.  Bound by memory (x read once, gathered rows mostly from L2) and integer issue about equally:
+// 8192 gathered rows of 2048 to E2M1 in 21 us, cold.  Several rows per CTA with the group looked up by each warp alone: 1 us slower at
+// 192 and at 8192 rows.
 constexpr int QUANT_ACCESSES = 4;                // accesses of 8 elements per lane = lanes of a block
 template <class KIn, class F, int OUT>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* x, const void* row_index, int index64, int64_t rows_in, const Groups g,
