@@ -30,17 +30,28 @@ class PTQLinearBase(nn.Module):
         return self.__dict__ | {"_row_weight": None}          # a copy counts its tensors' versions anew
 
     def _apply(self, fn, recurse=True):
-        before = {name: getattr(self, name).dtype for name in self._code_tensors if getattr(self, name) is not None}
+        def where():
+            kept = {name: getattr(self, name) for name in self._code_tensors if getattr(self, name) is not None}
+            return {name: (t.dtype, t.device, None if self._row_weight is None else t.data_ptr()) for name, t in kept.items()}
+
+        before = where()
         result = super()._apply(fn, recurse)
-        self._row_weight = None
-        for name, dtype in before.items():
-            now = getattr(self, name).dtype
+        after = where()
+        if any(after[name][1] != device for name, (_, device, _) in before.items()):
+            self._row_weight = None
+        elif self._row_weight is not None and after != before:
+            # other storage on the same device, which counts no version: packed anew, into the memory that captured graphs point at
+            self._row_weight = (None, *self._row_weight[1:])
+        for name, (dtype, _, _) in before.items():
+            now = after[name][0]
             if now != dtype:
                 raise ChangeDtypeError(f"Changing dtype of {name} from {dtype} to {now} is not allowed.")
         for meta_name, tensor_name in self._meta_follows.items():
             meta, tensor = getattr(self, meta_name), getattr(self, tensor_name)
             if meta is not None and tensor is not None:
-                setattr(self, meta_name, meta.create(device=tensor.device))
+                moved = meta.create(device=tensor.device)
+                if moved != meta:
+                    setattr(self, meta_name, moved)
         return result
 
     @staticmethod
