@@ -103,8 +103,9 @@ def pack_experts(w_scales: Tensor, w_elements: Tensor, groups: int, N: int, K: i
 
 def kept_weight(layer, groups: int, N: int, K: int) -> PackedExperts:
     """The packed weight of a layer (``w_scales``, ``w_elements``, ``w_tensor_meta``, ``x_mxfp_meta``), kept with it until its code tensors
-    are written, replaced or moved.  It is packed anew into the same memory, so that a captured graph finds it there, and before
-    this returns it is complete for every stream.  While a graph is captured nothing is kept: packing is then part of the graph."""
+    are written, replaced or moved.  It is packed anew into the same memory, so that a captured graph finds it there, once nothing
+    on the device reads that memory any more (a replay on any stream may), and before this returns it is complete for every
+    stream.  While a graph is captured nothing is kept: packing is then part of the graph."""
     params, kept = layer._parameters, layer._row_weight
     w_scales, w_elements = params["w_scales"], params["w_elements"]
     try:
@@ -116,6 +117,8 @@ def kept_weight(layer, groups: int, N: int, K: int) -> PackedExperts:
     _lib.require_cuda(w_elements, "pack_experts")
     with torch.cuda.device(w_elements.device):
         capturing = torch.cuda.is_current_stream_capturing()
+        if kept is not None and not capturing:
+            torch.cuda.synchronize()
         packed = pack_experts(w_scales.data, w_elements.data, groups, N, K, layer.w_tensor_meta.meta, layer.x_mxfp_meta,
                               None if kept is None or capturing else kept[5])
         if not capturing:

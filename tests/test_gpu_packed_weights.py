@@ -31,3 +31,33 @@ def test_a_captured_graph_keeps_its_weights_through_a_move_that_moves_nothing(li
     graph.replay()
     assert torch.equal(got, want) and torch.equal(got_lin, want_lin) and len(filled) == 8
     assert torch.equal(layer(x, off), want)
+
+
+@pytest.mark.parametrize("how", ["call", "replay"])
+def test_a_product_still_queued_elsewhere_has_the_weights_of_its_call(lib, how):
+    """A code tensor that is replaced leaves what a running call was given as it is; so does packing the new one."""
+    counts = [5, 200]
+    off = offsets_of(counts)
+    layer, _, _, x = grouped_case(counts, 512, 1024, MXFP8_E4M3_fn, MXFP8_E4M3_fn)
+    other = MXFPGroupedLinearPTQ.from_weight(rand(2, 512, 1024, seed=31), layer.bias, MXFP8_E4M3_fn, MXFP8_E4M3_fn)
+    old, new = layer(x, off), other(x, off)
+    assert not torch.equal(old, new)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        replayed = layer(x, off)
+    big = torch.ones(1 << 28, device=DEV)
+    busy = torch.cuda.Stream()
+    busy.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(busy):
+        for _ in range(20):
+            big.mul_(1.0)
+        if how == "call":
+            queued = layer(x, off)
+        else:
+            graph.replay()
+    layer.load_state_dict(other.state_dict(), assign=True)
+    now = layer(x, off)
+    torch.cuda.synchronize()
+    assert torch.equal(queued if how == "call" else replayed, old) and torch.equal(now, new)
+    graph.replay()
+    assert torch.equal(replayed, new)

@@ -89,3 +89,31 @@ def test_codes_with_new_storage_are_packed_into_the_same_memory(log):
     again = layer.row_weight()
     assert again.pointer == first and len(packs(log)) == 2
     assert torch.equal(again.blocks, layer.w_elements.reshape(-1))
+
+
+@pytest.mark.parametrize("change", ["written", "replaced", "loaded", "assigned", "functional_call"])
+def test_readers_on_every_stream_are_done_before_the_memory_is_written_again(log, change):
+    """A product that another stream, or a graph there, still runs reads the blocks; whoever replaces a Parameter writes to nothing
+    that it was given, and has no reason to wait for it."""
+    layer = a_layer()
+    first = layer.row_weight()
+    log.clear()
+    other = {"w_elements": layer.w_elements.data + 1, "w_scales": layer.w_scales.data.clone()}
+    if change == "written":
+        layer.w_elements.add_(1)
+    elif change == "replaced":
+        layer.w_elements = torch.nn.Parameter(other["w_elements"], requires_grad=False)
+    elif change == "functional_call":
+        layer.forward = lambda: layer.row_weight()
+        packed = torch.func.functional_call(layer, other, ())
+    else:
+        layer.load_state_dict(other, assign=change == "assigned")
+    if change != "functional_call":
+        packed = layer.row_weight()
+    assert packed.pointer == first.pointer and torch.equal(packed.blocks, other["w_elements"].reshape(-1))
+    assert log == ["wait for the device", ("pack", first.pointer), "wait for the stream"]
+
+
+def test_the_first_packing_waits_for_no_reader(log):
+    a_layer().row_weight()
+    assert log == [("pack", None), "wait for the stream"]
