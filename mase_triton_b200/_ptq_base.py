@@ -29,6 +29,11 @@ class PTQLinearBase(nn.Module):
     def __getstate__(self):
         return self.__dict__ | {"_row_weight": None}          # a copy counts its tensors' versions anew
 
+    def _replicate_for_data_parallel(self):
+        replica = super()._replicate_for_data_parallel()
+        replica._row_weight = None                            # packing the replica's tensors must not write to this layer's memory
+        return replica
+
     def _apply(self, fn, recurse=True):
         def where():
             kept = {name: getattr(self, name) for name in self._code_tensors if getattr(self, name) is not None}

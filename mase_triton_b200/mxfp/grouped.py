@@ -107,7 +107,10 @@ def kept_weight(layer, groups: int, N: int, K: int) -> PackedExperts:
     on the device reads that memory any more (a replay on any stream may), and before this returns it is complete for every
     stream.  While a graph is captured nothing is kept: packing is then part of the graph."""
     params, kept = layer._parameters, layer._row_weight
-    w_scales, w_elements = params["w_scales"], params["w_elements"]
+    if "w_elements" in params:
+        w_scales, w_elements = params["w_scales"], params["w_elements"]
+    else:                                                            # a replica of nn.DataParallel: plain attributes
+        w_scales, w_elements = layer.w_scales, layer.w_elements
     try:
         state = (w_elements._version, w_scales._version, w_elements.data_ptr(), w_scales.data_ptr())
     except RuntimeError:                                             # inference tensors count no versions: packed in every call

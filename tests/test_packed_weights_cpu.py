@@ -117,3 +117,16 @@ def test_readers_on_every_stream_are_done_before_the_memory_is_written_again(log
 def test_the_first_packing_waits_for_no_reader(log):
     a_layer().row_weight()
     assert log == [("pack", None), "wait for the stream"]
+
+
+@pytest.mark.parametrize("make", [a_layer, a_linear])
+def test_replicas_pack_their_own_copy(log, make):
+    """A replica of ``nn.DataParallel`` holds its tensors as plain attributes; its blocks are not those of the module it was made from."""
+    layer = make()
+    packed = layer.row_weight()
+    replica = layer._replicate_for_data_parallel()
+    replica.w_scales, replica.w_elements = layer.w_scales.data.clone(), layer.w_elements.data + 1
+    theirs = replica.row_weight()
+    assert theirs.pointer != packed.pointer and torch.equal(theirs.blocks, replica.w_elements.reshape(-1))
+    assert replica.row_weight() is theirs and layer.row_weight() is packed
+    assert torch.equal(packed.blocks, layer.w_elements.reshape(-1))
