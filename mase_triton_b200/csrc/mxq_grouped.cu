@@ -44,8 +44,10 @@ template <int BT_, int STAGES_, bool MXF4_, int CTAS_, int EPI_SIDES_> struct Cf
     using Tile = WeightTile<MXF4>;
     static constexpr int K_STEP = Tile::K_STEP, SF_STEPS = Tile::SF_STEPS;          // elements of K and 128-element steps of scales per stage
     static constexpr int X_BYTES = BT / CTAS * 128, X_CHUNKS = BT > 128 ? 2 : 1;
-    // a stage: weight codes | row codes | scales: [SF_STEPS][512] of the weights, [SF_STEPS][X_CHUNKS][512] of the rows
-    static constexpr int X = Tile::CODES, SFW = X + X_BYTES, SFX = SFW + SF_STEPS * 512;
+    // a stage: weight codes | row codes | scales: [SF_STEPS][512] of the weights, [SF_STEPS][X_CHUNKS][512] of the rows; in a pair the
+    // weights' scales lie behind their codes, as in memory: one copy brings both
+    static constexpr int X = CTAS == 2 ? (Tile::BYTES + 1023) / 1024 * 1024 : Tile::CODES, SFW = CTAS == 2 ? Tile::CODES : X + X_BYTES;
+    static constexpr int SFX = CTAS == 2 ? X + X_BYTES : SFW + SF_STEPS * 512;
     static constexpr int STAGE_BYTES = (SFX + SF_STEPS * X_CHUNKS * 512 + 1023) / 1024 * 1024;      // the 128-byte swizzle repeats every 1024 bytes
     // Two accumulators of BT columns, tiles in turn: one is read while the next is computed.  Behind them two sets of scale columns.
     static constexpr int ACC_STRIDE = BT > 128 ? 256 : BT;
@@ -68,32 +70,31 @@ using PairFp4 = Cfg<224, 5, true, 2, 3>;
 template <class C, int DT>
 __global__ void __launch_bounds__(C::THREADS, 1)
 grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constant__ CUtensorMap map_x16, const __grid_constant__ CUtensorMap map_x8,
-               const __grid_constant__ Params p) {
+               const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_sf, const __grid_constant__ Params p) {
     constexpr int STAGES = C::STAGES, CTAS = C::CTAS, EPI_SIDES = C::EPI_SIDES, EPI_WARPS = C::EPI_WARPS;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t ring = (raw + 1023u) & ~1023u;
     uint8_t* ring_ptr = smem_raw + (ring - raw);
-    const uint32_t bars = ring + STAGES * C::STAGE_BYTES;            // full[S], empty[S], peer_full[S], accum_full[2], accum_empty[2], drain, tmem slot
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ring_ptr + STAGES * C::STAGE_BYTES + 8 * (3 * STAGES + 5));
+    const uint32_t bars = ring + STAGES * C::STAGE_BYTES;            // full[S], empty[S], accum_full[2], accum_empty[2], drain, tmem slot
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ring_ptr + STAGES * C::STAGE_BYTES + 8 * (2 * STAGES + 5));
     int* tiles = reinterpret_cast<int*>(ring_ptr + STAGES * C::STAGE_BYTES + 256);
     int* first = tiles + MAX_GROUPS + 1;
     auto full_bar = [&](int s) { return bars + 8u * s; };
     auto empty_bar = [&](int s) { return bars + 8u * (STAGES + s); };
-    auto peer_full = [&](int s) { return bars + 8u * (2 * STAGES + s); };            // in the leader: the other CTA's part of the stage is there
-    auto accum_full = [&](int a) { return bars + 8u * (3 * STAGES + a); };
-    auto accum_empty = [&](int a) { return bars + 8u * (3 * STAGES + 2 + a); };
-    const uint32_t drain_bar = bars + 8u * (3 * STAGES + 4);
+    auto accum_full = [&](int a) { return bars + 8u * (2 * STAGES + a); };
+    auto accum_empty = [&](int a) { return bars + 8u * (2 * STAGES + 2 + a); };
+    const uint32_t drain_bar = bars + 8u * (2 * STAGES + 4);
 
     const int warp = __shfl_sync(~0u, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) { mbar_init(full_bar(s), 2); mbar_init(empty_bar(s), 1); mbar_init(peer_full(s), 1); }      // full: weight copies, row copies
+        for (int s = 0; s < STAGES; ++s) { mbar_init(full_bar(s), 2); mbar_init(empty_bar(s), 1); }      // full: weight copies, row copies
         for (int a = 0; a < 2; ++a) { mbar_init(accum_full(a), 1); mbar_init(accum_empty(a), EPI_WARPS * CTAS); }
         mbar_init(drain_bar, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == 0 && elect_one()) { prefetch_map(map_x16); prefetch_map(map_x64); if (CTAS == 2) prefetch_map(map_x8); }
+    if (warp == 0 && elect_one()) { prefetch_map(map_x16); prefetch_map(map_x64); if (CTAS == 2) { prefetch_map(map_x8); prefetch_map(map_w); prefetch_map(map_sf); } }
     if (warp == 1) tc_alloc<CTAS>(smem_u32(tmem_slot), 512);
     tc_fence_before();
     build_table(p.rows, tiles, first);
@@ -126,12 +127,27 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constan
             const uint8_t* w = p.w + (size_t)uniform(t.g) * p.w_group + (size_t)ftile * KT * C::Tile::BYTES;
             const uint8_t* x_sf = p.x_sf + (size_t)uniform(t.begin / p.rows.width + t.g + t.tile) * KT128 * (C::X_CHUNKS * 512);
             const uint32_t x_chunks = n > 128 ? 2 : 1;
+            const int w_line = (int)((w - p.w) >> 7), sf_line = (int)((x_sf - p.x_sf) >> 7);     // a pair's maps are of lines of 128 bytes
             for (int kt = 0; kt < KT; ++kt, ++issued, at.step()) {
                 ok = mbar_wait(empty_bar(at.s), at.phase ^ 1u, p.status, ST_PRODUCER_TIMEOUT);      // (a fresh barrier's phase before counts as complete)
                 if (!ok) break;
                 const uint32_t st = ring + at.s * C::STAGE_BYTES, full = full_bar(at.s);
                 if (elect_one()) {
-                    if (warp == 0) {
+                    if (CTAS == 2) {
+                        // both CTAs' copies complete the leader's barrier, where both CTAs' bytes are expected
+                        const uint32_t both = map_to_rank(full, 0);
+                        if (warp == 0) {
+                            if (rank == 0) mbar_expect_tx(full, 2u * C::Tile::BYTES);
+                            tma_load_2d_pair(st, &map_w, 0, w_line + kt * (C::Tile::BYTES / 128), both);
+                        } else {
+                            if (rank == 0) mbar_expect_tx(full, 2u * (mine * 128u + C::SF_STEPS * C::X_CHUNKS * 512u));
+                            uint32_t r = 0;
+                            for (; r + 64 <= mine; r += 64) tma_load_2d_pair(st + C::X + r * 128, &map_x64, kt * C::K_STEP, row + r, both);
+                            for (; r + 16 <= mine; r += 16) tma_load_2d_pair(st + C::X + r * 128, &map_x16, kt * C::K_STEP, row + r, both);
+                            if (r < mine) tma_load_2d_pair(st + C::X + r * 128, &map_x8, kt * C::K_STEP, row + r, both);
+                            tma_load_2d_pair(st + C::SFX, &map_sf, 0, sf_line + kt * (C::SF_STEPS * C::X_CHUNKS * 4), both);
+                        }
+                    } else if (warp == 0) {
                         const uint8_t* block = w + (size_t)kt * C::Tile::BYTES;
                         mbar_expect_tx(full, C::Tile::BYTES);
                         bulk_load(st, block, C::Tile::CODES, full);
@@ -141,7 +157,6 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constan
                         uint32_t r = 0;
                         for (; r + 64 <= mine; r += 64) tma_load_2d(st + C::X + r * 128, &map_x64, kt * C::K_STEP, row + r, full);
                         for (; r + 16 <= mine; r += 16) tma_load_2d(st + C::X + r * 128, &map_x16, kt * C::K_STEP, row + r, full);
-                        if (CTAS == 2 && r < mine) tma_load_2d(st + C::X + r * 128, &map_x8, kt * C::K_STEP, row + r, full);
 #pragma unroll
                         for (int c = 0; c < C::SF_STEPS; ++c)
                             bulk_load(st + C::SFX + c * C::X_CHUNKS * 512, x_sf + (size_t)(kt * C::SF_STEPS + c) * (C::X_CHUNKS * 512),
@@ -151,19 +166,12 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constan
                 __syncwarp();
             }
         }
-        // every copy this warp started must have landed before the CTA gives its shared memory back (returns at once in a run that went well)
+        // Every copy this warp started must have landed before the CTA gives its shared memory back (returns at once in a run that went
+        // well): the stage is full, or, where the leader's barrier tells that, the products have read it.
         for (uint32_t j = issued > (uint32_t)STAGES ? issued - STAGES : 0u; j < issued; ++j)
-            mbar_wait(full_bar(j % STAGES), (j / STAGES) & 1, p.status, ST_PRODUCER_TIMEOUT);
-    } else if (warp == 1 && CTAS == 2 && rank == 1) {
-        // ---------------- second CTA of a pair: tell the leader that this CTA's part of a stage is there ----------------
-        bool ok = true;
-        RingAt<STAGES> at;
-        for (int u = u_begin; u < walk.total && ok; u += u_step)
-            for (int kt = 0; kt < KT && ok; ++kt, at.step()) {
-                ok = mbar_wait(full_bar(at.s), at.phase, p.status, ST_MMA_TIMEOUT);
-                if (ok && elect_one()) signal_rank(peer_full(at.s), 0);
-                __syncwarp();
-            }
+            mbar_wait(rank == 0 ? full_bar(j % STAGES) : empty_bar(j % STAGES), (j / STAGES) & 1, p.status, ST_PRODUCER_TIMEOUT);
+    } else if (warp == 1 && rank == 1) {
+        // the leader issues the products of both
     } else if (warp == 1) {
         // ---------------- MMA issuer ----------------
         // One thread's issue rate is what a narrow tile's products run at, so everything here is uniform over the warp (the
@@ -175,6 +183,10 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constan
         RingAt<STAGES> at;
         int u = u_begin;
         Unit next = u < walk.total ? walk.at(u, C::FEATURES) : Unit{};
+        // of a pair: what the other CTA's copies completed and its epilogue arrived at
+        auto wait = [&](uint32_t bar, uint32_t parity) {
+            return CTAS == 1 ? mbar_wait(bar, parity, p.status, ST_MMA_TIMEOUT) : mbar_wait_cluster(bar, parity, p.status, ST_MMA_TIMEOUT);
+        };
         auto copy_scales = [&](int s, uint32_t into, uint32_t n) {
             const uint32_t from = ring + s * C::STAGE_BYTES, sfw = tmem + C::SFW_COL + into, sfx = tmem + C::SFX_COL + into;
             if (elect_one()) {
@@ -196,22 +208,20 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constan
             const uint32_t idesc = p.idesc | ((n >> 3) << 17);
             const int buf = (int)(count & 1u);
             // the first product into an accumulator overwrites it: the epilogue must have read what it held
-            if (count >= 2) ok = mbar_wait(accum_empty(buf), ((count >> 1) - 1) & 1, p.status, ST_MMA_TIMEOUT);
+            if (count >= 2) ok = wait(accum_empty(buf), ((count >> 1) - 1) & 1);
             tc_fence_after();
             const uint32_t d = tmem + buf * C::ACC_STRIDE;
             for (int kt = 0; kt < KT && ok; ++kt, set ^= C::SF_COLS) {
                 const uint32_t st = ring + at.s * C::STAGE_BYTES, empty = empty_bar(at.s);
                 if (!copied) {
-                    ok = mbar_wait(full_bar(at.s), at.phase, p.status, ST_MMA_TIMEOUT);
-                    if (CTAS == 2 && ok) ok = mbar_wait(peer_full(at.s), at.phase, p.status, ST_MMA_TIMEOUT);
+                    ok = wait(full_bar(at.s), at.phase);
                     tc_fence_after();
                     if (!ok) break;
                     copy_scales(at.s, set, n);
                 }
                 copied = false;
                 at.step();
-                if ((kt + 1 < KT || more) && mbar_test_wait(full_bar(at.s), at.phase) &&
-                    (CTAS == 1 || mbar_test_wait(peer_full(at.s), at.phase))) {
+                if ((kt + 1 < KT || more) && (CTAS == 1 ? mbar_test_wait(full_bar(at.s), at.phase) : mbar_test_wait_cluster(full_bar(at.s), at.phase))) {
                     tc_fence_after();
                     copy_scales(at.s, set ^ C::SF_COLS, kt + 1 < KT ? n : next_n);
                     copied = true;
@@ -300,7 +310,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_x64, const __grid_constan
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) { if (rank == 0) mbar_arrive(accum_empty(buf)); else signal_rank(accum_empty(buf), 0); }
+            if (lane == 0) { if (rank == 0) mbar_arrive(accum_empty(buf)); else arrive_after_tensor_reads(accum_empty(buf), 0); }
         }
         if (p.zero_rest) zero_rows_outside(out, first[0], first[p.rows.groups], p.rows.rows, p.N, threadIdx.x - FIRST_EPI_WARP * 32, EPI_WARPS * 32);
     }
@@ -519,19 +529,29 @@ static int quantize_rows(const void* x, int x_dtype, const void* row_index, int 
     return rc;
 }
 
+// slots of the rows' scales, one per row tile
+static int64_t tile_slots(int64_t rows, int64_t groups, int64_t width) { return rows / width + groups + 1; }
+
 template <class C, int DT>
 static int launch(const Params& p, const uint8_t* x_codes, cudaStream_t st) {
     static bool attr_done[MAX_DEVICES] = {false};
     const cudaError_t e = raise_smem_limit(grouped_kernel<C, DT>, C::SMEM_BYTES, attr_done);
     if (e != cudaSuccess) { set_last_cuda_error(e); return MXQ_ELAUNCH; }
-    CUtensorMap mx64, mx16, mx8;
+    CUtensorMap mx64, mx16, mx8, mw, msf;
     const Groups& g = p.rows;
     if (!make_map(&mx64, x_codes, g.rows, p.K, 64, C::MXF4) || !make_map(&mx16, x_codes, g.rows, p.K, 16, C::MXF4) ||
         (C::CTAS == 2 && !make_map(&mx8, x_codes, g.rows, p.K, 8, C::MXF4))) return MXQ_ELAUNCH;
-    if (C::CTAS == 1) mx8 = mx16;                                    // half of a 16-row step is a pair's only
+    if constexpr (C::CTAS == 2) {
+        // a block of the weights, a stage's scales of the rows, as lines of 128 bytes
+        const int64_t sf_lines = tile_slots(g.rows, g.groups, g.width) * ((p.K + 127) / 128) * (C::X_CHUNKS * 4);
+        if (!make_line_map(&mw, p.w, g.groups * (p.w_group / 128), C::Tile::BYTES / 128) || !make_line_map(&msf, p.x_sf, sf_lines, C::SF_STEPS * C::X_CHUNKS * 4))
+            return MXQ_ELAUNCH;
+    } else {
+        mx8 = mw = msf = mx16;                                       // a pair's only
+    }
     const int64_t units = most_units(g, p.N, C::FEATURES);
     const int64_t room = sm_count() / C::CTAS;
-    return launch_after(grouped_kernel<C, DT>, (unsigned)((units < room ? units : room) * C::CTAS), C::THREADS, C::SMEM_BYTES, C::CTAS, st, mx64, mx16, mx8, p);
+    return launch_after(grouped_kernel<C, DT>, (unsigned)((units < room ? units : room) * C::CTAS), C::THREADS, C::SMEM_BYTES, C::CTAS, st, mx64, mx16, mx8, mw, msf, p);
 }
 
 template <class C>
@@ -553,7 +573,7 @@ struct Plan {
     Shape shape;                 // the kernel for few rows, where x and its format allow; tiles of up to 128 rows; up to 240 (224 of E2M1 pairs); these on a pair of CTAs
     int width;                   // rows per tile at most
     int chunks() const { return shape <= NARROW ? 1 : 2; }
-    int64_t sf_bytes(int64_t rows, int64_t groups, int64_t K) const { return (rows / width + groups + 1) * ((K + 127) / 128) * chunks() * 512; }
+    int64_t sf_bytes(int64_t rows, int64_t groups, int64_t K) const { return tile_slots(rows, groups, width) * ((K + 127) / 128) * chunks() * 512; }
 };
 // The tiles that take the fewest estimated nanoseconds of the whole GPU: rounds of tiles x steps of K x what a step takes.  That is
 // what one thread issues (215) at least; else, for one CTA, what L2 gives all SMs together (13.4 TB/s measured: 47.6 KB of a 240-row step in

@@ -328,6 +328,13 @@ template <int CTAS> __device__ __forceinline__ void tc_commit(uint32_t bar) {
     else asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
 }
 
+// tiled load into this CTA's shared memory that completes a barrier of either CTA of the pair
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+        ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+
 // Clusters: an address in another CTA's shared memory, arrival on another CTA's barrier (behind this thread's accesses), a barrier of
 // all threads, and bounded waits for what other CTAs complete.
 __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
@@ -338,13 +345,23 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
 __device__ __forceinline__ void arrive_at(uint32_t bar, int rank) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(map_to_rank(bar, (uint32_t)rank)) : "memory");
 }
-// the same where no ordinary accesses have to be ordered (what the copy engine and the tensor cores write is ordered by the barriers that
-// they complete): orderings of cluster scope cost some 500 ns each
-__device__ __forceinline__ void signal_rank(uint32_t bar, int rank) {
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(map_to_rank(bar, (uint32_t)rank)) : "memory");
+// The same behind reads of tensor memory that products of another CTA's thread will overwrite: those are ordered by
+// tcgen05.fence::before_thread_sync here, ::after_thread_sync there and a relaxed arrival of cluster scope between them.  A release would
+// wait for the thread's stores as well (8192 rows over 32 experts of 2048 x 2048, 4-bit pairs: 63 -> 68 us).
+__device__ __forceinline__ void arrive_after_tensor_reads(uint32_t bar, int rank) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(map_to_rank(bar, (uint32_t)rank)) : "memory");
 }
 __device__ __forceinline__ void cluster_barrier() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ bool mbar_test_wait_cluster(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
 }
 __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, int* status, int code) {
     for (uint32_t i = 0; i < SPIN_LIMIT; ++i) {
@@ -535,6 +552,17 @@ static bool make_map(CUtensorMap* map, const void* codes, int64_t rows, int64_t 
     const cuuint32_t estr[2] = {1, 1};
     return fn(map, nibbles ? CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN8B : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, box, estr,
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// box of `box` lines of 128 bytes, as they lie in memory
+static bool make_line_map(CUtensorMap* map, const void* lines, int64_t n, int box) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[2] = {128, (cuuint64_t)n};
+    const cuuint64_t strides[1] = {128};
+    const cuuint32_t boxes[2] = {128, (cuuint32_t)box};
+    const cuuint32_t estr[2] = {1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(lines), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace grouped
