@@ -54,13 +54,19 @@ template <class T> __device__ __forceinline__ void store_four(T* at, int left, i
     for (int k = 0; k < 4; ++k) if (k < left) at[k] = o.v[k];
 }
 
-// z * sigmoid(2u) is 0.5 z (1 + tanh u); exp overflows to Inf for very negative arguments and the quotient is then 0
-__device__ __forceinline__ float sigmoid_times(float z, float a) { return __fdividef(z, 1.0f + __expf(-a)); }
-template <int ACT> __device__ __forceinline__ float activate(float z) {
+// z sigmoid(a), the tail included: with t = exp(-|a|) the divisor lies in [1, 2], where the fast division holds (beyond 2^126 it gives 0), and
+// nothing overflows.  For fp32 results expf: in __expf the rounding of a log2(e) alone costs |a| half steps of 2^-24.  16-bit results have
+// steps of 2^-11 at least, beside at most 104 of those half steps where t is not 0: __expf (expf: 8192 x 4096 x 14336 532 -> 551 us).
+// (z sigmoid(2u) is 0.5 z (1 + tanh u).)
+template <class T> __device__ __forceinline__ float sigmoid_times(float z, float a) {
+    const float t = sizeof(T) == 4 ? expf(-fabsf(a)) : __expf(-fabsf(a));
+    return __fdividef(a < 0.0f ? z * t : z, 1.0f + t);
+}
+template <int ACT, class T> __device__ __forceinline__ float activate(float z) {
     if constexpr (ACT == MXQ_ACT_RELU) return z < 0.0f ? 0.0f : z;                       // NaN stays NaN
     else if constexpr (ACT == MXQ_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-    else if constexpr (ACT == MXQ_ACT_GELU_TANH) return sigmoid_times(z, 1.5957691216057308f * (z + 0.044715f * z * z * z));
-    else if constexpr (ACT == MXQ_ACT_SILU) return sigmoid_times(z, z);
+    else if constexpr (ACT == MXQ_ACT_GELU_TANH) return sigmoid_times<T>(z, 1.5957691216057308f * (z + 0.044715f * z * z * z));
+    else if constexpr (ACT == MXQ_ACT_SILU) return sigmoid_times<T>(z, z);
     else return z;
 }
 // The epilogue of one lane's 4 x 4 values: rows at, at + 4 * pitch, ... (`rows` of them exist, at most four), four features each.
@@ -75,7 +81,7 @@ __device__ __forceinline__ void finish(const float* slot, int lane, const float 
         y[4 * i] = v.x; y[4 * i + 1] = v.y; y[4 * i + 2] = v.z; y[4 * i + 3] = v.w;
     }
 #pragma unroll
-    for (int k = 0; k < 16; ++k) y[k] = activate<ACT>(y[k] + bias[k & 3]);
+    for (int k = 0; k < 16; ++k) y[k] = activate<ACT, T>(y[k] + bias[k & 3]);
     if (extra_mode == X_MUL) {
 #pragma unroll
         for (int k = 0; k < 16; ++k) y[k] *= widen(extra[k >> 2].v[k & 3]);
