@@ -6,7 +6,7 @@
 //     shared memory that the tensor cores read, a stage each in turn: one warp's way through a stage (a load, the block
 //     maximum, the rounding, a proxy fence) takes far longer than the stage's products.  Every CTA repeats this for its own features,
 //     out of L2 and beside the weights' copies, which take longer; there is no second launch, no operand in memory and no workspace;
-//   * two CTAs fit on an SM (a ring of 64 to 80 KB each): one's start and end hide behind the other's copies, within a call and, with
+//   * two CTAs fit on an SM (a ring of 95 KB each, 80 for 4-bit pairs; and for up to 1024 groups): one's start and end hide behind the other's copies, within a call and, with
 //     the launch that may overlap the kernel before, between calls;
 //   * where the features leave SMs idle, K is split over a cluster of 2 or 4 CTAs.  Each sums its part in tensor memory; the
 //     partial sums go to the CTA that finishes those features through distributed shared memory and are added in the
@@ -40,10 +40,13 @@ template <bool MXF4> struct Cfg {
     static constexpr int W = X_BYTES, SFW = W + Tile::CODES, SFX = W + Tile::BYTES;
     static constexpr int STAGE_BYTES = SFX + SF_STEPS * 512;
     static constexpr int SLOTS = 4 * 2048, EXCHANGE = 3 * 2048;                      // 32 features x 16 rows per epilogue warp, and per part received
-    static constexpr int FIXED_BYTES = 1024 + STAGES * STAGE_BYTES + 256 + SLOTS + EXCHANGE;
-    static int smem_bytes(int groups) { return FIXED_BYTES + 2 * (groups + 1) * 4; }  // the group table comes last
+    static constexpr int FIXED_BYTES = 1024 + STAGES * STAGE_BYTES + 256 + SLOTS;
+    // behind these the group table and the exchange of a cluster; CTAs that share no unit have none
+    static constexpr int smem_bytes(int groups, int split) { return FIXED_BYTES + (split > 1 ? EXCHANGE : 0) + 2 * (groups + 1) * 4; }
+    static constexpr int per_sm(int groups, int split) { return 2 * (smem_bytes(groups, split) + 1024) <= 233472 ? 2 : 1; }
     static_assert(STAGE_BYTES % 1024 == 0, "the 128-byte swizzle repeats every 1024 bytes");
-    static_assert(FIXED_BYTES + 2 * (MAX_GROUPS + 1) * 4 <= 232448, "more shared memory than a CTA can have");
+    static_assert(smem_bytes(MAX_GROUPS, 2) <= 232448, "more shared memory than a CTA can have");
+    static_assert(per_sm(MAX_GROUPS, 1) == 2, "two CTAs fit on an SM");
 };
 
 struct Source {
@@ -70,8 +73,7 @@ decode_kernel(const __grid_constant__ Params p, const __grid_constant__ Source s
     const uint32_t bars = ring + STAGES * C::STAGE_BYTES;            // full[S], empty[S], accum_full[2], accum_empty[2], drain, parts, rows requested, tmem slot
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ring_ptr + STAGES * C::STAGE_BYTES + 8 * (2 * STAGES + 7));
     float* slots = reinterpret_cast<float*>(ring_ptr + STAGES * C::STAGE_BYTES + 256);
-    float* exchange = slots + C::SLOTS / 4;
-    int* tiles = reinterpret_cast<int*>(exchange + C::EXCHANGE / 4);
+    int* tiles = reinterpret_cast<int*>(slots + C::SLOTS / 4);
     int* first = tiles + p.rows.groups + 1;
     auto full_bar = [&](int s) { return bars + 8u * s; };
     auto empty_bar = [&](int s) { return bars + 8u * (STAGES + s); };
@@ -335,7 +337,7 @@ decode_kernel(const __grid_constant__ Params p, const __grid_constant__ Source s
             if (lane == 0) mbar_arrive(accum_empty(a));
             if (split > 1) {
                 // a cluster works on one unit: parts are received once.  Part of CTA c for this quadrant: slot c, own one left out
-                float* mine = exchange + (q % quads) * 512;
+                float* mine = reinterpret_cast<float*>(first + p.rows.groups + 1) + (q % quads) * 512;
                 if (owner != rank) {
                     const int place = rank < owner ? rank : rank - 1;
                     const uint32_t to = map_to_rank(smem_u32(mine + place * quads * 512 + lane), (uint32_t)owner);
@@ -382,11 +384,11 @@ template <int DT, class F, int OUT>
 static int launch(const Params& p, const Source& src, int split, cudaStream_t st) {
     using C = Cfg<OUT == 5>;
     static bool attr_done[MAX_DEVICES] = {false};
-    const cudaError_t e = raise_smem_limit(decode_kernel<DT, F, OUT>, C::smem_bytes(MAX_GROUPS), attr_done);
+    const cudaError_t e = raise_smem_limit(decode_kernel<DT, F, OUT>, C::smem_bytes(MAX_GROUPS, 2), attr_done);
     if (e != cudaSuccess) { set_last_cuda_error(e); return MXQ_ELAUNCH; }
     const int64_t units = most_units(p.rows, p.N, FEATURES), room = 2 * sm_count();
     // a cluster works on one unit; without clusters the CTAs stay and walk over theirs
-    return launch_after(decode_kernel<DT, F, OUT>, (unsigned)(split > 1 ? units * split : units < room ? units : room), THREADS, C::smem_bytes(p.rows.groups),
+    return launch_after(decode_kernel<DT, F, OUT>, (unsigned)(split > 1 ? units * split : units < room ? units : room), THREADS, C::smem_bytes(p.rows.groups, split),
                         (unsigned)split, st, p, src, split);
 }
 
@@ -396,11 +398,12 @@ int decode_rows() { return decode::ROWS; }
 
 int launch_decode(const Params& p, int dt, const void* x, const void* row_index, int index64, int64_t rows_in, int eb, int fb, bool nibbles,
                   cudaStream_t st) {
-    // CTAs that share a unit: as many as the SMs hold (two each), the steps of K allow, and 4 at most (a lane quadrant each)
+    // CTAs that share a unit: as many as the SMs hold (two each, beside a large table one), the steps of K allow, and 4 at most (a lane quadrant each)
     const int64_t units = most_units(p.rows, p.N, decode::FEATURES);
     const int steps = (p.K + (nibbles ? 255 : 127)) / (nibbles ? 256 : 128);
     int split = 1;
-    while (split < 4 && units * split * 2 <= 2 * sm_count() && steps >= split * 2 * 4) split *= 2;
+    const int64_t room = (int64_t)sm_count() * (nibbles ? decode::Cfg<true>::per_sm(p.rows.groups, 2) : decode::Cfg<false>::per_sm(p.rows.groups, 2));
+    while (split < 4 && units * split * 2 <= room && steps >= split * 2 * 4) split *= 2;
     const decode::Source src{x, row_index, index64, rows_in};
     int rc = MXQ_ESIZE;
     with_row_format(eb, fb, nibbles, [&](auto fmt, auto out) {

@@ -153,3 +153,16 @@ def test_product_and_bias_alone(lib, dtype, M):
     check(alone, y, tol)
     check(layer(x), y, tol, "without an epilogue")
     assert math.isfinite(alone.double().abs().max().item())
+
+
+@pytest.mark.parametrize("groups", [351, 352, 1024])
+@pytest.mark.parametrize("K,few", [(1024, False), (1024, True), (160, False)])
+def test_many_groups_beside_the_ring(lib, groups, K, few):
+    """Group tables around the size where they and a cluster's exchange no longer fit twice beside the ring; ``few``: rows in two groups only,
+    so that clusters share units."""
+    counts = [(i * 5) % 3 for i in range(groups)] if not few else [0] * 7 + [3] + [0] * (groups - 9) + [16]
+    layer, wq, b, x = grouped_case(counts, 136, K, MXFP8_E4M3_fn, MXFP8_E4M3_fn)
+    first = [sum(counts[:i]) for i in range(groups)]
+    got = layer(x, offsets_of(counts), activation="silu")
+    G.check_status(DEV)
+    check(got, *grouped_expected(dequant(x, MXFP8_E4M3_fn), wq, b, first, counts, "silu", None, None, torch.bfloat16, torch.zeros_like(got)))
