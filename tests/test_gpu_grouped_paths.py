@@ -40,7 +40,7 @@ def test_pairs_of_ctas_over_ragged_groups(lib, pair, N, start):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("K", [2048, 4096])
-@pytest.mark.parametrize("M", [1, 7, 16])
+@pytest.mark.parametrize("M", [1, 7, 12, 16])
 def test_few_rows_in_four_bits_over_a_cluster(lib, dtype, K, M):
     layer, wq, b = linear_layer(520, K, OCP_MXFP4_E2M1, OCP_MXFP4_E2M1, dtype, bias=True)
     x, r = rand(M, K, dtype=dtype), rand(M, 520, dtype=dtype, seed=1)
@@ -100,7 +100,7 @@ def test_borders_through_the_quantiser_on_the_chip(lib, meta, dtype, K):
     tol = tol + (1 + torch.finfo(dtype).eps) * lost_by_halving(xq, wq)
     off = layer(aside, activation="relu")
     assert torch.equal(off.isnan(), bad[:, None].expand_as(off))
-    for rows in (slice(0, 16), slice(16, 32), slice(4, 5), slice(3, 12), slice(8, 9)):
+    for rows in (slice(0, 16), slice(16, 32), slice(0, 11), slice(11, 22), slice(22, 32), slice(4, 5), slice(8, 9)):
         got = layer(x[rows], activation="relu")
         assert torch.equal(got.isnan(), off[rows].isnan())
         check(torch.where(bad[rows, None], torch.zeros_like(got), got), y[rows], tol[rows], str(rows))
@@ -166,3 +166,31 @@ def test_many_groups_beside_the_ring(lib, groups, K, few):
     got = layer(x, offsets_of(counts), activation="silu")
     G.check_status(DEV)
     check(got, *grouped_expected(dequant(x, MXFP8_E4M3_fn), wq, b, first, counts, "silu", None, None, torch.bfloat16, torch.zeros_like(got)))
+
+
+@pytest.mark.parametrize("pair", [(MXFP8_E4M3_fn, OCP_MXFP6_E2M3, 1184), (MXFP8_E5M2_fn, MXFP8_E4M3_fn, 64), (OCP_MXFP4_E2M1, OCP_MXFP4_E2M1, 512)],
+                         ids=lambda p: f"{p[0].tag}-{p[1].tag}-{p[2]}")
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("N", [264, 129])
+def test_popular_groups_among_idle_ones(lib, pair, dtype, N):
+    """Few rows a group on average (one kernel), but groups of several tiles of 16 rows, the last one whole, of one row or of 15."""
+    x_meta, w_meta, K = pair
+    counts = [0, 32, 0, 0, 17, 1, 0, 47] + [0] * 60 + [16, 33] + [0] * 7
+    layer, wq, b, x = grouped_case(counts, N, K, x_meta, w_meta, dtype)
+    r = rand(sum(counts), N, dtype=dtype, seed=6)
+    got = layer(x, offsets_of(counts), activation="gelu", residual=r)
+    G.check_status(DEV)
+    first = [sum(counts[:i]) for i in range(len(counts))]
+    check(got, *grouped_expected(dequant(x, x_meta), wq, b, first, counts, "gelu", None, r, dtype, torch.zeros_like(r)))
+
+
+@pytest.mark.parametrize("meta", [MXFP8_E4M3_fn, OCP_MXFP4_E2M1], ids=lambda m: m.tag)
+@pytest.mark.parametrize("N", [512, 9600])
+def test_rows_around_the_choice_of_kernel(lib, meta, N):
+    """Row counts on both sides of where the choice falls, by the width and the operands' bits."""
+    layer, wq, b = linear_layer(N, 256, meta, meta, bias=True)
+    x, r = rand(18, 256), rand(18, N, seed=1)
+    y, tol = expected(dequant(x, meta), wq, b, "silu", None, r, torch.bfloat16)
+    for M in (4, 5, 6, 8, 9, 12, 13, 16, 17):
+        check(layer(x[:M], activation="silu", residual=r[:M]), y[:M], tol[:M], str(M))
+    G.check_status(DEV)
