@@ -575,18 +575,23 @@ struct Plan {
     int chunks() const { return shape <= NARROW ? 1 : 2; }
     int64_t sf_bytes(int64_t rows, int64_t groups, int64_t K) const { return tile_slots(rows, groups, width) * ((K + 127) / 128) * chunks() * 512; }
 };
-// Whether the kernel for few rows is the faster one.  There every CTA quantises the rows for its own features, some 60 ns a row and 128
-// elements, which from some 8 rows on takes longer than the weights' copies; a group's tiles of 16 rows each read its weights.
-// Narrow tiles have a second launch in front, and no split of K: they need N to fill the SMs.  Measured with cold weights, microseconds, few
-// rows / narrow tiles.  Linear, 4096 -> 14336: 15.0 / 15.4 (6 rows), 16.0 / 15.4 (8), 18.5 / 15.4 (10), 31.6 / 15.4 (16); 8192 -> 28672: 40.5 / 45.9 (8),
-// 50.8 / 45.9 (10); 14336 -> 4096: 28.6 / 33.1 (16); 4096 -> 4096: 13.3 / 13.4 (16).  4-bit pairs: 4096 -> 14336: 10.4 / 10.9 (4), 11.7 / 10.9 (6);
-// 8192 -> 28672: 26.7 / 27.8 (6), 31.9 / 27.8 (8); 14336 -> 4096: 18.9 / 20.8 (12), 21.4 / 20.8 (14).  64 experts, 2048 -> 1024, rows dealt evenly:
-// 26.1 / 29.4 (2 a group), 26.7 / 29.8 (4); by uneven popularity: 25.4 / 23.5 (2), 28.8 / 28.9 (3), 35.4 / 29.6 (4), 39.3 / 31.4 (8); 8 experts, 4096 -> 14336,
-// uneven: 65.4 / 71.1 (2), 69.4 / 71.2 (3), 76.3 / 71.3 (4).  (The host knows the average only.)
-static bool takes_few(int64_t rows, int64_t groups, int64_t N, bool fp4) {
-    if (groups > 1) return rows <= 2 * groups;
-    const bool fills = (N + 127) / 128 * 2 > sm_count();
-    return rows <= (fp4 ? (fills ? 5 : 12) : fills ? decode_rows() / 2 : decode_rows());
+// Whether the kernel for few rows is the faster one.  There every CTA quantises the rows for its own features, some 62 ns a row and 128
+// elements (`load`: that on every SM), which from some 8 rows on takes longer than the weights' copies; a group's tiles of 16 rows each
+// read its weights.  Narrow tiles have a second launch in front (calls from the host: 14.5 us against 9.5, while the GPU takes less), and no split
+// of K: they need N to fill the SMs.  Measured with cold weights, microseconds, few rows / narrow tiles:
+//   linear, 4096 -> 14336: 15.0 / 15.4 (6 rows), 16.0 / 15.4 (8), 18.5 / 15.4 (10), 31.6 / 15.4 (16); 8192 -> 28672: 40.5 / 45.9 (8), 50.8 / 45.9 (10);
+//     14336 -> 4096: 28.6 / 33.1 (16); 4096 -> 4096: 13.3 / 13.4 (16);
+//   4-bit pairs, 4096 -> 14336: 10.4 / 10.9 (4), 11.7 / 10.9 (6); 8192 -> 28672: 26.7 / 27.8 (6), 31.9 / 27.8 (8); 14336 -> 4096: 18.9 / 20.8 (12), 21.4 / 20.8 (14);
+//   64 experts, 2048 -> 1024, rows dealt evenly: 26.1 / 29.4 (2 a group), 26.7 / 29.8 (4); by uneven popularity: 25.4 / 23.5 (2), 28.8 / 28.9 (3),
+//     35.4 / 29.6 (4), 39.3 / 31.4 (8); 8 experts, 4096 -> 14336, uneven: 65.4 / 71.1 (2), 69.4 / 71.2 (3), 76.3 / 71.3 (4).  (The host knows the average only.)
+//   small ones, called from the host: linear, 1024 -> 14336: 11.7 / 14.4 (16 rows, load 6 us); 2048 -> 12288: 12.0 / 14.5 (12, 7.7 us), 17.9 / 14.5 (16, 10.3 us);
+//     uneven experts: 16 of 1024 -> 1024: 10.0 / 14.8 (3 a group, 1.3 us); 4 of 4096 -> 2048: 11.3 / 14.6 (3, 2.6 us), 17.8 / 14.6 (4, 3.4 us).
+static bool takes_few(int64_t rows, int64_t groups, int64_t N, int64_t K, bool fp4, int64_t sms) {
+    const int64_t ftiles = (N + 127) / 128;
+    const double load = (double)rows * (double)((K + 127) / 128) * (double)ftiles * 0.062 / (double)sms;          // microseconds
+    if (groups > 1) return rows <= 2 * groups || (rows / groups <= decode_rows() / 2 && load <= 2.5);
+    const bool fills = ftiles * 2 > sms;
+    return rows <= (load <= 8.0 ? decode_rows() : fp4 ? (fills ? 5 : 12) : fills ? decode_rows() / 2 : decode_rows());
 }
 // The tiles that take the fewest estimated nanoseconds of the whole GPU: rounds of tiles x steps of K x what a step takes.  That is
 // what one thread issues (215) at least; else, for one CTA, what L2 gives all SMs together (13.4 TB/s measured: 47.6 KB of a 240-row step in
@@ -594,9 +599,9 @@ static bool takes_few(int64_t rows, int64_t groups, int64_t N, bool fp4) {
 // cap, which large products run into).  Measured, microseconds, one CTA / pair: 8192 rows, 14336 x 4096: 570 / 570 (128 rows), 525 / 477 (192),
 // 482 / 458 (224); 192 rows, 4096 x 4096: 20.6 / 20.0 (64), 19.4 / 19.9 (128); 2048 rows, 2048 x 2048: 25.9 (128), 24.8 (240), 29.8 (pair, 240).
 // (One CTA with 256 x 240 has the pair's bytes, but fills tensor memory: its epilogue overlaps nothing, 544.)
-static Plan make_plan(int64_t rows, int64_t groups, int64_t N, int64_t K, bool fp4) {
-    if (takes_few(rows, groups, N, fp4)) return Plan{DECODE, Narrow::BT};
-    const int64_t sms = sm_count(), each = (rows + groups - 1) / groups, ftiles = (N + 127) / 128, steps = (K + (fp4 ? 255 : 127)) / (fp4 ? 256 : 128);
+static Plan make_plan(int64_t rows, int64_t groups, int64_t N, int64_t K, bool fp4, int64_t sms) {
+    if (takes_few(rows, groups, N, K, fp4, sms)) return Plan{DECODE, Narrow::BT};
+    const int64_t each = (rows + groups - 1) / groups, ftiles = (N + 127) / 128, steps = (K + (fp4 ? 255 : 127)) / (fp4 ? 256 : 128);
     Plan best{NARROW, 0};
     double least = 0.0;
     for (int ctas = 1; ctas <= 2; ++ctas)
@@ -646,13 +651,17 @@ static bool takes_decode(const grouped::Plan& plan, const void* x, int round_mod
     return plan.shape == grouped::DECODE && round_mode == MXQ_RN && reinterpret_cast<uintptr_t>(x) % 16 == 0;
 }
 
+static int64_t scratch_of(const grouped::Plan& plan, const void* x, int round_mode, int64_t rows_in, int64_t rows, int64_t K, int64_t groups) {
+    if (rows == 0 || takes_decode(plan, x, round_mode)) return 0;
+    return grouped::align256(rows * K) + grouped::align256(plan.sf_bytes(rows, groups, K)) + grouped::align256(rows_in * K) + grouped::align256(rows_in * K / 32);
+}
+
 extern "C" int64_t mxq_mx_grouped_scratch_bytes(const void* x, int round_mode, int64_t rows_in, int64_t rows, int64_t K, int64_t groups, int64_t N) {
     if (rows_in < 0 || rows < 0 || groups <= 0 || N <= 0 || K <= 0 || K % 32 != 0) return MXQ_EINVAL;
+    const int64_t sms = tc::sm_count();
     // whichever way the weight is packed
-    const grouped::Plan plan = grouped::make_plan(rows, groups, N, K, false), plan4 = grouped::make_plan(rows, groups, N, K, true);
-    if (rows == 0 || (takes_decode(plan, x, round_mode) && takes_decode(plan4, x, round_mode))) return 0;
-    const int64_t sf = std::max(plan.sf_bytes(rows, groups, K), plan4.sf_bytes(rows, groups, K));
-    return grouped::align256(rows * K) + grouped::align256(sf) + grouped::align256(rows_in * K) + grouped::align256(rows_in * K / 32);
+    return std::max(scratch_of(grouped::make_plan(rows, groups, N, K, false, sms), x, round_mode, rows_in, rows, K, groups),
+                    scratch_of(grouped::make_plan(rows, groups, N, K, true, sms), x, round_mode, rows_in, rows, K, groups));
 }
 
 extern "C" int mxq_mx_grouped_linear(const mxq_grouped_linear_args* args) {
@@ -669,9 +678,6 @@ extern "C" int mxq_mx_grouped_linear(const mxq_grouped_linear_args* args) {
     if (rows == 0) return MXQ_OK;
     if ((!x && rows_in > 0) || !w_packed || !out || (extra_mode != MXQ_EXTRA_NONE && !extra)) return MXQ_EINVAL;
     if (reinterpret_cast<uintptr_t>(w_packed) % 16 != 0 || reinterpret_cast<uintptr_t>(scratch) % 256 != 0) return MXQ_EINVAL;
-    const int64_t needed = mxq_mx_grouped_scratch_bytes(x, x_round_mode, rows_in, rows, K, groups, N);
-    if (needed > 0 && !scratch) return MXQ_EINVAL;
-    if (scratch_bytes < needed) return MXQ_ESIZE;
     // both operands E2M1 and the weight kept as nibbles: the 4-bit kind
     const bool x_e2m1 = x_exp_bits == 2 && x_frac_bits == 1;
     const bool fp4 = w_hw_format == 5;
@@ -680,7 +686,10 @@ extern "C" int mxq_mx_grouped_linear(const mxq_grouped_linear_args* args) {
     if (!grouped::valid_mx_preset(x_exp_bits, x_frac_bits) || x_round_mode < MXQ_RN || x_round_mode > MXQ_RZ) return MXQ_EINVAL;
     const int x_fmt = x_exp_bits == 5 ? 1 : 0;
 
-    const grouped::Plan plan = grouped::make_plan(rows, groups, N, K, fp4);
+    const grouped::Plan plan = grouped::make_plan(rows, groups, N, K, fp4, tc::sm_count());
+    const int64_t needed = scratch_of(plan, x, x_round_mode, rows_in, rows, K, groups);
+    if (needed > 0 && !scratch) return MXQ_EINVAL;
+    if (scratch_bytes < needed) return MXQ_ESIZE;
     grouped::Params p{};
     p.w = w_packed;
     p.w_group = fp4 ? grouped::WeightTile<true>::group_bytes(N, K) : grouped::WeightTile<false>::group_bytes(N, K);

@@ -185,11 +185,11 @@ def test_popular_groups_among_idle_ones(lib, pair, dtype, N):
 
 
 @pytest.mark.parametrize("meta", [MXFP8_E4M3_fn, OCP_MXFP4_E2M1], ids=lambda m: m.tag)
-@pytest.mark.parametrize("N", [512, 9600])
-def test_rows_around_the_choice_of_kernel(lib, meta, N):
-    """Row counts on both sides of where the choice falls, by the width and the operands' bits."""
-    layer, wq, b = linear_layer(N, 256, meta, meta, bias=True)
-    x, r = rand(18, 256), rand(18, N, seed=1)
+@pytest.mark.parametrize("N,K", [(512, 256), (9600, 256), (9600, 4096), (4096, 8192)])
+def test_rows_around_the_choice_of_kernel(lib, meta, N, K):
+    """Row counts on both sides of where the choice falls, by the sizes and the operands' bits."""
+    layer, wq, b = linear_layer(N, K, meta, meta, bias=True)
+    x, r = rand(18, K), rand(18, N, seed=1)
     y, tol = expected(dequant(x, meta), wq, b, "silu", None, r, torch.bfloat16)
     for M in (4, 5, 6, 8, 9, 12, 13, 16, 17):
         check(layer(x[:M], activation="silu", residual=r[:M]), y[:M], tol[:M], str(M))
