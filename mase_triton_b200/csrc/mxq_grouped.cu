@@ -20,8 +20,9 @@
 //   rows:    codes [rows, K], scales [tile slot][ceil(K / 128)][chunks][512] bytes.  With tiles of at most `width` rows, tile t of a
 //            group that begins at row f has slot f / width + group + t: no two tiles share one, and no sum over the groups before is needed.
 //
-// Measured (replays in a row, quantiser included): 8192 rows, 4096 -> 14336, E4M3, silu and multiplier: 441 us, 2.2 PFLOP/s under the power cap;
-// 192 rows, 4096 -> 4096: 19.1 us, of which the products are 32 steps at the issue rate; 8192 rows over 32 experts, 2048 -> 2048, E2M1: 65 us.
+// Measured (replays in a row, quantiser included): 8192 rows, 4096 -> 14336, E4M3, silu and multiplier: 460 to 480 us for the first calls, 515 to 540 us run for
+// seconds (1.8 PFLOP/s at 1.37 GHz under the power cap; the tensor pipe is active for 54 % of the cycles, what idles it for the rest is not known);
+// 192 rows, 4096 -> 4096: 19.1 us; 8192 rows over 32 experts, 2048 -> 2048, E2M1: 65 us.
 #include <algorithm>
 
 #include "mxq_grouped.cuh"
@@ -599,6 +600,9 @@ static bool takes_few(int64_t rows, int64_t groups, int64_t N, int64_t K, bool f
 // cap, which large products run into).  Measured, microseconds, one CTA / pair: 8192 rows, 14336 x 4096: 570 / 570 (128 rows), 525 / 477 (192),
 // 482 / 458 (224); 192 rows, 4096 x 4096: 20.6 / 20.0 (64), 19.4 / 19.9 (128); 2048 rows, 2048 x 2048: 25.9 (128), 24.8 (240), 29.8 (pair, 240).
 // (One CTA with 256 x 240 has the pair's bytes, but fills tensor memory: its epilogue overlaps nothing, 544.)
+// The estimate ranks tiles of one problem and no more: it counts steps of K and no epilogue, with constants of 8-bit products, and lies below the
+// kernel's time where K is short or operands have four bits.  Estimate / kernel alone, microseconds: 192 rows, 4096 x 4096: 6.9 / 17.7; 3001 rows
+// over 17 experts, 520 x 1184: 2.6 / 17.2; 4-bit pairs, 4096 x 4096 x 4096: 34 / 41, 8192 rows over 32 experts, 2048 x 2048: 19 / 48.
 static Plan make_plan(int64_t rows, int64_t groups, int64_t N, int64_t K, bool fp4, int64_t sms) {
     if (takes_few(rows, groups, N, K, fp4, sms)) return Plan{DECODE, Narrow::BT};
     const int64_t each = (rows + groups - 1) / groups, ftiles = (N + 127) / 128, steps = (K + (fp4 ? 255 : 127)) / (fp4 ? 256 : 128);

@@ -12,9 +12,10 @@
 //     partial sums go to the CTA that finishes those features through distributed shared memory and are added in the
 //     order of the CTAs, so that results do not depend on which comes first.
 // The layout of weights, the walk over the units and the epilogue are those of mxq_grouped.cu.
-// Measured (replays in a row): 1 row, 4096 -> 14336, E4M3: 15.1 us (4.0 TB/s of all bytes; 9.3 at the copy rate); 2 rows over 8 such
-// experts: 24.0 (5.0 TB/s); 256 rows over 64 experts, 2048 -> 1024: 32.4 (4.3 TB/s).  CTAs of one unit each in the hardware's order instead of
-// CTAs that stay: 36.0; weights held back until the first rows have arrived, not just been asked for: 33.6.
+// Measured (replays in a row): 1 row, 4096 -> 14336, E4M3: 14.1 us (4.3 TB/s of all bytes; 9.3 at the copy rate); 2 rows over 8 such
+// experts: 23.6 (5.1 TB/s); 5 rows, 14336 -> 4096, E3M2: 16.4.  256 rows over 64 experts, 2048 -> 1024 (which narrow tiles take by now, in 30.6): 32.4; there
+// CTAs of one unit each in the hardware's order instead of CTAs that stay: 36.0; weights held back until the first rows have arrived, not
+// just been asked for: 33.6.
 #include "mxq_grouped.cuh"
 
 namespace mxq {
